@@ -1,0 +1,61 @@
+// What decode and prefill over packed pages share: the tile of 32 keys that
+// one wave scores and accumulates.
+//
+// Both products run on the 16x16x32 matrix instruction with the keys in its
+// rows and up to 16 query rows (heads of a group, or (token, head) pairs) in
+// its columns:
+//   S^T[key, row]  = sum_d K[key, d] Q[row, d]
+//   O^T[d, row]    = sum_key V[key, d] P[row, key]
+// The result layout of the first (lane: column lane % 16, rows 4 * (lane / 16)
+// .. + 3) holds for each lane 4 keys of its own query row, and two such
+// results are 8 keys: exactly the lane's part of the second product's operand
+// when both operands number the keys of a tile as
+//   k = 8 * g + j  ->  key 4 * g + j (j < 4), 16 + 4 * g + j - 4 (j >= 4)
+// So probabilities never leave their lane.  V^T comes from row-major fp16 rows
+// in LDS by transposing reads (4 keys of 16 dims per 16 lanes and read).
+#pragma once
+
+#include "fp4_cache.h"
+
+namespace mvme {
+namespace fp4 {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Probabilities are exp2(x - reference) with the reference kept 8 below the
+// largest score seen when it was set, and moved when a score passes it by 14:
+// fp16 then holds every probability down to 2^-24 - 8 of the largest with
+// full 11 bits from 2^-22 on, and none overflows.
+constexpr float kRefBelow = 8.f;
+constexpr float kRefSlack = 14.f;
+constexpr float kRefNone = -3.0e38f;  // no score yet: below every finite one
+
+constexpr int kTileKeys = 32;
+
+// Byte address inside a tile of rows of 2 * D bytes: 16-byte chunks are
+// XORed with the row, so that 16 rows of one chunk fall into different banks
+// (both for writes of whole rows and for transposing reads).
+template <int D>
+struct TileLayout {
+    static constexpr int kChunks = D / 8;
+    static constexpr int kMask = (kChunks & -kChunks) < 16 ? (kChunks & -kChunks) - 1 : 15;
+    __device__ static inline int at(int row, int chunk) { return row * 2 * D + ((chunk ^ (row & kMask)) << 4); }
+};
+
+// 16 dims of 8 keys for the value product: A operand of dims 16 n .. 16 n + 15.
+// `base` is the tile, rows in fp16.
+template <int D>
+__device__ inline u32x4 value_operand(const uint8_t* base, int n, int first_row) {
+    const int lane = __lane_id(), r = lane & 15, g = lane >> 4;
+    const int row = first_row + 4 * g + (r >> 2);
+    const int at = TileLayout<D>::at(row, 2 * n + ((r & 3) >> 1)) + (r & 1) * 8;
+    const int at2 = TileLayout<D>::at(row + 16, 2 * n + ((r & 3) >> 1)) + (r & 1) * 8;
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(base + at));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(base + at2));
+    const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+    return u32x4{x[0], x[1], y[0], y[1]};
+}
+
+}  // namespace fp4
+}  // namespace mvme

@@ -1,0 +1,446 @@
+// Ragged chunked prefill over packed 4-bit pages.
+//
+// The query rows of one sequence and kv head are its (token, head of the
+// group) pairs, numbered token-major, so that any group size fills the tiles.
+// A work-group takes 128 of them, 32 per wave, and one chunk of the keys.
+// Tiles of 64 keys are unpacked once into LDS (keys in the query's type,
+// values in fp16) and used by all rows.  Chunks of split calls are joined by a
+// second kernel.
+#include "fp4_attention.h"
+
+namespace mvme {
+namespace fp4 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRows = 128;   // query rows of a work-group
+constexpr int kKeys = 64;    // keys of a tile
+
+struct PrefillArgs {
+    void* out;
+    const void* q;
+    const uint8_t* key;
+    const uint8_t* value;
+    const int64_t* cu;
+    const int64_t* starts;
+    const int64_t* tables;
+    const int64_t* lens;
+    float* partial;  // [total_tokens, q_heads, chunks, D], then [total_tokens, q_heads, chunks, 2]
+    int64_t stats;
+    int64_t num_blocks, record, total_tokens;
+    int num_seqs, kv_heads, q_heads, group, width;
+    int items;       // work-groups per kv head and chunk; the last one clears rows that no sequence owns
+    int chunks, chunk_len;
+    BlockDiv div;
+    float scale;     // log2(e) / sqrt(D)
+};
+
+template <int D>
+struct Shape {
+    static constexpr int kChunks = D / 32;
+    static constexpr int kPer = D % 128 == 0 ? 4 : D == 64 || D == 192 ? 2 : 1;
+    static constexpr int kScales = kChunks / kPer;
+    static constexpr int kDimTiles = D / 16;
+    static constexpr int kMinWaves = D <= 128 ? 2 : 1;
+};
+
+struct Seq {
+    int64_t row0, rows, start, len;
+};
+__device__ inline Seq sequence(const PrefillArgs& a, int s) {
+    const int64_t lo = min(max(a.cu[s], (int64_t)0), a.total_tokens);
+    const int64_t hi = min(max(a.cu[s + 1], lo), a.total_tokens);
+    return {lo, hi - lo, a.starts[s], a.lens[s]};
+}
+// Keys that a sequence's rows may see: none where its start or length cannot be.
+__device__ inline int64_t usable_keys(const PrefillArgs& a, const Seq& q) {
+    const int64_t capacity = (int64_t)a.width * a.div.size;
+    return q.start < 0 || q.start >= q.len || q.len > capacity ? 0 : q.len;
+}
+
+template <typename T, int D>
+__device__ inline void store4(const PrefillArgs& a, int64_t head, int d, f32x4 v) {
+    u32x2 w = {T::pack(v[0], v[1]), T::pack(v[2], v[3])};
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + head * D + d) = w;
+}
+
+// Rows before the first and behind the last sequence: zeros.
+template <int D>
+__device__ void clear_rows(const PrefillArgs& a, int kv_head) {
+    const int64_t first = min(max(a.cu[0], (int64_t)0), a.total_tokens);
+    const int64_t last = min(max(a.cu[a.num_seqs], first), a.total_tokens);
+    const int64_t width = (int64_t)a.group * D;
+    const int64_t count = (first + a.total_tokens - last) * width;
+    for (int64_t i = threadIdx.x; i < count; i += kThreads) {
+        const int64_t n = i / width, token = n < first ? n : last + n - first;
+        static_cast<uint16_t*>(a.out)[(token * a.q_heads + (int64_t)kv_head * a.group) * D + i % width] = 0;
+    }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_kernel(PrefillArgs a) {
+    using S = Shape<D>;
+    __shared__ __attribute__((aligned(16))) uint8_t keys[kKeys * 2 * D];
+    __shared__ __attribute__((aligned(16))) uint8_t values[kKeys * 2 * D];
+    __shared__ uint8_t present[kKeys];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int kv_head = blockIdx.x % a.kv_heads, chunk = blockIdx.x / a.kv_heads % a.chunks;
+    int item = blockIdx.x / a.kv_heads / a.chunks;
+    if (item == a.items - 1) {
+        if (chunk == 0) clear_rows<D>(a, kv_head);
+        return;
+    }
+    // The sequence and the row block that `item` is.
+    Seq seq;
+    int s = 0;
+    for (;; ++s) {
+        if (s == a.num_seqs) return;
+        seq = sequence(a, s);
+        const int64_t blocks = (seq.rows * a.group + kRows - 1) / kRows;
+        if (item < blocks) break;
+        item -= (int)blocks;
+    }
+    const int64_t usable = usable_keys(a, seq);
+    const int64_t row0 = (int64_t)item * kRows, rows = seq.rows * a.group;
+    // Keys of this work-group: up to the last row's position, in its chunk.
+    const int64_t last_token = (min(row0 + kRows, rows) - 1) / a.group;
+    const int64_t first_pos = seq.start + row0 / a.group;
+    const uint32_t key_end = (uint32_t)min(usable, max(seq.start + last_token + 1, (int64_t)0));
+    const uint32_t begin = (uint32_t)chunk * a.chunk_len;
+    const uint32_t end = min(key_end, begin + (uint32_t)a.chunk_len);
+    if (chunk > 0 && begin >= end) return;
+
+    // This lane's rows: column r of two blocks of 16.
+    int64_t head[2];
+    int32_t limit[2];  // last visible key, -1 for rows without any
+    u32x4 q[2][S::kChunks];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int64_t row = row0 + wave * 32 + c * 16 + r;
+        const bool live = row < rows;
+        const int64_t token = live ? row / a.group : 0;
+        const int64_t pos = seq.start + token;
+        limit[c] = live && pos < usable ? (int32_t)pos : -1;
+        head[c] = live ? (seq.row0 + token) * a.q_heads + (int64_t)kv_head * a.group + row % a.group : -1;
+#pragma unroll
+        for (int i = 0; i < S::kChunks; ++i)
+            q[c][i] = live ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + head[c] * D +
+                                                             g * (D / 4) + 8 * i)
+                           : u32x4{0u, 0u, 0u, 0u};
+    }
+    f32x4 acc[2][S::kDimTiles];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int n = 0; n < S::kDimTiles; ++n) acc[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float ref[2] = {kRefNone, kRefNone}, sum[2] = {0.f, 0.f};
+    const int64_t* table = a.tables + (int64_t)s * a.width;
+
+    for (uint32_t t0 = begin; t0 < end; t0 += kKeys) {
+        __syncthreads();  // the last tile has been read
+        {
+            const int row = threadIdx.x >> 2, part = threadIdx.x & 3;
+            const uint32_t token = t0 + row;
+            uint32_t codes[2][S::kChunks], scales[2][S::kScales];
+            bool there = token < end;
+            if (there) {
+                const uint32_t block = a.div.page(token);
+                const int64_t page = table[block];
+                there = page >= 0 && page < a.num_blocks;
+                if (there) {
+                    const uint32_t place = token - block * a.div.size;
+                    const int64_t at = (page * a.kv_heads + kv_head) * a.record;
+#pragma unroll
+                    for (int plane = 0; plane < 2; ++plane) {
+                        const uint8_t* record = (plane ? a.value : a.key) + at;
+                        const uint8_t* from = record + place * (D / 2) + part * (D / 8);
+#pragma unroll
+                        for (int i = 0; i < S::kChunks; ++i)
+                            codes[plane][i] = reinterpret_cast<const uint32_t*>(from)[i];
+#pragma unroll
+                        for (int i = 0; i < S::kScales; ++i)
+                            scales[plane][i] = record[a.div.size * (D / 2) + place * (D / kBlockDims) +
+                                                      (part * (D / 4) + 8 * i * S::kPer) / kBlockDims];
+                    }
+                }
+            }
+            if (!there) {
+#pragma unroll
+                for (int plane = 0; plane < 2; ++plane) {
+#pragma unroll
+                    for (int i = 0; i < S::kChunks; ++i) codes[plane][i] = 0u;
+#pragma unroll
+                    for (int i = 0; i < S::kScales; ++i) scales[plane][i] = 127u;
+                }
+            }
+            // A NaN block of the values must not reach rows that do not see its key, as 0 * NaN would: it is staged as
+            // zeros, and the key's score is NaN instead.
+            bool nan = false;
+#pragma unroll
+            for (int i = 0; i < S::kScales; ++i) {
+                nan |= scales[1][i] == 255u;
+                scales[1][i] = scales[1][i] == 255u ? 0u : scales[1][i];
+            }
+            nan = (__ballot(nan) >> (lane & ~3)) & 15;
+            if (part == 0) present[row] = there ? nan ? 2 : 1 : 0;
+#pragma unroll
+            for (int i = 0; i < S::kChunks; ++i) {
+                const int at = TileLayout<D>::at(row, part * S::kChunks + i);
+                *reinterpret_cast<u32x4*>(keys + at) = values_of<T>(codes[0][i], scale_of(scales[0][i / S::kPer]));
+                *reinterpret_cast<u32x4*>(values + at) = values_of<Half>(codes[1][i], scale_of(scales[1][i / S::kPer]));
+            }
+        }
+        __syncthreads();
+        float x[2][16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
+#pragma unroll
+            for (int i = 0; i < S::kChunks; ++i) {
+                const u32x4 kt = *reinterpret_cast<const u32x4*>(
+                    keys + TileLayout<D>::at(16 * k + r, g * S::kChunks + i));
+                c0 = T::mfma16x16x32(kt, q[0][i], c0);
+                c1 = T::mfma16x16x32(kt, q[1][i], c1);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[0][4 * k + j] = c0[j] * a.scale;
+                x[1][4 * k + j] = c1[j] * a.scale;
+            }
+        }
+        const int state = present[lane];
+        const uint64_t mask = __ballot(state != 0), nans = __ballot(state == 2);
+        if (nans) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if ((nans >> (16 * (k >> 2) + 4 * g + (k & 3))) & 1) x[0][k] = x[1][k] = __builtin_nanf("");
+        }
+        if (mask != ~uint64_t(0) || (int64_t)t0 + kKeys - 1 > first_pos) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int key = 16 * k + 4 * g + j;
+                    const bool there = (mask >> key) & 1;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        if (!there || (int32_t)(t0 + key) > limit[c]) x[c][4 * k + j] = kNegInf;
+                }
+        }
+        u32x4 weights[2][2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float top = x[c][0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) top = fmaxf(top, x[c][j]);
+            top = row4_max(top);
+            if (__any(top > ref[c] + kRefSlack)) {
+                const float moved = top > ref[c] + kRefSlack ? top - kRefBelow : ref[c];
+                const float by = fast_exp2(ref[c] - moved);
+                ref[c] = moved;
+                sum[c] *= by;
+#pragma unroll
+                for (int n = 0; n < S::kDimTiles; ++n) acc[c][n] *= by;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                x[c][j] = fast_exp2(x[c][j] - ref[c]);
+                sum[c] += x[c][j];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) weights[c][h][j] = Half::pack(x[c][8 * h + 2 * j], x[c][8 * h + 2 * j + 1]);
+        }
+#pragma unroll
+        for (int n = 0; n < S::kDimTiles; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const u32x4 vt = value_operand<D>(values, n, 32 * h);
+                acc[0][n] = Half::mfma16x16x32(vt, weights[0][h], acc[0][n]);
+                acc[1][n] = Half::mfma16x16x32(vt, weights[1][h], acc[1][n]);
+            }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const float total = row4_sum(sum[c]);
+        if (head[c] < 0) continue;
+        if (a.chunks == 1) {
+            const float by = 1.f / total;
+            const bool zero = limit[c] < 0 || total == 0.f;  // a row that sees no key
+#pragma unroll
+            for (int n = 0; n < S::kDimTiles; ++n)
+                store4<T, D>(a, head[c], 16 * n + 4 * g, zero ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[c][n] * by);
+        } else {
+            const int64_t at = head[c] * a.chunks + chunk;
+#pragma unroll
+            for (int n = 0; n < S::kDimTiles; ++n)
+                *reinterpret_cast<f32x4*>(a.partial + at * D + 16 * n + 4 * g) = acc[c][n];
+            if (g == 0) {
+                a.partial[a.stats + at * 2] = ref[c];
+                a.partial[a.stats + at * 2 + 1] = total;
+            }
+        }
+    }
+}
+
+// Joins the key chunks of one packed row and query head.
+template <typename T, int D>
+__global__ __launch_bounds__(64) void fp4_prefill_merge_kernel(PrefillArgs a) {
+    const int64_t head = blockIdx.x, token = head / a.q_heads;
+    int lo = 0, hi = a.num_seqs;  // the first sequence that ends behind the row
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (a.cu[mid + 1] <= token) lo = mid + 1;
+        else hi = mid;
+    }
+    if (lo == a.num_seqs || token < a.cu[lo]) return;  // no sequence's row: cleared by the first kernel
+    const Seq seq = sequence(a, lo);
+    const int64_t pos = seq.start + token - seq.row0;
+    const int chunks = pos < usable_keys(a, seq) ? (int)(pos / a.chunk_len) + 1 : 0;
+    const float* stats = a.partial + a.stats + head * a.chunks * 2;
+    const float* partial = a.partial + head * a.chunks * D;
+    float top = kRefNone;
+    for (int c = 0; c < chunks; ++c) top = fmaxf(top, stats[2 * c]);
+    for (int d = threadIdx.x; d < D; d += 64) {
+        float total = 0.f, value = 0.f;
+        for (int c = 0; c < chunks; ++c) {
+            const float by = fast_exp2(stats[2 * c] - top);
+            total += by * stats[2 * c + 1];
+            value += by * partial[(int64_t)c * D + d];
+        }
+        static_cast<uint16_t*>(a.out)[head * D + d] = T::from_float(total != 0.f ? value / total : 0.f);
+    }
+}
+
+bool attention_dim(int64_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
+
+bool prefill_shape(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                   int64_t block_size, int64_t width) {
+    return num_seqs > 0 && num_seqs <= 2147483647 / 2 && total >= 0 && q_heads > 0 && kv_heads > 0 &&
+           q_heads % kv_heads == 0 && attention_dim(head_dim) && valid_format(block_size, head_dim) && width > 0 &&
+           width <= kMaxCapacity / block_size && q_heads <= 2147483647 / head_dim &&
+           total <= 2147483647 / (q_heads);
+}
+
+struct Plan {
+    int64_t items, chunks, chunk_len;
+};
+
+Plan plan(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, int64_t block_size, int64_t width,
+          int64_t chunk_tokens) {
+    const int64_t capacity = block_size * width, group = q_heads / kv_heads;
+    // Row blocks: full ones, at most one partial per sequence, and the one that clears.
+    const int64_t items = total * group / kRows + num_seqs + 1;
+    int64_t len = capacity;
+    if (chunk_tokens > 0) {
+        len = chunk_tokens;
+    } else if (items * kv_heads < 512) {
+        const int64_t want = 512 / (items * kv_heads) + 1;
+        len = (capacity + want - 1) / want;
+        if (len < 256) len = 256;
+    }
+    if (len > capacity) len = capacity;
+    len = (len + kKeys - 1) / kKeys * kKeys;
+    return {items, (capacity - 1) / len + 1, len};
+}
+
+template <typename T, int D>
+int launch(const PrefillArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((fp4_prefill_kernel<T, D>), dim3((unsigned)((int64_t)a.items * a.chunks * a.kv_heads)),
+                       dim3(kThreads), 0, s, a);
+    if (int rc = check_launch("packed prefill")) return rc;
+    if (a.chunks == 1) return MVME_OK;
+    hipLaunchKernelGGL((fp4_prefill_merge_kernel<T, D>), dim3((unsigned)(a.total_tokens * a.q_heads)), dim3(64), 0, s,
+                       a);
+    return check_launch("packed prefill merge");
+}
+
+template <typename T>
+int launch_dim(const PrefillArgs& a, int64_t head_dim, hipStream_t s) {
+    switch (head_dim) {
+        case 32: return launch<T, 32>(a, s);
+        case 64: return launch<T, 64>(a, s);
+        case 96: return launch<T, 96>(a, s);
+        case 128: return launch<T, 128>(a, s);
+        case 192: return launch<T, 192>(a, s);
+        default: return launch<T, 256>(a, s);
+    }
+}
+
+}  // namespace
+}  // namespace fp4
+}  // namespace mvme
+
+using namespace mvme;
+using namespace mvme::fp4;
+
+extern "C" size_t mvme_fp4_paged_prefill_workspace_size(int64_t num_seqs, int64_t total_tokens, int64_t q_heads,
+                                                        int64_t kv_heads, int64_t head_dim, int64_t block_size,
+                                                        int64_t table_width, int64_t chunk_tokens) {
+    if (!prefill_shape(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width)) return 0;
+    const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, block_size, table_width, chunk_tokens);
+    return p.chunks == 1 ? 0
+                         : (size_t)(total_tokens * q_heads) * (size_t)p.chunks * (size_t)(head_dim + 2) * sizeof(float);
+}
+
+extern "C" int mvme_fp4_paged_prefill_attention(void* out, const void* q, const void* key_cache,
+                                                const void* value_cache, const int64_t* cu_seqlens_q,
+                                                const int64_t* query_starts, const int64_t* block_tables,
+                                                const int64_t* context_lens, int64_t num_seqs, int64_t total_tokens,
+                                                int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                int64_t num_blocks, int64_t block_size, int64_t table_width,
+                                                int64_t chunk_tokens, int dtype, void* workspace,
+                                                size_t workspace_bytes, void* stream) {
+    if (!valid_dtype(dtype)) return fail(MVME_EINVAL, "FP16/BF16 required");
+    if (num_seqs <= 0 || total_tokens < 0 || q_heads <= 0 || kv_heads <= 0 || num_blocks <= 0)
+        return fail(MVME_EINVAL, "empty batch/heads/cache");
+    if (q_heads % kv_heads != 0) return fail(MVME_EINVAL, "head dimension or GQA mismatch");
+    if (!attention_dim(head_dim)) return fail(MVME_EINVAL, "supported head_dim: 32,64,96,128,192,256");
+    if (block_size <= 0 || table_width <= 0) return fail(MVME_EINVAL, "invalid block table");
+    if (block_size > kMaxCapacity || table_width > kMaxCapacity / block_size)
+        return fail(MVME_EINVAL, "maximum table capacity is 1M tokens");
+    if (!prefill_shape(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width))
+        return fail(MVME_EINVAL, "too many packed query rows");
+    const int64_t record = record_bytes(block_size, head_dim);
+    if (num_blocks > (int64_t(1) << 62) / record / kv_heads) return fail(MVME_EINVAL, "KV cache too large");
+    if (chunk_tokens < 0) return fail(MVME_EINVAL, "chunk_tokens must not be negative");
+    if (total_tokens == 0) return MVME_OK;
+    if (!out || !q || !key_cache || !value_cache || !cu_seqlens_q || !query_starts || !block_tables || !context_lens)
+        return fail(MVME_EINVAL, "packed prefill: null pointer");
+    if (!aligned(q, 16) || !aligned(key_cache, 16) || !aligned(value_cache, 16) || !aligned(out, 8))
+        return fail(MVME_EINVAL, "packed prefill: queries and caches must be 16-byte, the output 8-byte aligned");
+    const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, block_size, table_width, chunk_tokens);
+    if (p.chunks > 2147483647 / kv_heads / p.items) return fail(MVME_EINVAL, "too many packed query rows");
+    const size_t need = mvme_fp4_paged_prefill_workspace_size(num_seqs, total_tokens, q_heads, kv_heads, head_dim,
+                                                              block_size, table_width, chunk_tokens);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+        return fail(MVME_EWORKSPACE, "packed prefill workspace too small: " + std::to_string(need) +
+                                         " bytes, 16-byte aligned, are needed");
+    PrefillArgs a{};
+    a.out = out;
+    a.q = q;
+    a.key = static_cast<const uint8_t*>(key_cache);
+    a.value = static_cast<const uint8_t*>(value_cache);
+    a.cu = cu_seqlens_q;
+    a.starts = query_starts;
+    a.tables = block_tables;
+    a.lens = context_lens;
+    a.partial = static_cast<float*>(workspace);
+    a.stats = total_tokens * q_heads * p.chunks * head_dim;
+    a.num_blocks = num_blocks;
+    a.record = record;
+    a.total_tokens = total_tokens;
+    a.num_seqs = (int)num_seqs;
+    a.kv_heads = (int)kv_heads;
+    a.q_heads = (int)q_heads;
+    a.group = (int)(q_heads / kv_heads);
+    a.width = (int)table_width;
+    a.items = (int)p.items;
+    a.chunks = (int)p.chunks;
+    a.chunk_len = (int)p.chunk_len;
+    a.div = make_block_div(block_size);
+    a.scale = kLog2e / __builtin_sqrtf((float)head_dim);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == MVME_FP16 ? launch_dim<Half>(a, head_dim, s) : launch_dim<BFloat16>(a, head_dim, s);
+}

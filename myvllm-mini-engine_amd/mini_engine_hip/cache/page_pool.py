@@ -8,6 +8,10 @@ their tables (refcount = number of holders), and a request can be given
 retained pages only (``attach``, block_manager.py:83-97 — the prefix cache's
 whole-prompt hit, prefix_cache.py:45-48), so its table holds no private
 page at all.  Host-side only.
+
+``fork``, ``make_writable`` and ``compact`` return the page copies that have
+to follow on the device, as (source, destination) pairs: ``copy_pages`` and
+``compact_pages`` of the cache pools run them.
 """
 
 from __future__ import annotations
@@ -82,6 +86,62 @@ class PagePool:
             self._refs[page] += 1
         self._owned[request_id] = pages
         return list(pages)
+
+    def fork(self, request_id: str, new_request: str, token_count: int):
+        """Give ``new_request`` the first ``token_count`` tokens of a request.
+
+        Whole pages are shared; a partly written last page is copied, since both
+        requests write on behind it.  Returns (the new table, page copies).
+        """
+        if new_request in self._owned:
+            raise ValueError(f"request already owns blocks: {new_request}")
+        table = self._owned[request_id]
+        if not 0 <= token_count <= len(table) * self.block_size:
+            raise ValueError("fork passes the request's pages")
+        whole, rest = divmod(token_count, self.block_size)
+        copy = self._take(1 if rest else 0)
+        for page in table[:whole]:
+            self._refs[page] += 1
+        self._owned[new_request] = table[:whole] + copy
+        return list(self._owned[new_request]), [(table[whole], page) for page in copy]
+
+    def make_writable(self, request_id: str, index: int):
+        """Before writing into page ``index`` of a table: a page that others hold too is replaced by a copy.
+
+        Returns (the page to write, page copies).
+        """
+        table = self._owned[request_id]
+        if not 0 <= index < len(table):
+            raise IndexError("page index out of range")
+        page = table[index]
+        if self._refs[page] == 1:
+            return page, []
+        (copy,) = self._take(1)
+        self._release(page)
+        table[index] = copy
+        return copy, [(page, copy)]
+
+    def compact(self):
+        """Move live pages down into free lower ones, and renumber every table.
+
+        Returns the moves, sources rising; no page is both source and
+        destination.  Pages pinned from outside stay, since whoever pinned them
+        goes by their number.  Until the moves have run on the device, and the
+        device's block tables have been renumbered, nothing may be written.
+        """
+        held = [0] * self.num_blocks
+        for table in self._owned.values():
+            for page in table:
+                held[page] += 1
+        movable = [p for p in range(self.num_blocks - 1, -1, -1) if self._refs[p] and self._refs[p] == held[p]]
+        moves = [(src, dst) for src, dst in zip(movable, sorted(self._free)) if dst < src]
+        number = dict(moves)
+        for src, dst in moves:
+            self._refs[dst], self._refs[src] = self._refs[src], 0
+        for table in self._owned.values():
+            table[:] = [number.get(page, page) for page in table]
+        self._free = [p for p in range(self.num_blocks - 1, -1, -1) if not self._refs[p]]  # the lowest goes out first
+        return moves[::-1]
 
     def pin(self, pages) -> None:
         """Hold one external reference (e.g. a prefix-cache entry)."""

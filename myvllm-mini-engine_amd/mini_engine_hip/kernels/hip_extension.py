@@ -57,6 +57,22 @@ SIGNATURES = {
     "mvme_linear_rows": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp]),
 }
 
+# The packed 4-bit cache and the page operators; mirrors include/mvme_fp4.h.
+PACKED_SIGNATURES = {
+    "mvme_fp4_record_bytes": (_i64, [_i64, _i64]),
+    "mvme_fp4_write_slots": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "mvme_fp4_write_batch": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64,
+                                    _int, _vp]),
+    "mvme_fp4_gather_slots": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp]),
+    "mvme_fp4_gather": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _int, _vp]),
+    "mvme_fp4_paged_attention_workspace_size": (_size, [_i64] * 7),
+    "mvme_fp4_paged_attention": (_int, [_vp] * 6 + [_i64] * 8 + [_int, _vp, _size, _vp]),
+    "mvme_fp4_paged_prefill_workspace_size": (_size, [_i64] * 8),
+    "mvme_fp4_paged_prefill_attention": (_int, [_vp] * 8 + [_i64] * 9 + [_int, _vp, _size, _vp]),
+    "mvme_copy_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "mvme_compact_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp]),
+}
+
 
 class HipLibrary:
     """Typed handle on the shared object; every call checks its status."""
@@ -64,7 +80,7 @@ class HipLibrary:
     def __init__(self, lib: ctypes.CDLL, path):
         self._lib = lib
         self.path = path
-        for name, (restype, argtypes) in SIGNATURES.items():
+        for name, (restype, argtypes) in (SIGNATURES | PACKED_SIGNATURES).items():
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -89,6 +105,12 @@ class HipLibrary:
 
     def dense_prefill_workspace_size(self, *args) -> int:
         return int(self._lib.mvme_prefill_attention_workspace_size(*args))
+
+    def fp4_workspace_size(self, *args) -> int:
+        return int(self._lib.mvme_fp4_paged_attention_workspace_size(*args))
+
+    def fp4_prefill_workspace_size(self, *args) -> int:
+        return int(self._lib.mvme_fp4_paged_prefill_workspace_size(*args))
 
     def argmax_workspace_size(self, *args) -> int:
         return int(self._lib.mvme_greedy_argmax_workspace_size(*args))
@@ -218,3 +240,15 @@ def current_stream(device: torch.device) -> int:
 
 def ptr(tensor: torch.Tensor) -> int:
     return tensor.data_ptr()
+
+
+def share_bytes(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet (two views of one storage need not)."""
+    def span(t):
+        reach = sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (reach + 1) * t.element_size()
+
+    if a.device != b.device or a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1

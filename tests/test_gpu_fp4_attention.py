@@ -1,0 +1,319 @@
+"""Decode and prefill attention over packed 4-bit pages, on the GPU, against
+float64 with bounds that count the roundings (fp4_cases.attention)."""
+
+import pytest
+import torch
+
+import fp4_cases as f4
+from mini_engine_hip.kernels.fp4 import (fp4_prefill_workspace_bytes, fp4_workspace_bytes, paged_attention_fp4,
+                                         paged_prefill_attention_fp4)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def decode_case(lens, dtype, *, heads=16, kv=8, dim=128, block=16, seed=0, pad=0):
+    gen = torch.Generator().manual_seed(seed + 31 * dim + block)
+    tables, pages = f4.tables_of(gen, lens, block, pad=pad)
+    kc, vc = f4.random_caches(gen, pages, kv, block, dim, dtype)
+    query = torch.randn(len(lens), heads, dim, generator=gen).to(dtype)
+    return [query, kc, vc, tables, torch.tensor(lens)], block
+
+
+def run_decode(args, block, **kw):
+    return paged_attention_fp4(*[a.to(DEV) for a in args], block, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("block", [16, 256, 7])
+def test_decode_head_dims(dtype, dim, block):
+    args, block = decode_case((1, 17, 257, 521), dtype, dim=dim, block=block, heads=6, kv=2)
+    f4.assert_within(run_decode(args, block), *f4.decode_oracle(*args, block))
+
+
+@pytest.mark.parametrize("heads,kv", [(8, 8), (14, 2), (16, 1), (17, 1), (40, 2), (33, 1), (24, 3)])
+@pytest.mark.parametrize("partition", [0, 64])
+def test_decode_groups(heads, kv, partition):
+    """Groups that fill a matrix tile, leave columns of it idle, and take several."""
+    args, block = decode_case((300, 1, 95), torch.bfloat16, heads=heads, kv=kv, dim=64, seed=heads)
+    f4.assert_within(run_decode(args, block, partition_tokens=partition), *f4.decode_oracle(*args, block))
+
+
+@pytest.mark.parametrize("block,lens", [(1, (3, 70)), (16, (16, 32, 33)), (24, (70, 24)), (256, (255, 256, 257)),
+                                        (5000, (4999,)), (16, (31, 63, 64, 65, 511, 512, 513))])
+def test_decode_block_and_tile_boundaries(block, lens):
+    args, block = decode_case(lens, torch.float16, block=block, heads=4, kv=2)
+    want = f4.decode_oracle(*args, block)
+    for partition in (0, 32, 96, 4096):
+        f4.assert_within(run_decode(args, block, partition_tokens=partition), *want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("partition", [0, 32])
+def test_decode_empty_sequences_and_absent_pages(dtype, partition):
+    """Lengths that give no keys, pages that do not exist (a whole sequence of them too), trusted metadata."""
+    args, block = decode_case((40, 100, 130, 64, 9, 50), dtype, heads=8, kv=2, pad=2)
+    tables, lens = args[3], args[4]
+    lens[1], lens[4], lens[3] = 0, -7, (tables.shape[1] * block) + 1
+    tables[2, 3], tables[2, 5], tables[2, 8] = -1, 1 << 40, args[1].shape[0]
+    tables[5] = -1
+    want = f4.decode_oracle(*args, block)
+    got = run_decode(args, block, validate=False, partition_tokens=partition)
+    f4.assert_within(got, *want)
+    assert not got[[1, 3, 4, 5]].any()
+
+
+def test_decode_ignores_what_is_behind_the_length():
+    """Bytes behind a sequence's last token, whatever they are, change nothing; so does the padding."""
+    args, block = decode_case((33, 5), torch.bfloat16, heads=8, kv=2, dim=96, block=7)
+    base = run_decode(args, block)
+    for fill in (0xFF, 0xFE, 0x00):
+        dirty = [args[0], *(torch.full_like(c, fill) for c in args[1:3]), *args[3:]]
+        for cache, clean in zip(dirty[1:3], args[1:3]):
+            code, byte = f4.split(clean, block, 96)
+            dcode, dbyte = f4.split(cache, block, 96)
+            for b, n in enumerate(args[4].tolist()):
+                for t in range(n):
+                    page = args[3][b, t // block]
+                    dcode[page, :, t % block], dbyte[page, :, t % block] = code[page, :, t % block], byte[page, :, t % block]
+            cache.copy_(f4.join(dcode, dbyte))
+            cache[..., block * (96 // 2 + 96 // 32):] = fill
+        assert torch.equal(run_decode(dirty, block), base)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_decode_extreme_values(dtype):
+    """Scores in the hundreds, rising with the position, tiny and large values: the running reference moves."""
+    gen = torch.Generator().manual_seed(8)
+    n, dim, block = 700, 128, 16
+    tables, pages = f4.tables_of(gen, (n,), block)
+    rows = torch.randn(pages, 2, block, dim, generator=gen)
+    for at in range(n):
+        rows[tables[0, at // block], :, at % block] += at / 100
+    kc = f4.packed((rows * 3).to(dtype))
+    for size in (2.0 ** -20, 1.0, 40000.0):
+        vc = f4.packed((torch.randn(pages, 2, block, dim, generator=gen) * size).clamp(-60000, 60000).to(dtype))
+        query = torch.cat((torch.ones(1, 2, dim), -torch.ones(1, 2, dim)), 1).to(dtype) * 2
+        args = [query, kc, vc, tables, torch.tensor([n])]
+        want = f4.decode_oracle(*args, block)
+        for partition in (0, 64):
+            f4.assert_within(run_decode(args, block, partition_tokens=partition), *want)
+
+
+def test_decode_nan_blocks_reach_the_sequences_that_hold_them():
+    args, block = decode_case((70, 70), torch.float16, heads=4, kv=2, dim=64)
+    code, byte = f4.split(args[2], block, 64)
+    byte[args[3][0, 2], 1, 5] = 255  # sequence 0, kv head 1, token 37
+    args[2] = f4.join(code, byte)
+    got = run_decode(args, block)
+    assert got[0, 2:].isnan().all() and not got[0, :2].isnan().any() and not got[1].isnan().any()
+    code, byte = f4.split(args[1], block, 64)
+    byte[args[3][1, 0], 0, 0, 1] = 255
+    args[1] = f4.join(code, byte)
+    got = run_decode(args, block)
+    assert got[1, :2].isnan().all() and not got[1, 2:].isnan().any()
+
+
+def test_decode_long_sequence_and_many_partitions():
+    args, block = decode_case((70001,), torch.bfloat16, heads=4, kv=1, block=256)
+    want = f4.decode_oracle(*args, block)
+    for partition in (0, 32, 1000):
+        f4.assert_within(run_decode(args, block, partition_tokens=partition), *want)
+
+
+def test_decode_is_repeatable_and_takes_buffers():
+    args, block = decode_case((900, 31, 400), torch.bfloat16)
+    dev = [a.to(DEV) for a in args]
+    base = paged_attention_fp4(*dev, block)
+    need = fp4_workspace_bytes(3, 16, 8, 128, block, args[3].shape[1])
+    out, workspace = torch.empty_like(dev[0]), torch.full((need + 64,), 255, dtype=torch.uint8, device=DEV)
+    for _ in range(3):
+        assert paged_attention_fp4(*dev, block, out=out, workspace=workspace) is out
+        assert torch.equal(out, base)
+    strided = torch.empty(3, 16, 256, dtype=torch.bfloat16, device=DEV)[..., ::2]
+    strided.copy_(dev[0])
+    shifted = torch.empty(3 * 16 * 128 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(3, 16, 128)
+    shifted.copy_(dev[0])
+    assert torch.equal(paged_attention_fp4(strided, *dev[1:], block), base)
+    assert torch.equal(paged_attention_fp4(shifted, *dev[1:], block), base)
+
+
+def test_decode_pages_past_four_gigabytes():
+    gen = torch.Generator().manual_seed(9)
+    block, dim, kv, pages = 256, 128, 8, 33000
+    kc, vc = (torch.empty(pages, kv, f4.record_bytes(block, dim), dtype=torch.uint8, device=DEV) for _ in range(2))
+    small = f4.random_caches(gen, 3, kv, block, dim, torch.bfloat16)
+    where = torch.tensor([[32999, 17, 31111]])
+    for cache, source in zip((kc, vc), small):
+        cache[where[0].to(DEV)] = source.to(DEV)
+    query = torch.randn(1, 8, dim, generator=gen).bfloat16()
+    lens = torch.tensor([700])
+    got = paged_attention_fp4(query.to(DEV), kc, vc, where.to(DEV), lens.to(DEV), block)
+    f4.assert_within(got, *f4.decode_oracle(query, *small, torch.tensor([[0, 1, 2]]), lens, block))
+    got = paged_prefill_attention_fp4(query.to(DEV), kc, vc, torch.tensor([0, 1], device=DEV),
+                                      torch.tensor([699], device=DEV), where.to(DEV), lens.to(DEV), block)
+    f4.assert_within(got, *f4.decode_oracle(query, *small, torch.tensor([[0, 1, 2]]), lens, block))
+
+
+# ---------------------------------------------------------------------------
+# Prefill
+# ---------------------------------------------------------------------------
+def prefill_case(new, prior, dtype, *, heads=4, kv=2, dim=128, block=16, seed=0, pad=0):
+    gen = torch.Generator().manual_seed(seed + 31 * dim + block)
+    lens = [n + p for n, p in zip(new, prior)]
+    tables, pages = f4.tables_of(gen, lens, block, pad=pad)
+    kc, vc = f4.random_caches(gen, pages, kv, block, dim, dtype)
+    query = torch.randn(sum(new), heads, dim, generator=gen).to(dtype)
+    cu = torch.tensor([0, *new]).cumsum(0)
+    return [query, kc, vc, cu, torch.tensor(prior), tables, torch.tensor(lens)], block
+
+
+def run_prefill(args, block, **kw):
+    return paged_prefill_attention_fp4(*[a.to(DEV) for a in args], block, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [32, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("block", [16, 256, 7])
+def test_prefill_head_dims(dtype, dim, block):
+    args, block = prefill_case((33, 1, 70), (0, 130, 61), dtype, dim=dim, block=block)
+    f4.assert_within(run_prefill(args, block), *f4.prefill_oracle(*args, block))
+
+
+@pytest.mark.parametrize("heads,kv", [(8, 8), (14, 2), (16, 1), (7, 1), (40, 2), (130, 1)])
+@pytest.mark.parametrize("chunk", [0, 64])
+def test_prefill_groups(heads, kv, chunk):
+    """Groups that divide the row tiles, do not, and pass them."""
+    args, block = prefill_case((50, 3), (20, 100), torch.bfloat16, heads=heads, kv=kv, dim=32, seed=heads)
+    f4.assert_within(run_prefill(args, block, chunk_tokens=chunk), *f4.prefill_oracle(*args, block))
+
+
+@pytest.mark.parametrize("new,prior", [((1,), (0,)), ((64,), (0,)), ((65, 64, 63), (0, 1, 63)), ((128, 129), (128, 0)),
+                                       ((1, 1, 1, 1), (0, 62, 63, 64)), ((0, 5, 0), (0, 3, 0)), ((200,), (333,))])
+@pytest.mark.parametrize("chunk", [0, 64, 100])
+def test_prefill_row_and_key_boundaries(new, prior, chunk):
+    args, block = prefill_case(new, prior, torch.float16, block=16)
+    f4.assert_within(run_prefill(args, block, chunk_tokens=chunk), *f4.prefill_oracle(*args, block))
+
+
+@pytest.mark.parametrize("chunk", [0, 64])
+def test_prefill_rows_without_keys(chunk):
+    """Absent pages, lengths that do not fit the rows, rows of no sequence: zeros, with trusted metadata."""
+    args, block = prefill_case((20, 30, 40, 10, 25), (50, 0, 7, 3, 0), torch.bfloat16, dim=64, pad=1)
+    query, _, _, cu, starts, tables, lens = args
+    lens[0] = 60            # ten rows past it
+    starts[2] = -1
+    lens[3] = tables.shape[1] * block + 1
+    tables[4] = -1          # no page at all
+    tables[1, 0] = 1 << 33  # the first sixteen keys: rows 0..15 see none
+    args[0] = torch.cat((query, query[:9]))  # rows behind the last sequence
+    want = f4.prefill_oracle(*args, block)
+    got = run_prefill(args, block, validate=False, chunk_tokens=chunk)
+    f4.assert_within(got, *want)
+    assert not got[10:36].any() and not got[50:].any()
+    args[3] = cu.clone()
+    args[3][0] = 4          # rows before the first sequence
+    got = run_prefill(args, block, validate=False, chunk_tokens=chunk)
+    assert not got[:4].any()
+
+
+def test_prefill_offsets_out_of_order_stay_in_bounds():
+    args, block = prefill_case((31, 20, 20), (9, 3, 10), torch.bfloat16)
+    for cu in ([0, 50, 30, 71], [0, 50, 1 << 40, 71], [-5, 20, 60, 1 << 33], [71, 71, 0, 3]):
+        args[3] = torch.tensor(cu)
+        for chunk in (0, 64):
+            out = run_prefill(args, block, validate=False, chunk_tokens=chunk)
+            torch.cuda.synchronize()
+            assert out.shape == args[0].shape
+
+
+@pytest.mark.parametrize("chunk", [0, 64])
+@pytest.mark.parametrize("plane", [1, 2])
+def test_prefill_nan_behind_the_mask_stays_there(plane, chunk):
+    """A NaN block reaches the rows that see its key and no other (in particular not as 0 * NaN)."""
+    args, block = prefill_case((100,), (30,), torch.float16, heads=4, kv=2, dim=64)
+    clean = run_prefill(args, block, chunk_tokens=chunk)
+    code, byte = f4.split(args[plane], block, 64)
+    byte[args[5][0, 90 // block], 1, 90 % block, 1] = 255  # kv head 1, key 90: rows from 60 on
+    args[plane] = f4.join(code, byte)
+    got = run_prefill(args, block, chunk_tokens=chunk)
+    assert torch.equal(got[:60], clean[:60]) and torch.equal(got[:, :2], clean[:, :2])
+    assert got[60:, 2:].isnan().all()
+
+
+def test_prefill_many_sequences():
+    gen = torch.Generator().manual_seed(11)
+    new = torch.randint(0, 9, (150,), generator=gen).tolist()
+    prior = torch.randint(0, 40, (150,), generator=gen).tolist()
+    new[3] = 90
+    prior = [p if n else 0 for n, p in zip(new, prior)]
+    args, block = prefill_case(new, prior, torch.bfloat16, dim=32, block=5)
+    f4.assert_within(run_prefill(args, block), *f4.prefill_oracle(*args, block))
+
+
+def test_prefill_of_single_rows_equals_decode():
+    """One new token per sequence is a decode step: both kernels are within their bounds of each other."""
+    args, block = decode_case((1, 300, 77), torch.bfloat16)
+    query, kc, vc, tables, lens = args
+    want, bound = f4.decode_oracle(*args, block)
+    got = run_prefill([query, kc, vc, torch.arange(4), lens - 1, tables, lens], block)
+    f4.assert_within(got, want, bound)
+
+
+def test_prefill_takes_a_workspace():
+    args, block = prefill_case((40, 60), (900, 500), torch.bfloat16, heads=16, kv=8)
+    dev = [a.to(DEV) for a in args]
+    base = paged_prefill_attention_fp4(*dev, block)
+    need = fp4_prefill_workspace_bytes(2, 100, 16, 8, 128, block, args[5].shape[1])
+    assert need > 0
+    workspace = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
+    assert torch.equal(paged_prefill_attention_fp4(*dev, block, workspace=workspace), base)
+
+
+# ---------------------------------------------------------------------------
+# Streams and graphs
+# ---------------------------------------------------------------------------
+def test_other_stream_sees_its_own_order():
+    args, block = decode_case((500, 40), torch.float16)
+    dev = [a.to(DEV) for a in args]
+    base = paged_attention_fp4(*dev, block)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        late = dev[0] * 0
+        torch.cuda._sleep(2_000_000)
+        late += dev[0]
+        got = paged_attention_fp4(late, *dev[1:], block, validate=False)
+    side.synchronize()
+    assert torch.equal(got, base)
+
+
+def test_graph_replays_follow_their_inputs():
+    """A captured decode step and prefill: new lengths, tables and queries before every replay."""
+    args, block = decode_case((800, 800, 800), torch.bfloat16, seed=5)
+    dev = [a.to(DEV) for a in args]
+    cu = torch.arange(4, device=DEV)
+    starts = dev[4] - 1
+
+    def step():
+        return (paged_attention_fp4(*dev, block, validate=False),
+                paged_prefill_attention_fp4(*dev[:3], cu, starts, *dev[3:], block, validate=False))
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    gen = torch.Generator().manual_seed(12)
+    for lens in ((1, 800, 33), (0, 5, 640), (799, 256, 257), (32, 31, 1)):
+        dev[0].copy_(torch.randn(3, 16, 128, generator=gen).bfloat16())
+        dev[3].copy_(dev[3][torch.randperm(3, generator=gen).to(DEV)].clone())
+        dev[4].copy_(torch.tensor(lens))
+        starts.copy_(dev[4] - 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, eager))
