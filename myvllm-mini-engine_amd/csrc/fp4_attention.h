@@ -42,17 +42,31 @@ struct TileLayout {
     __device__ static inline int at(int row, int chunk) { return row * 2 * D + ((chunk ^ (row & kMask)) << 4); }
 };
 
-// 16 dims of 8 keys for the value product: A operand of dims 16 n .. 16 n + 15.
-// `base` is the tile, rows in fp16.
+// A lane's place in a tile, for accesses at chunks `first + i` of its row.  For
+// power-of-two rows the XOR of the layout acts on address bits of its own, so
+// one register and an XOR with a constant give every address; `forget` keeps
+// the compiler from holding them all in registers across a loop.
 template <int D>
-__device__ inline u32x4 value_operand(const uint8_t* base, int n, int first_row) {
-    const int lane = __lane_id(), r = lane & 15, g = lane >> 4;
-    const int row = first_row + 4 * g + (r >> 2);
-    const int at = TileLayout<D>::at(row, 2 * n + ((r & 3) >> 1)) + (r & 1) * 8;
-    const int at2 = TileLayout<D>::at(row + 16, 2 * n + ((r & 3) >> 1)) + (r & 1) * 8;
+struct TileAddress {
+    static constexpr bool kPow2 = (D & (D - 1)) == 0;
+    int row, first, base;
+    __device__ inline TileAddress(int row, int first, int bytes = 0) : row(row), first(first) {
+        base = (kPow2 ? TileLayout<D>::at(row, first) : row * 2 * D) + bytes;
+    }
+    __device__ inline void forget() { asm volatile("" : "+v"(base)); }
+    __device__ inline int chunk(int i) const {  // first is a multiple of the power of two above i, or i of the one above it
+        if constexpr (kPow2) return base ^ (i << 4);
+        return base + (((first + i) ^ (row & TileLayout<D>::kMask)) << 4);
+    }
+};
+
+// 16 dims of 8 keys for the value product: A operand of 16 dims and 32 keys of a tile in fp16.  `at` is the lane's
+// address for the first 16 keys: row 4 g + r / 4, the 8 bytes r % 4 of the 16 dims.
+template <int D>
+__device__ inline u32x4 value_operand(const uint8_t* tile, int at) {
     typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(base + at));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(base + at2));
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + at));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + at + 16 * 2 * D));
     const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
     return u32x4{x[0], x[1], y[0], y[1]};
 }

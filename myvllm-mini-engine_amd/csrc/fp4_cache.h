@@ -47,6 +47,11 @@ inline bool valid_format(int64_t block_size, int64_t head_dim) {
            head_dim % kBlockDims == 0;
 }
 
+// A load by all lanes from one address that no kernel writes meanwhile, through the scalar cache.
+__device__ inline int64_t uniform_load(const int64_t* p) {
+    return *(const __attribute__((address_space(4))) int64_t*)(uintptr_t)p;
+}
+
 // The f32 whose exponent is a scale byte (255: the conversions give NaN).
 __device__ inline float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 

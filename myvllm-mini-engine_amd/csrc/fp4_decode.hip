@@ -1,9 +1,12 @@
 // Decode attention over packed 4-bit pages: one query token per sequence.
 //
-// A work-group owns one sequence, one kv head (16 of its query heads) and one
-// partition of the keys; its waves take tiles of 32 keys in turn and keep
-// their own maximum, sum and accumulators, joined through LDS at the end.
-// Partitions of a split sequence are joined by a second kernel.
+// A unit is one sequence and kv head (16 of its query heads).  A work-group's
+// waves take the tiles of 32 keys of a unit in turn and keep their own
+// maximum, sum and accumulators, joined through LDS at the end.  Units are
+// handed out whole, or all units are laid end to end and cut into equal
+// shares (in rounds: one tile for every wave), one per work-group, so that
+// ragged and few long sequences load every CU alike; a second kernel joins the
+// units that a share boundary cuts.
 #include "fp4_attention.h"
 
 namespace mvme {
@@ -17,12 +20,14 @@ struct DecodeArgs {
     const uint8_t* value;
     const int64_t* tables;
     const int64_t* lens;
-    float* partial;  // [batch, q_heads, parts, D] accumulators, then [batch, q_heads, parts, 2] (reference, sum)
+    float* pieces;   // [work-groups, 2, 16, D] accumulators, then [work-groups, 2, 16, 2] (reference, sum)
     int64_t num_blocks, record;
+    uint64_t page_bytes;
     int64_t stats;   // offset of the (reference, sum) pairs, in floats
-    int kv_heads, group, q_heads, width;
+    int batch, kv_heads, group, q_heads, width;
     int head_tiles;  // ceil(group / 16)
-    int parts, part_tokens;
+    int groups;      // work-groups of the walk; 0: one per unit
+    int share;       // rounds of a share; 0: as many as spread all rounds over the work-groups
     BlockDiv div;
     float scale;     // log2(e) / sqrt(D)
 };
@@ -36,18 +41,139 @@ struct Shape {
     static constexpr int kDimTiles = D / 16;
     static constexpr int kTileBytes = kTileKeys * 2 * D;  // fp16 rows of a tile; as large as a wave's accumulators
     static constexpr int kMinWaves = D <= 128 ? 4 : 2;
+    static constexpr int kRound = kWaves * kTileKeys;     // keys of a round
+};
+
+// The walk's order: sequences, their units, a unit's rounds.
+template <int D>
+__device__ inline int rounds_of(const DecodeArgs& a, int64_t len) {
+    const bool usable = len > 0 && len <= (int64_t)a.width * a.div.size;
+    return usable ? (int)(((uint32_t)len - 1) / Shape<D>::kRound) + 1 : 0;
+}
+
+__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ inline int64_t length_of(const DecodeArgs& a, int seq) { return seq < a.batch ? a.lens[seq] : 0; }
+
+// Shares of the walk, in rounds.  Every wave computes the same, lane-parallel over the sequences; the first 64 lengths
+// stay in registers.
+template <int D>
+struct Walk {
+    int64_t len;  // of sequence `lane`
+    int units;    // of a sequence
+    int total, share;
+    __device__ inline void count(const DecodeArgs& a) {
+        units = a.kv_heads * a.head_tiles;
+        const int lane = __lane_id();
+        len = length_of(a, lane);
+        total = lane_value(wave_incl_scan(rounds_of<D>(a, len)), kWave - 1);
+        for (int s0 = kWave; s0 < a.batch; s0 += kWave)
+            total += lane_value(wave_incl_scan(rounds_of<D>(a, length_of(a, s0 + lane))), kWave - 1);
+        total *= units;
+        share = a.share > 0 ? a.share : (total + a.groups - 1) / a.groups;
+    }
+    // The sequence that owns round `round` (< total), the round it begins at, its rounds per unit and its length.
+    __device__ inline void find(const DecodeArgs& a, int round, int& seq, int& base, int& rounds, uint32_t& tokens) const {
+        const int lane = __lane_id();
+        int before = 0;
+        for (int s0 = 0;; s0 += kWave) {
+            const int64_t n = s0 == 0 ? len : length_of(a, s0 + lane);
+            const int mine = rounds_of<D>(a, n) * units, incl = before + wave_incl_scan(mine);
+            const uint64_t hit = __ballot(incl > round);
+            if (hit || s0 + kWave >= a.batch) {
+                const int at = hit ? __builtin_ctzll(hit) : 0;
+                seq = s0 + at;
+                rounds = lane_value(mine, at);
+                base = lane_value(incl, at) - rounds;
+                rounds /= units;
+                tokens = (uint32_t)lane_value((int)n, at);
+                return;
+            }
+            before = lane_value(incl, kWave - 1);
+        }
+    }
+    // First round of sequence `seq`.
+    __device__ inline int first_of(const DecodeArgs& a, int seq) const {
+        const int lane = __lane_id();
+        int base = 0;
+        for (int s0 = 0; s0 < seq; s0 += kWave) {
+            const int mine = s0 + lane < seq ? rounds_of<D>(a, s0 == 0 ? len : length_of(a, s0 + lane)) : 0;
+            base += lane_value(wave_incl_scan(mine), kWave - 1);
+        }
+        return base * units;
+    }
+};
+
+// A run of rounds of one unit: what a work-group does at a time.  Wave-uniform.
+struct Segment {
+    int seq, kv_head, tile;
+    uint32_t begin, end;  // keys
+    int slot;             // where its piece goes; -1: it is the whole unit, straight to the output
+    int rounds;           // 0: none
 };
 
 template <int D>
-struct Row {  // a lane's part of one token: D / 4 dims
+struct Part {  // a lane's part of one token of one plane: D / 4 dims
     uint32_t codes[Shape<D>::kChunks];
     uint32_t scales[Shape<D>::kScales];
 };
 
 template <int D>
-__device__ inline void load_row(Row<D>& x, const uint8_t* record, uint32_t place, uint32_t block, int g) {
-    const uint8_t* codes = record + place * (D / 2) + g * (D / 8);
-    const uint8_t* scales = record + block * (D / 2) + place * (D / kBlockDims);
+__device__ inline void clear_part(Part<D>& x, bool keep) {
+#pragma unroll
+    for (int i = 0; i < Shape<D>::kChunks; ++i) x.codes[i] = keep ? x.codes[i] : 0u;
+#pragma unroll
+    for (int i = 0; i < Shape<D>::kScales; ++i) x.scales[i] = keep ? x.scales[i] : 127u;
+}
+
+// Where a tile's tokens are.  RUN tokens (block sizes that are multiples of
+// RUN) lie in one page at consecutive places: their record and first place are
+// wave-uniform, and a lane's own offset never changes.  RUN 1: every lane looks
+// its tokens up.
+template <int D, int RUN>
+struct Where {
+    static constexpr int kCount = RUN == 32 ? 1 : 2;
+    int64_t codes[kCount];     // byte offset of the run's first token in a plane; of a page that exists, to load without a branch
+    uint32_t scales[kCount];   // from there to its scales
+    bool there[kCount];
+};
+
+template <int D, int RUN>
+__device__ inline Where<D, RUN> look_up(const DecodeArgs& a, const int64_t* table, int64_t head, uint32_t first,
+                                        uint32_t end, int r) {
+    Where<D, RUN> w;
+#pragma unroll
+    for (int s = 0; s < Where<D, RUN>::kCount; ++s) {
+        const uint32_t token = first + 16 * s + (RUN == 1 ? r : 0), block = a.div.page(token);
+        const int64_t* entry = table + min(block, (uint32_t)a.width - 1u);
+        int64_t page = RUN == 1 ? *entry : uniform_load(entry);
+        uint32_t place = token - block * a.div.size;
+        w.there[s] = token < end && (uint64_t)page < (uint64_t)a.num_blocks;
+        page = w.there[s] ? page : 0;
+        place = w.there[s] ? place : 0u;
+        w.codes[s] = head + (int64_t)((uint64_t)(uint32_t)page * a.page_bytes) + place * (D / 2);
+        w.scales[s] = a.div.size * (D / 2) - place * (D / 2 - D / kBlockDims);
+    }
+    return w;
+}
+
+// A lane's offsets in a run.  Kept from being widened outside of the loop, they stay the 32-bit offset of a load.
+template <int D, int RUN>
+struct LaneAt {
+    uint32_t codes, scales[Shape<D>::kScales];
+    __device__ inline LaneAt(int r, int g) : codes((RUN == 1 ? 0 : r * (D / 2)) + g * (D / 8)) {
+#pragma unroll
+        for (int i = 0; i < Shape<D>::kScales; ++i)
+            scales[i] = (RUN == 1 ? 0 : r * (D / kBlockDims)) + (g * (D / 4) + 8 * i * Shape<D>::kPer) / kBlockDims;
+    }
+    __device__ inline void forget() {
+        asm volatile("" : "+v"(codes));
+#pragma unroll
+        for (int i = 0; i < Shape<D>::kScales; ++i) asm volatile("" : "+v"(scales[i]));
+    }
+};
+
+template <int D>
+__device__ inline void load_codes(Part<D>& x, const uint8_t* codes) {
     if constexpr (Shape<D>::kChunks % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < Shape<D>::kChunks; i += 4) {
@@ -66,186 +192,306 @@ __device__ inline void load_row(Row<D>& x, const uint8_t* record, uint32_t place
 #pragma unroll
         for (int i = 0; i < Shape<D>::kChunks; ++i) x.codes[i] = reinterpret_cast<const uint32_t*>(codes)[i];
     }
+}
+
+template <int D, int RUN>
+__device__ inline void load_tile(Part<D> (&x)[2], const uint8_t* plane, const Where<D, RUN>& w, const LaneAt<D, RUN>& at) {
 #pragma unroll
-    for (int i = 0; i < Shape<D>::kScales; ++i)
-        x.scales[i] = scales[(g * (D / 4) + 8 * i * Shape<D>::kPer) / kBlockDims];
+    for (int s = 0; s < 2; ++s) {
+        const int run = RUN == 32 ? 0 : s, more = RUN == 32 ? 16 * s : 0;
+        const uint8_t* base = plane + w.codes[run];
+        load_codes<D>(x[s], base + at.codes + more * (D / 2));
+#pragma unroll
+        for (int i = 0; i < Shape<D>::kScales; ++i)
+            x[s].scales[i] = (base + (at.scales[i] + w.scales[run]))[more * (D / kBlockDims)];
+    }
 }
 
 template <int D>
-__device__ inline void zero_row(Row<D>& x) {
+__device__ inline void load_query(u32x4 (&q)[Shape<D>::kChunks], const DecodeArgs& a, const Segment& s, int r, int g) {
+    // Head r, dims g * D / 4 + 8 c .. + 7: the order in which a lane's codes lie.
+    const bool live = r < min(16, a.group - s.tile * 16);
+    const int64_t head = (int64_t)s.seq * a.q_heads + s.kv_head * a.group + s.tile * 16 + r;
 #pragma unroll
-    for (int i = 0; i < Shape<D>::kChunks; ++i) x.codes[i] = 0u;
-#pragma unroll
-    for (int i = 0; i < Shape<D>::kScales; ++i) x.scales[i] = 127u;
+    for (int c = 0; c < Shape<D>::kChunks; ++c) {
+        q[c] = u32x4{0u, 0u, 0u, 0u};
+        if (live) q[c] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.query) + head * D + g * (D / 4) + 8 * c);
+    }
 }
 
-template <typename T, int D>
+template <typename T, int D, int RUN>
 __global__ __launch_bounds__(64 * Shape<D>::kWaves, Shape<D>::kMinWaves) void fp4_decode_kernel(DecodeArgs a) {
     using S = Shape<D>;
     __shared__ __attribute__((aligned(16))) uint8_t tiles[S::kWaves][S::kTileBytes];
     __shared__ float stats[S::kWaves][2][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int part = blockIdx.x % a.parts, unit = blockIdx.x / a.parts;
-    const int tile = unit % a.head_tiles, kv_head = unit / a.head_tiles % a.kv_heads;
-    const int b = unit / a.head_tiles / a.kv_heads;
-    const int64_t len = a.lens[b];
-    const int heads = min(16, a.group - tile * 16);
-    const int64_t first_head = (int64_t)b * a.q_heads + kv_head * a.group + tile * 16;
-    const bool usable = len > 0 && len <= (int64_t)a.width * a.div.size;
-    const uint32_t begin = (uint32_t)part * a.part_tokens;
-    const uint32_t end = usable ? min((uint32_t)len, begin + (uint32_t)a.part_tokens) : 0u;
-    if (begin >= end && (part > 0 || a.parts > 1)) return;  // no partial; an empty sequence is written by the merge
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    // Query operand: head r, dims g * D / 4 + 8 c .. + 7, the order in which a lane's codes lie.
-    u32x4 q[S::kChunks];
-#pragma unroll
-    for (int c = 0; c < S::kChunks; ++c) {
-        q[c] = u32x4{0u, 0u, 0u, 0u};
-        if (r < heads)
-            q[c] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.query) + (first_head + r) * D +
-                                                   g * (D / 4) + 8 * c);
+    Walk<D> walk;
+    int first = 0, stop = 0;  // the share, in rounds
+    if (a.groups) {
+        walk.count(a);
+        const int64_t from = (int64_t)blockIdx.x * walk.share;
+        first = (int)min(from, (int64_t)walk.total);
+        stop = (int)min(from + walk.share, (int64_t)walk.total);
+        if (first == stop) return;
     }
-    f32x4 acc[S::kDimTiles];
-#pragma unroll
-    for (int n = 0; n < S::kDimTiles; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float ref = kRefNone, sum = 0.f;
-    uint8_t* tile_lds = tiles[wave];
-    const int64_t* table = a.tables + (int64_t)b * a.width;
+    // The segment that begins at round `at` of the share (or the work-group's unit).
+    const auto segment = [&](int at) {
+        Segment s;
+        int unit, from, n, rounds;
+        uint32_t tokens;
+        if (a.groups) {
+            int base;
+            walk.find(a, at, s.seq, base, rounds, tokens);
+            unit = (at - base) / rounds;
+            from = at - base - unit * rounds;
+            n = min(rounds - from, stop - at);
+            s.slot = n == rounds ? -1 : (int)blockIdx.x * 2 + (at > first ? 1 : 0);
+        } else {
+            const int units = a.kv_heads * a.head_tiles;
+            s.seq = blockIdx.x / units;
+            unit = blockIdx.x - s.seq * units;
+            const int64_t len = a.lens[s.seq];
+            rounds = rounds_of<D>(a, len);
+            tokens = rounds ? (uint32_t)len : 0u;
+            from = 0;
+            n = max(rounds, 1);  // an empty sequence: one round without keys, which writes the zeros
+            s.slot = -1;
+        }
+        // (Uniform all along, but only now provably so: what these address is loaded and computed once per wave.)
+        s.seq = uniform(s.seq);
+        s.kv_head = uniform(unit / a.head_tiles);
+        s.tile = uniform(unit) - s.kv_head * a.head_tiles;
+        s.begin = (uint32_t)uniform(from * S::kRound);
+        s.end = (uint32_t)uniform((int)min(tokens, (uint32_t)(from + n) * S::kRound));
+        s.slot = uniform(s.slot);
+        s.rounds = uniform(n);
+        return s;
+    };
 
-    for (uint32_t t0 = begin + wave * kTileKeys; t0 < end; t0 += S::kWaves * kTileKeys) {
-        Row<D> k[2], v[2];
-        uint32_t present[2];
+    TileAddress<D> write_at(r, g * S::kChunks), read_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
+    LaneAt<D, RUN> lane_at(r, g);
+    uint8_t* tile_lds = tiles[wave];
+    // A tile's registers are refilled as soon as they are used up: keys after
+    // the scores, values when they are in LDS.  The lookups run a tile ahead,
+    // and all of it runs on into the next segment.
+    u32x4 q[S::kChunks];
+    Part<D> k[2], v[2];
+    Where<D, RUN> now;
+    const auto find_tile = [&](const Segment& s, uint32_t t) {
+        return look_up<D, RUN>(a, a.tables + (int64_t)s.seq * a.width, s.kv_head * a.record, t, s.end, r);
+    };
+    int at = first;
+    Segment seg = segment(at);
+    uint32_t t0 = seg.begin + wave * kTileKeys;
+    now = find_tile(seg, t0);
+    load_query<D>(q, a, seg, r, g);
+    load_tile<D, RUN>(k, a.key, now, lane_at);
+    load_tile<D, RUN>(v, a.value, now, lane_at);
+#pragma unroll 1
+    for (;;) {
+        at += seg.rounds;
+        Segment ahead;
+        ahead.rounds = 0;
+        if (at < stop) ahead = segment(at);
+        f32x4 acc[S::kDimTiles];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const uint32_t token = t0 + 16 * s + r;
-            bool there = token < end;
-            if (there) {
-                const uint32_t block = a.div.page(token);
-                const int64_t page = table[block];
-                there = page >= 0 && page < a.num_blocks;
-                if (there) {
-                    const int64_t at = (page * a.kv_heads + kv_head) * a.record;
-                    load_row<D>(k[s], a.key + at, token - block * a.div.size, a.div.size, g);
-                    load_row<D>(v[s], a.value + at, token - block * a.div.size, a.div.size, g);
+        for (int n = 0; n < S::kDimTiles; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float ref = kRefNone, sum = 0.f;
+        const bool idle = t0 >= seg.end;  // no tile of this segment for this wave
+#pragma unroll 1
+        for (; t0 < seg.end; t0 += S::kRound) {
+            const bool more = t0 + S::kRound < seg.end;
+            write_at.forget();
+            read_at.forget();
+            lane_at.forget();
+            Where<D, RUN> next = now;
+            if (more) next = find_tile(seg, t0 + S::kRound);
+            else if (ahead.rounds) next = find_tile(ahead, ahead.begin + wave * kTileKeys);
+            // Scores.
+            f32x4 x[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < S::kChunks; ++i)
+                    x[s] = T::mfma16x16x32(values_of<T>(k[s].codes[i], scale_of(k[s].scales[i / S::kPer])), q[i], x[s]);
+            }
+            if (!more && ahead.rounds) load_query<D>(q, a, ahead, r, g);
+            if (more || ahead.rounds) load_tile<D, RUN>(k, a.key, next, lane_at);
+            // Keys that are not there: no weight, and zeros as values (0 * NaN is NaN).
+            constexpr int kLast = Where<D, RUN>::kCount - 1;
+            bool whole = t0 + kTileKeys <= seg.end && now.there[0] && now.there[kLast];
+            if constexpr (RUN == 1) whole = __all(whole);
+            if (!whole) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const bool mine = now.there[s < kLast ? s : kLast] && t0 + 16 * s + r < seg.end;
+                    const uint32_t present = (uint32_t)__ballot(mine) >> (4 * g);
+                    clear_part<D>(v[s], mine);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[s][j] = (present >> j) & 1 ? x[s][j] : kNegInf;
                 }
             }
-            if (!there) {
-                zero_row<D>(k[s]);
-                zero_row<D>(v[s]);
+            // Values to LDS in fp16, row-major.
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < S::kChunks; ++i)
+                    *reinterpret_cast<u32x4*>(tile_lds + write_at.chunk(i) + 16 * s * 2 * D) =
+                        values_of<Half>(v[s].codes[i], scale_of(v[s].scales[i / S::kPer]));
+            if (more || ahead.rounds) load_tile<D, RUN>(v, a.value, next, lane_at);
+            // Reference and probabilities.
+            float top = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+            for (int j = 1; j < 4; ++j) top = fmaxf(top, fmaxf(x[0][j], x[1][j]));
+            top = row4_max(top) * a.scale;
+            if (__any(top > ref + kRefSlack)) {
+                const float moved = top > ref + kRefSlack ? top - kRefBelow : ref;
+                const float by = fast_exp2(ref - moved);
+                ref = moved;
+                sum *= by;
+#pragma unroll
+                for (int n = 0; n < S::kDimTiles; ++n) acc[n] *= by;
             }
-            present[s] = (uint32_t)(__ballot(there) & 0xffffu);
+            u32x4 weights;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                float p[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[j] = fast_exp2(__builtin_fmaf(x[s][j], a.scale, -ref));
+                    sum += p[j];
+                }
+                weights[2 * s] = Half::pack(p[0], p[1]);
+                weights[2 * s + 1] = Half::pack(p[2], p[3]);
+            }
+            // A wave reads only what it wrote: the LDS queue is in order, no barrier.
+#pragma unroll
+            for (int n = 0; n < S::kDimTiles; ++n) {
+                const u32x4 vt = value_operand<D>(tile_lds, read_at.chunk(2 * n));
+                acc[n] = Half::mfma16x16x32(vt, weights, acc[n]);
+            }
+            now = next;
         }
-        // Scores.
-        float x[8];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            f32x4 c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < S::kChunks; ++i)
-                c = T::mfma16x16x32(values_of<T>(k[s].codes[i], scale_of(k[s].scales[i / S::kPer])), q[i], c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[4 * s + j] = (present[s] >> (4 * g + j)) & 1 ? c[j] * a.scale : kNegInf;
+        if (idle && ahead.rounds) {
+            now = find_tile(ahead, ahead.begin + wave * kTileKeys);
+            load_query<D>(q, a, ahead, r, g);
+            load_tile<D, RUN>(k, a.key, now, lane_at);
+            load_tile<D, RUN>(v, a.value, now, lane_at);
         }
-        // Values to LDS in fp16, row-major.
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < S::kChunks; ++i)
-                *reinterpret_cast<u32x4*>(tile_lds + TileLayout<D>::at(16 * s + r, g * S::kChunks + i)) =
-                    values_of<Half>(v[s].codes[i], scale_of(v[s].scales[i / S::kPer]));
-        // Reference and probabilities.
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-        top = row4_max(top);
-        if (__any(top > ref + kRefSlack)) {
-            const float moved = top > ref + kRefSlack ? top - kRefBelow : ref;
-            const float by = fast_exp2(ref - moved);
-            ref = moved;
-            sum *= by;
-#pragma unroll
-            for (int n = 0; n < S::kDimTiles; ++n) acc[n] *= by;
-        }
-        float p[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            p[j] = fast_exp2(x[j] - ref);
-            sum += p[j];
-        }
-        const u32x4 weights = {Half::pack(p[0], p[1]), Half::pack(p[2], p[3]), Half::pack(p[4], p[5]),
-                               Half::pack(p[6], p[7])};
-        // A wave reads only what it wrote: the LDS queue is in order, no barrier.
-#pragma unroll
-        for (int n = 0; n < S::kDimTiles; ++n) {
-            const u32x4 vt = value_operand<D>(tile_lds, n, 0);
-            acc[n] = Half::mfma16x16x32(vt, weights, acc[n]);
-        }
-    }
-    sum = row4_sum(sum);
+        sum = row4_sum(sum);
 
-    // Join the waves: accumulators [16][D] in the tiles' LDS, each wave relative to its own reference.
-    __syncthreads();
-    float* mine = reinterpret_cast<float*>(tiles[wave]);
-    if (r < heads) {
+        // Join the waves: accumulators [16][D] in their tiles' LDS, each relative to its own reference.
+        const int heads = min(16, a.group - seg.tile * 16);
+        float* mine = reinterpret_cast<float*>(tile_lds);
+        if (r < heads) {
 #pragma unroll
-        for (int n = 0; n < S::kDimTiles; ++n) *reinterpret_cast<f32x4*>(mine + r * D + 16 * n + 4 * g) = acc[n];
-        if (g == 0) {
-            stats[wave][0][r] = ref;
-            stats[wave][1][r] = sum;
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < heads * D; i += 64 * S::kWaves) {
-        const int h = i / D, d = i - h * D;
-        float top = stats[0][0][h];
-#pragma unroll
-        for (int w = 1; w < S::kWaves; ++w) top = fmaxf(top, stats[w][0][h]);
-        float total = 0.f, value = 0.f;
-#pragma unroll
-        for (int w = 0; w < S::kWaves; ++w) {
-            const float by = fast_exp2(stats[w][0][h] - top);
-            total += by * stats[w][1][h];
-            value += by * reinterpret_cast<const float*>(tiles[w])[i];
-        }
-        const int64_t head = first_head + h;
-        if (a.parts == 1) {
-            static_cast<uint16_t*>(a.out)[head * D + d] = T::from_float(total != 0.f ? value / total : 0.f);
-        } else {
-            a.partial[(head * a.parts + part) * D + d] = value;
-            if (d == 0) {
-                a.partial[a.stats + (head * a.parts + part) * 2] = top;
-                a.partial[a.stats + (head * a.parts + part) * 2 + 1] = total;
+            for (int n = 0; n < S::kDimTiles; ++n) *reinterpret_cast<f32x4*>(mine + r * D + 16 * n + 4 * g) = acc[n];
+            if (g == 0) {
+                stats[wave][0][r] = ref;
+                stats[wave][1][r] = sum;
             }
         }
+        __syncthreads();
+        const int64_t first_head = (int64_t)seg.seq * a.q_heads + seg.kv_head * a.group + seg.tile * 16;
+        for (int i = threadIdx.x; i < heads * D; i += 64 * S::kWaves) {
+            const int h = i / D, d = i - h * D;
+            float top = stats[0][0][h];
+#pragma unroll
+            for (int w = 1; w < S::kWaves; ++w) top = fmaxf(top, stats[w][0][h]);
+            float total = 0.f, value = 0.f;
+#pragma unroll
+            for (int w = 0; w < S::kWaves; ++w) {
+                const float by = fast_exp2(stats[w][0][h] - top);
+                total += by * stats[w][1][h];
+                value += by * reinterpret_cast<const float*>(tiles[w])[i];
+            }
+            if (seg.slot < 0) {
+                static_cast<uint16_t*>(a.out)[first_head * D + i] = T::from_float(total != 0.f ? value / total : 0.f);
+            } else {
+                const int64_t slot = (int64_t)seg.slot * 16;
+                a.pieces[slot * D + i] = value;
+                if (d == 0) {
+                    a.pieces[a.stats + (slot + h) * 2] = top;
+                    a.pieces[a.stats + (slot + h) * 2 + 1] = total;
+                }
+            }
+        }
+        if (!ahead.rounds) return;
+        __syncthreads();  // the tiles are free again
+        seg = ahead;
+        t0 = seg.begin + wave * kTileKeys;
     }
 }
 
-// Joins the partitions of one (sequence, query head).
+// Joins the pieces of the units that share boundaries cut, and clears what has no keys; one work-group per query head.
+// The pieces go round the thread groups of D / 4 lanes; a group joins its own on the way.
+constexpr int kMergeThreads = 256;
+
 template <typename T, int D>
-__global__ __launch_bounds__(D < 64 ? 64 : D) void fp4_merge_kernel(DecodeArgs a) {
-    const int64_t head = blockIdx.x;
-    const int64_t b = head / a.q_heads;
-    const int64_t len = a.lens[b];
-    const bool usable = len > 0 && len <= (int64_t)a.width * a.div.size;
-    const int parts = usable ? ((uint32_t)len - 1) / (uint32_t)a.part_tokens + 1 : 0;
-    const float* stats = a.partial + a.stats + head * a.parts * 2;
-    const float* partial = a.partial + head * a.parts * D;
-    const int d = threadIdx.x;
-    if (d >= D) return;
-    float top = kRefNone;
-    for (int p = 0; p < parts; ++p) top = fmaxf(top, stats[2 * p]);
-    float total = 0.f, value = 0.f;
-    for (int p = 0; p < parts; ++p) {
-        const float by = fast_exp2(stats[2 * p] - top);
-        total += by * stats[2 * p + 1];
-        value += by * partial[(int64_t)p * D + d];
+__global__ __launch_bounds__(kMergeThreads) void fp4_merge_kernel(DecodeArgs a) {
+    constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
+    __shared__ __attribute__((aligned(16))) float sums[kGroups][D];
+    __shared__ float stats[kGroups][2];
+    const int head = blockIdx.x % a.q_heads, b = blockIdx.x / a.q_heads;
+    Walk<D> walk;
+    walk.count(a);
+    const int rounds = rounds_of<D>(a, a.lens[b]);
+    const int kv_head = head / a.group, in_group = head % a.group;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)blockIdx.x * D;
+    if (rounds == 0) {
+        for (int d = threadIdx.x; d < D; d += kMergeThreads) out[d] = 0;
+        return;
     }
-    static_cast<uint16_t*>(a.out)[head * D + d] = T::from_float(total != 0.f ? value / total : 0.f);
+    const int at = walk.first_of(a, b) + (kv_head * a.head_tiles + in_group / 16) * rounds;
+    const int first = at / walk.share, last = (at + rounds - 1) / walk.share;
+    if (first == last) return;  // one share has it all
+    const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    f32x4 value = {0.f, 0.f, 0.f, 0.f};
+    float ref = kRefNone, sum = 0.f;
+    if (group < kGroups) {
+        for (int i = first + group; i <= last; i += kGroups) {
+            // A piece that begins its share is in the share's first slot.
+            const int64_t slot = (int64_t)i * 2 + (i == first && at > first * walk.share ? 1 : 0);
+            const float* s = a.pieces + a.stats + (slot * 16 + in_group % 16) * 2;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(a.pieces + (slot * 16 + in_group % 16) * D + 4 * lane);
+            const float top = fmaxf(ref, s[0]), keep = fast_exp2(ref - top), by = fast_exp2(s[0] - top);
+            value = value * keep + v * by;
+            sum = sum * keep + s[1] * by;
+            ref = top;
+        }
+        *reinterpret_cast<f32x4*>(&sums[group][4 * lane]) = value;
+        if (lane == 0) {
+            stats[group][0] = ref;
+            stats[group][1] = sum;
+        }
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += kMergeThreads) {
+        float top = stats[0][0];
+#pragma unroll
+        for (int i = 1; i < kGroups; ++i) top = fmaxf(top, stats[i][0]);
+        float total = 0.f, v = 0.f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) {
+            const float by = fast_exp2(stats[i][0] - top);
+            total += by * stats[i][1];
+            v += by * sums[i][d];
+        }
+        out[d] = T::from_float(total != 0.f ? v / total : 0.f);
+    }
 }
 
 struct Plan {
-    int64_t parts, part_tokens;
+    int64_t groups;  // work-groups of the walk (0: one per unit, no workspace)
+    int64_t share;   // rounds of a share (0: by the lengths)
 };
+
+constexpr int64_t kWalkGroups = 512;   // two per CU: what LDS and registers hold at once
+constexpr int64_t kManyUnits = 2048;
+constexpr int64_t kMostRounds = int64_t(1) << 30;
 
 bool attention_dim(int64_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
 
@@ -256,42 +502,43 @@ bool decode_shape(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head
            batch <= 2147483647 / q_heads;
 }
 
-// Partitions from shapes alone (lengths stay on the device).
+// From shapes alone (lengths stay on the device).
 Plan plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t block_size, int64_t width,
           int64_t partition_tokens) {
-    const int64_t capacity = block_size * width;
-    const int64_t round = head_dim <= 128 ? 256 : 128;  // one tile for each wave
+    const int64_t capacity = block_size * width, round = head_dim <= 128 ? 256 : 128;
     const int64_t units = batch * kv_heads * ((q_heads / kv_heads + 15) / 16);
-    int64_t tokens;
+    const int64_t rounds = (capacity - 1) / round + 1;  // of a unit, at most
     if (partition_tokens > 0) {
-        tokens = (partition_tokens + kTileKeys - 1) / kTileKeys * kTileKeys;
-    } else {
-        const int64_t want = units >= 1024 ? 1 : (1024 + units - 1) / units;  // two rounds of two work-groups per CU
-        tokens = ((capacity + want - 1) / want + round - 1) / round * round;
+        const int64_t share = (partition_tokens + round - 1) / round;
+        if (share >= rounds && partition_tokens >= capacity) return {0, 0};
+        return {(units * rounds - 1) / share + 1, share};
     }
-    if (tokens > capacity) tokens = (capacity + kTileKeys - 1) / kTileKeys * kTileKeys;
-    return {(capacity - 1) / tokens + 1, tokens};
+    // Units of one round have nothing to share; many units level each other out.
+    if (rounds == 1 || units >= kManyUnits) return {0, 0};
+    return {units * rounds < kWalkGroups ? units * rounds : kWalkGroups, 0};
 }
 
 template <typename T, int D>
-int launch(const DecodeArgs& a, int64_t units, int64_t heads, hipStream_t s) {
-    hipLaunchKernelGGL((fp4_decode_kernel<T, D>), dim3((unsigned)(units * a.parts)), dim3(64 * Shape<D>::kWaves), 0, s,
-                       a);
+int launch(const DecodeArgs& a, int64_t units, hipStream_t s) {
+    const dim3 grid((unsigned)(a.groups ? a.groups : units)), block(64 * Shape<D>::kWaves);
+    if (a.div.size % 32 == 0) hipLaunchKernelGGL((fp4_decode_kernel<T, D, 32>), grid, block, 0, s, a);
+    else if (a.div.size % 16 == 0) hipLaunchKernelGGL((fp4_decode_kernel<T, D, 16>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((fp4_decode_kernel<T, D, 1>), grid, block, 0, s, a);
     if (int rc = check_launch("packed decode")) return rc;
-    if (a.parts == 1) return MVME_OK;
-    hipLaunchKernelGGL((fp4_merge_kernel<T, D>), dim3((unsigned)heads), dim3(D < 64 ? 64 : D), 0, s, a);
+    if (a.groups == 0) return MVME_OK;
+    hipLaunchKernelGGL((fp4_merge_kernel<T, D>), dim3((unsigned)(a.batch * a.q_heads)), dim3(kMergeThreads), 0, s, a);
     return check_launch("packed decode merge");
 }
 
 template <typename T>
-int launch_dim(const DecodeArgs& a, int64_t head_dim, int64_t units, int64_t heads, hipStream_t s) {
+int launch_dim(const DecodeArgs& a, int64_t head_dim, int64_t units, hipStream_t s) {
     switch (head_dim) {
-        case 32: return launch<T, 32>(a, units, heads, s);
-        case 64: return launch<T, 64>(a, units, heads, s);
-        case 96: return launch<T, 96>(a, units, heads, s);
-        case 128: return launch<T, 128>(a, units, heads, s);
-        case 192: return launch<T, 192>(a, units, heads, s);
-        default: return launch<T, 256>(a, units, heads, s);
+        case 32: return launch<T, 32>(a, units, s);
+        case 64: return launch<T, 64>(a, units, s);
+        case 96: return launch<T, 96>(a, units, s);
+        case 128: return launch<T, 128>(a, units, s);
+        case 192: return launch<T, 192>(a, units, s);
+        default: return launch<T, 256>(a, units, s);
     }
 }
 
@@ -307,7 +554,8 @@ extern "C" size_t mvme_fp4_paged_attention_workspace_size(int64_t batch, int64_t
                                                           int64_t partition_tokens) {
     if (!decode_shape(batch, q_heads, kv_heads, head_dim, block_size, table_width)) return 0;
     const Plan p = plan(batch, q_heads, kv_heads, head_dim, block_size, table_width, partition_tokens);
-    return p.parts == 1 ? 0 : (size_t)(batch * q_heads * p.parts) * (size_t)(head_dim + 2) * sizeof(float);
+    // Two pieces of up to 16 heads a share.
+    return (size_t)p.groups * 2 * 16 * (size_t)(head_dim + 2) * sizeof(float);
 }
 
 extern "C" int mvme_fp4_paged_attention(void* out, const void* query, const void* key_cache, const void* value_cache,
@@ -326,7 +574,8 @@ extern "C" int mvme_fp4_paged_attention(void* out, const void* query, const void
     if (!decode_shape(batch, q_heads, kv_heads, head_dim, block_size, table_width))
         return fail(MVME_EINVAL, "batch/head product too large");
     const int64_t record = record_bytes(block_size, head_dim);
-    if (num_blocks > (int64_t(1) << 62) / record / kv_heads) return fail(MVME_EINVAL, "KV cache too large");
+    if (num_blocks > 2147483647 || num_blocks > (int64_t(1) << 62) / record / kv_heads)
+        return fail(MVME_EINVAL, "KV cache too large");
     if (!out || !query || !key_cache || !value_cache || !block_tables || !context_lens)
         return fail(MVME_EINVAL, "packed decode: null pointer");
     if (!aligned(query, 16) || !aligned(key_cache, 16) || !aligned(value_cache, 16) || !aligned(out, 2))
@@ -334,7 +583,7 @@ extern "C" int mvme_fp4_paged_attention(void* out, const void* query, const void
     if (partition_tokens < 0) return fail(MVME_EINVAL, "partition_tokens must not be negative");
     const Plan p = plan(batch, q_heads, kv_heads, head_dim, block_size, table_width, partition_tokens);
     const int64_t tiles = (q_heads / kv_heads + 15) / 16, units = batch * kv_heads * tiles;
-    if (p.parts > 2147483647 / units) return fail(MVME_EINVAL, "too many partitions");
+    if (p.groups > kMostRounds || units > 2147483647) return fail(MVME_EINVAL, "too many partitions");
     const size_t need = mvme_fp4_paged_attention_workspace_size(batch, q_heads, kv_heads, head_dim, block_size,
                                                                 table_width, partition_tokens);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
@@ -347,20 +596,22 @@ extern "C" int mvme_fp4_paged_attention(void* out, const void* query, const void
     a.value = static_cast<const uint8_t*>(value_cache);
     a.tables = block_tables;
     a.lens = context_lens;
-    a.partial = static_cast<float*>(workspace);
+    a.pieces = static_cast<float*>(workspace);
     a.num_blocks = num_blocks;
     a.record = record;
-    a.stats = batch * q_heads * p.parts * head_dim;
+    a.page_bytes = (uint64_t)(record * kv_heads);
+    a.stats = p.groups * 2 * 16 * head_dim;
+    a.batch = (int)batch;
     a.kv_heads = (int)kv_heads;
     a.q_heads = (int)q_heads;
     a.group = (int)(q_heads / kv_heads);
     a.width = (int)table_width;
     a.head_tiles = (int)tiles;
-    a.parts = (int)p.parts;
-    a.part_tokens = (int)p.part_tokens;
+    a.groups = (int)p.groups;
+    a.share = (int)p.share;
     a.div = make_block_div(block_size);
     a.scale = kLog2e / __builtin_sqrtf((float)head_dim);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return dtype == MVME_FP16 ? launch_dim<Half>(a, head_dim, units, batch * q_heads, s)
-                              : launch_dim<BFloat16>(a, head_dim, units, batch * q_heads, s);
+    return dtype == MVME_FP16 ? launch_dim<Half>(a, head_dim, units, s)
+                              : launch_dim<BFloat16>(a, head_dim, units, s);
 }

@@ -135,6 +135,7 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         for (int n = 0; n < S::kDimTiles; ++n) acc[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     float ref[2] = {kRefNone, kRefNone}, sum[2] = {0.f, 0.f};
     const int64_t* table = a.tables + (int64_t)s * a.width;
+    const TileAddress<D> read_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
 
     for (uint32_t t0 = begin; t0 < end; t0 += kKeys) {
         __syncthreads();  // the last tile has been read
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         for (int n = 0; n < S::kDimTiles; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const u32x4 vt = value_operand<D>(values, n, 32 * h);
+                const u32x4 vt = value_operand<D>(values + 32 * h * 2 * D, read_at.chunk(2 * n));
                 acc[0][n] = Half::mfma16x16x32(vt, weights[0][h], acc[0][n]);
                 acc[1][n] = Half::mfma16x16x32(vt, weights[1][h], acc[1][n]);
             }
