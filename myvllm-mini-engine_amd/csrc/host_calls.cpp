@@ -8,6 +8,7 @@
 // return None for anything else, also for everything the entry points refuse:
 // the Python code then runs its checks in full and raises what it always
 // raised.  Nothing is kept between calls.
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -20,6 +21,7 @@
 #include <cstdint>
 #include <cstring>
 
+#include "mvme_fp4.h"
 #include "mvme_paged.h"
 
 namespace {
@@ -37,6 +39,16 @@ struct Library {
     decltype(&mvme_write_kv_cache_slots) write_slots;
     decltype(&mvme_linear_rows) linear;
     decltype(&mvme_qk_norm_rope_write_kv) rope;
+    decltype(&mvme_fp4_record_bytes) fp4_record;
+    decltype(&mvme_fp4_write_slots) fp4_write_slots;
+    decltype(&mvme_fp4_write_batch) fp4_write_batch;
+    decltype(&mvme_fp4_gather_slots) fp4_gather_slots;
+    decltype(&mvme_fp4_paged_attention_workspace_size) fp4_decode_workspace;
+    decltype(&mvme_fp4_paged_attention) fp4_decode;
+    decltype(&mvme_fp4_paged_prefill_workspace_size) fp4_prefill_workspace;
+    decltype(&mvme_fp4_paged_prefill_attention) fp4_prefill;
+    decltype(&mvme_copy_pages) copy_pages;
+    decltype(&mvme_compact_pages) compact_pages;
 } lib;
 PyObject* current_raw_stream = nullptr;  // torch's getter: device index -> hipStream_t
 
@@ -427,6 +439,225 @@ PyObject* rope_slots(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// The packed 4-bit cache and the page operators.
+// ---------------------------------------------------------------------------
+// What the entry points ask of a packed layer's caches.
+bool packed_caches(const at::Tensor& k, const at::Tensor& v, int64_t block, int64_t dim) {
+    if (k.dim() != 3 || v.sizes() != k.sizes() || k.numel() <= 0 || k.scalar_type() != at::kByte ||
+        v.scalar_type() != at::kByte || !k.is_contiguous() || !v.is_contiguous() || v.device() != k.device() ||
+        !aligned16(k) || !aligned16(v))
+        return false;
+    const int64_t record = lib.fp4_record(block, dim);
+    return record > 0 && k.size(2) == record;
+}
+
+bool index_list(const at::Tensor& t, const at::Tensor& beside) {
+    return t.scalar_type() == at::kLong && t.is_contiguous() && t.device() == beside.device();
+}
+const int64_t* indices(const at::Tensor& t) { return static_cast<const int64_t*>(t.data_ptr()); }
+
+// fp4_decode(query, key_cache, value_cache, block_tables, context_lens, block_size, partition_tokens)
+PyObject* fp4_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0, partition = 0;
+    if (n != 7 || !as_int(args[5], block) || !as_int(args[6], partition)) Py_RETURN_NONE;
+    const at::Tensor* t[5];
+    for (int i = 0; i < 5; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2], &tables = *t[3], &lens = *t[4];
+    if (!eager() || !on_current_device(q) || q.dim() != 3 || !half_type(q) || !q.is_contiguous() || q.numel() <= 0 ||
+        !aligned16(q) || k.device() != q.device() || !packed_caches(k, v, block, q.size(2)) || partition < 0)
+        Py_RETURN_NONE;
+    const int64_t batch = q.size(0), q_heads = q.size(1), kv_heads = k.size(1), d = q.size(2);
+    if (q_heads % kv_heads != 0 || (d != 32 && d != 64 && d != 96 && d != 128 && d != 192 && d != 256)) Py_RETURN_NONE;
+    if (tables.dim() != 2 || tables.size(0) != batch || tables.size(1) <= 0 || tables.size(1) > kMaxCapacity / block ||
+        lens.dim() != 1 || lens.size(0) != batch || !index_list(tables, q) || !index_list(lens, q))
+        Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(q, stream)) return nullptr;
+    at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+    const size_t need = lib.fp4_decode_workspace(batch, q_heads, kv_heads, d, block, tables.size(1), partition);
+    at::Tensor workspace;
+    if (need) workspace = bytes_like(q, need);
+    void* ws = need ? workspace.data_ptr() : nullptr;
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.fp4_decode(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), indices(tables), indices(lens),
+                            batch, q_heads, kv_heads, d, k.size(0), block, tables.size(1), partition, dtype_code(q), ws,
+                            need, stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_fp4_paged_attention", status);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// fp4_prefill(q, key_cache, value_cache, cu_seqlens_q, query_starts, block_tables, context_lens, block_size, chunk_tokens)
+PyObject* fp4_prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0, chunk = 0;
+    if (n != 9 || !as_int(args[7], block) || !as_int(args[8], chunk)) Py_RETURN_NONE;
+    const at::Tensor* t[7];
+    for (int i = 0; i < 7; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2], &cu = *t[3], &starts = *t[4], &tables = *t[5], &lens = *t[6];
+    if (!eager() || !on_current_device(q) || q.dim() != 3 || !half_type(q) || !q.is_contiguous() || q.numel() <= 0 ||
+        !aligned16(q) || k.device() != q.device() || !packed_caches(k, v, block, q.size(2)) || chunk < 0)
+        Py_RETURN_NONE;
+    const int64_t tokens = q.size(0), q_heads = q.size(1), kv_heads = k.size(1), d = q.size(2);
+    if (q_heads % kv_heads != 0 || (d != 32 && d != 64 && d != 96 && d != 128 && d != 192 && d != 256)) Py_RETURN_NONE;
+    if (cu.dim() != 1 || starts.dim() != 1 || lens.dim() != 1 || tables.dim() != 2) Py_RETURN_NONE;
+    const int64_t seqs = starts.size(0), width = tables.size(1);
+    if (seqs <= 0 || tables.size(0) != seqs || lens.size(0) != seqs || cu.size(0) != seqs + 1 || width <= 0 ||
+        width > kMaxCapacity / block)
+        Py_RETURN_NONE;
+    for (int i = 3; i < 7; ++i)
+        if (!index_list(*t[i], q)) Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(q, stream)) return nullptr;
+    at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+    const size_t need = lib.fp4_prefill_workspace(seqs, tokens, q_heads, kv_heads, d, block, width, chunk);
+    at::Tensor workspace;
+    if (need) workspace = bytes_like(q, need);
+    void* ws = need ? workspace.data_ptr() : nullptr;
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.fp4_prefill(out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), indices(cu), indices(starts),
+                             indices(tables), indices(lens), seqs, tokens, q_heads, kv_heads, d, k.size(0), block, width,
+                             chunk, dtype_code(q), ws, need, stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_fp4_paged_prefill_attention", status);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// Rows [tokens, kv_heads, head_dim] for a packed cache, and their token strides.
+bool packed_rows(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& key, const at::Tensor& value,
+                 int64_t block, int64_t& key_stride, int64_t& value_stride) {
+    if (!eager() || !on_current_device(kc) || key.dim() != 3 || value.sizes() != key.sizes() || !half_type(key) ||
+        value.scalar_type() != key.scalar_type() || key.device() != kc.device() || value.device() != kc.device() ||
+        key.size(0) <= 0 || !packed_caches(kc, vc, block, key.size(2)) || key.size(1) != kc.size(1))
+        return false;
+    key_stride = row_stride(key);
+    value_stride = row_stride(value);
+    return key_stride >= 0 && value_stride >= 0;
+}
+
+// fp4_write_slots(key_cache, value_cache, slot_mapping, key, value, block_size): True when the rows were written.
+PyObject* fp4_write_slots(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0, ks = 0, vs = 0;
+    if (n != 6 || !as_int(args[5], block)) Py_RETURN_NONE;
+    const at::Tensor* t[5];
+    for (int i = 0; i < 5; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &kc = *t[0], &vc = *t[1], &slots = *t[2], &key = *t[3], &value = *t[4];
+    if (!packed_rows(kc, vc, key, value, block, ks, vs) || slots.dim() != 1 || slots.size(0) != key.size(0) ||
+        !index_list(slots, kc))
+        Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(kc, stream)) return nullptr;
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.fp4_write_slots(kc.data_ptr(), vc.data_ptr(), kc.size(0), block, kc.size(1), key.size(2),
+                                 indices(slots), key.data_ptr(), value.data_ptr(), key.size(0), ks, vs, dtype_code(key),
+                                 stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_fp4_write_slots", status);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// fp4_write_batch(key_cache, value_cache, block_tables, token_offsets, key, value, block_size): True when written.
+PyObject* fp4_write_batch(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0, ks = 0, vs = 0;
+    if (n != 7 || !as_int(args[6], block)) Py_RETURN_NONE;
+    const at::Tensor* t[6];
+    for (int i = 0; i < 6; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &kc = *t[0], &vc = *t[1], &tables = *t[2], &offsets = *t[3], &key = *t[4], &value = *t[5];
+    if (!packed_rows(kc, vc, key, value, block, ks, vs) || tables.dim() != 2 || tables.size(0) != key.size(0) ||
+        tables.size(1) <= 0 || offsets.dim() != 1 || offsets.size(0) != key.size(0) || !index_list(tables, kc) ||
+        !index_list(offsets, kc))
+        Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(kc, stream)) return nullptr;
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.fp4_write_batch(kc.data_ptr(), vc.data_ptr(), kc.size(0), block, kc.size(1), key.size(2),
+                                 indices(tables), tables.size(1), indices(offsets), key.data_ptr(), value.data_ptr(),
+                                 key.size(0), ks, vs, dtype_code(key), stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_fp4_write_batch", status);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// fp4_gather_slots(key_cache, value_cache, slot_mapping, block_size, head_dim, dtype): (key, value) rows.
+PyObject* fp4_gather_slots(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0, dim = 0;
+    if (n != 6 || !as_int(args[3], block) || !as_int(args[4], dim) || !THPDtype_Check(args[5])) Py_RETURN_NONE;
+    const at::ScalarType type = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+    const at::Tensor* t[3];
+    for (int i = 0; i < 3; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &kc = *t[0], &vc = *t[1], &slots = *t[2];
+    if ((type != at::kHalf && type != at::kBFloat16) || !eager() || !on_current_device(kc) ||
+        !packed_caches(kc, vc, block, dim) || slots.dim() != 1 || slots.size(0) <= 0 || !index_list(slots, kc))
+        Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(kc, stream)) return nullptr;
+    const int64_t tokens = slots.size(0), heads = kc.size(1);
+    at::Tensor rows = at::empty({2, tokens, heads, dim}, kc.options().dtype(type).requires_grad(false));
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.fp4_gather_slots(rows.data_ptr(), static_cast<char*>(rows.data_ptr()) + tokens * heads * dim * 2,
+                                  kc.data_ptr(), vc.data_ptr(), kc.size(0), block, heads, dim, indices(slots), tokens,
+                                  type == at::kHalf ? MVME_FP16 : MVME_BF16, stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_fp4_gather_slots", status);
+    PyObject* key = THPVariable_Wrap(rows.select(0, 0));
+    PyObject* value = key ? THPVariable_Wrap(rows.select(0, 1)) : nullptr;
+    PyObject* both = value ? PyTuple_Pack(2, key, value) : nullptr;
+    Py_XDECREF(key);
+    Py_XDECREF(value);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// move_pages(cache, src_pages, dst_pages, block_tables or None, page_dim): True when the pages were moved.
+PyObject* move_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t dim = 0;
+    if (n != 5 || !as_int(args[4], dim)) Py_RETURN_NONE;
+    const at::Tensor *cache = plain(args[0]), *src = plain(args[1]), *dst = plain(args[2]);
+    const at::Tensor* tables = args[3] == Py_None ? nullptr : plain(args[3]);
+    if (!cache || !src || !dst || (args[3] != Py_None && !tables) || !eager() || !on_current_device(*cache))
+        Py_RETURN_NONE;
+    if (dim < 0 || dim >= cache->dim() || !cache->is_contiguous() || cache->numel() <= 0) Py_RETURN_NONE;
+    if (src->dim() != 1 || dst->sizes() != src->sizes() || src->size(0) <= 0 || src->size(0) > cache->size(dim) ||
+        !index_list(*src, *cache) || !index_list(*dst, *cache) || (tables && !index_list(*tables, *cache)))
+        Py_RETURN_NONE;
+    int64_t planes = 1;
+    for (int64_t i = 0; i < dim; ++i) planes *= cache->size(i);
+    const int64_t pages = cache->size(dim);
+    const int64_t bytes = cache->numel() / (planes * pages) * static_cast<int64_t>(cache->element_size());
+    void* stream = nullptr;
+    if (!stream_of(*cache, stream)) return nullptr;
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = tables ? lib.compact_pages(cache->data_ptr(), planes, pages, bytes, indices(*src), indices(*dst),
+                                        src->size(0), static_cast<int64_t*>(tables->data_ptr()), tables->numel(), stream)
+                    : lib.copy_pages(cache->data_ptr(), planes, pages, bytes, indices(*src), indices(*dst),
+                                     src->size(0), stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status(tables ? "mvme_compact_pages" : "mvme_copy_pages", status);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(raw_stream_getter, (address, ...)): the library's entry points in the order of Library.
 PyObject* bind(PyObject*, PyObject* args) {
     PyObject *getter = nullptr, *addresses = nullptr;
@@ -461,6 +692,12 @@ PyMethodDef methods[] = {
     {"linear", reinterpret_cast<PyCFunction>(linear), METH_FASTCALL, nullptr},
     {"rope_slots", reinterpret_cast<PyCFunction>(rope_slots), METH_FASTCALL, nullptr},
     {"write_slots", reinterpret_cast<PyCFunction>(write_slots), METH_FASTCALL, nullptr},
+    {"fp4_decode", reinterpret_cast<PyCFunction>(fp4_decode), METH_FASTCALL, nullptr},
+    {"fp4_prefill", reinterpret_cast<PyCFunction>(fp4_prefill), METH_FASTCALL, nullptr},
+    {"fp4_write_slots", reinterpret_cast<PyCFunction>(fp4_write_slots), METH_FASTCALL, nullptr},
+    {"fp4_write_batch", reinterpret_cast<PyCFunction>(fp4_write_batch), METH_FASTCALL, nullptr},
+    {"fp4_gather_slots", reinterpret_cast<PyCFunction>(fp4_gather_slots), METH_FASTCALL, nullptr},
+    {"move_pages", reinterpret_cast<PyCFunction>(move_pages), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -81,14 +81,14 @@ def source_digest() -> str:
 
 def host_digest() -> str:
     """What the native call path is built from: its source and the library's
-    header, and the torch and the Python whose headers it inlines (it reads
+    headers, and the torch and the Python whose headers it inlines (it reads
     tensors through them, so another build of either needs another module)."""
     import sysconfig
 
     import torch
 
     digest = hashlib.sha256()
-    for path in (SOURCE_DIR / "host_calls.cpp", INCLUDE_DIR / "mvme_paged.h"):
+    for path in (SOURCE_DIR / "host_calls.cpp", INCLUDE_DIR / "mvme_paged.h", INCLUDE_DIR / "mvme_fp4.h"):
         digest.update(path.read_bytes())
     for part in (torch.__version__, torch.version.git_version, torch._C._GLIBCXX_USE_CXX11_ABI,
                  sysconfig.get_config_var("EXT_SUFFIX")):

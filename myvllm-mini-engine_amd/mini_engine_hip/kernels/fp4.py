@@ -84,6 +84,8 @@ def write_kv_cache_slots_fp4(key_cache, value_cache, slot_mapping, key, value, b
     be strided views whose per-token ``[kv_heads, head_dim]`` rows are dense.
     """
     _backend(backend, "data")
+    if not validate and ext.native.fp4_write_slots(key_cache, value_cache, slot_mapping, key, value, block_size):
+        return
     if key.ndim != 3:
         raise ValueError("packed key/value must be [tokens, kv_heads, head_dim] matching the cache")
     tokens, _, head_dim = key.shape
@@ -123,6 +125,9 @@ def write_kv_cache_batch_fp4(key_cache, value_cache, block_tables, token_offsets
                              backend="hip", validate=True):
     """Decode-step write: row b goes to position ``token_offsets[b]`` of the pages ``block_tables[b]``."""
     _backend(backend, "data")
+    if not validate and ext.native.fp4_write_batch(key_cache, value_cache, block_tables, token_offsets, key, value,
+                                                   block_size):
+        return
     if key.ndim != 3:
         raise ValueError("packed key/value must be [tokens, kv_heads, head_dim] matching the cache")
     batch, _, head_dim = key.shape
@@ -167,6 +172,10 @@ def gather_kv_cache_slots_fp4(key_cache, value_cache, slot_mapping, block_size, 
     ``validate=False`` reads slots outside the pool as zeros.
     """
     _backend(backend, "data")
+    if not validate:
+        rows = ext.native.fp4_gather_slots(key_cache, value_cache, slot_mapping, block_size, head_dim, dtype)
+        if rows is not None:
+            return rows
     _check_caches(key_cache, value_cache, block_size, head_dim)
     if dtype not in _HALF:
         raise ValueError("packed KV rows require FP16/BF16")
@@ -239,6 +248,11 @@ def paged_attention_fp4(query, key_cache, value_cache, block_tables, context_len
     work-groups; ``out`` / ``workspace`` may supply the buffers.
     """
     _backend(backend, "decode")
+    if not validate and out is None and workspace is None:
+        result = ext.native.fp4_decode(query, key_cache, value_cache, block_tables, context_lens, block_size,
+                                       partition_tokens)
+        if result is not None:
+            return result
     if query.dtype not in _HALF:
         raise ValueError("HIP paged attention supports FP16/BF16")
     if query.ndim != 3 or any(size <= 0 for size in query.shape):
@@ -324,6 +338,11 @@ def paged_prefill_attention_fp4(q, key_cache, value_cache, cu_seqlens_q, query_s
     work-groups; ``workspace`` may supply the buffer for it.
     """
     _backend(backend, "prefill")
+    if not validate and workspace is None:
+        result = ext.native.fp4_prefill(q, key_cache, value_cache, cu_seqlens_q, query_starts, block_tables,
+                                        context_lens, block_size, chunk_tokens)
+        if result is not None:
+            return result
     if q.dtype not in _HALF:
         raise ValueError("HIP paged prefill requires HIP FP16/BF16")
     if q.ndim != 3 or q.shape[1] <= 0:

@@ -140,6 +140,7 @@ class NoNativeCalls:
         return None
 
     decode = decode_write = prefill = dense = linear = rope_slots = write_slots = _decline
+    fp4_decode = fp4_prefill = fp4_write_slots = fp4_write_batch = fp4_gather_slots = move_pages = _decline
 
 
 # What the entry points ask first; `load_hip_extension` puts the native call
@@ -177,7 +178,10 @@ _HOST_ENTRY_POINTS = ("mvme_last_error", "mvme_paged_attention_workspace_size", 
                       "mvme_paged_attention_decode_write", "mvme_paged_prefill_workspace_size",
                       "mvme_paged_prefill_attention", "mvme_prefill_attention_workspace_size",
                       "mvme_prefill_attention", "mvme_write_kv_cache_slots", "mvme_linear_rows",
-                      "mvme_qk_norm_rope_write_kv")
+                      "mvme_qk_norm_rope_write_kv", "mvme_fp4_record_bytes", "mvme_fp4_write_slots",
+                      "mvme_fp4_write_batch", "mvme_fp4_gather_slots", "mvme_fp4_paged_attention_workspace_size",
+                      "mvme_fp4_paged_attention", "mvme_fp4_paged_prefill_workspace_size",
+                      "mvme_fp4_paged_prefill_attention", "mvme_copy_pages", "mvme_compact_pages")
 
 
 @functools.lru_cache(maxsize=1)

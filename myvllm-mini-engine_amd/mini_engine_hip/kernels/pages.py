@@ -69,6 +69,8 @@ def copy_kv_pages(cache, src_pages, dst_pages, *, page_dim=0, backend="hip", val
     the same time); with ``validate=False`` moves with a page out of range are
     skipped, and the caller answers for the other two.
     """
+    if backend == "hip" and not validate and ext.native.move_pages(cache, src_pages, dst_pages, None, page_dim):
+        return
     planes, pages, page_bytes = _planes(cache, page_dim)
     _check_moves(cache, pages, src_pages, dst_pages, backend, validate, False)
     _need_hip(cache)
@@ -87,6 +89,9 @@ def compact_kv_pages(cache, src_pages, dst_pages, block_tables, *, page_dim=0, b
     entries, padding among them, stay.  block_tables: contiguous int64 of any
     shape, changed in place.
     """
+    if (backend == "hip" and not validate and block_tables is not None
+            and ext.native.move_pages(cache, src_pages, dst_pages, block_tables, page_dim)):
+        return
     planes, pages, page_bytes = _planes(cache, page_dim)
     _check_moves(cache, pages, src_pages, dst_pages, backend, validate, True)
     if block_tables.dtype != torch.int64 or not block_tables.is_contiguous():
