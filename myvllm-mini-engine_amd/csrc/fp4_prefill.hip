@@ -77,27 +77,46 @@ __device__ void clear_rows(const PrefillArgs& a, int kv_head) {
     }
 }
 
+// What a thread unpacks of a tile: one quarter of one token's key and value.
+template <int D>
+struct Staged {
+    uint32_t codes[2][Shape<D>::kChunks];
+    uint32_t scales[2][Shape<D>::kScales];
+    bool there;
+};
+
+// Barrier of the work-group for LDS alone: loads from memory stay in flight.
+__device__ inline void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_kernel(PrefillArgs a) {
     using S = Shape<D>;
-    __shared__ __attribute__((aligned(16))) uint8_t keys[kKeys * 2 * D];
-    __shared__ __attribute__((aligned(16))) uint8_t values[kKeys * 2 * D];
-    __shared__ uint8_t present[kKeys];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    constexpr int kPlane = kKeys * 2 * D;
+    __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][kPlane];  // [buffer][keys, values]
+    __shared__ uint8_t present[2][kKeys];
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv_head = blockIdx.x % a.kv_heads, chunk = blockIdx.x / a.kv_heads % a.chunks;
     int item = blockIdx.x / a.kv_heads / a.chunks;
     if (item == a.items - 1) {
         if (chunk == 0) clear_rows<D>(a, kv_head);
         return;
     }
-    // The sequence and the row block that `item` is.
+    // The sequence and the row block that `item` is: a sequence's blocks from the last, which sees most keys.
     Seq seq;
     int s = 0;
     for (;; ++s) {
         if (s == a.num_seqs) return;
         seq = sequence(a, s);
         const int64_t blocks = (seq.rows * a.group + kRows - 1) / kRows;
-        if (item < blocks) break;
+        if (item < blocks) {
+            item = (int)blocks - 1 - item;
+            break;
+        }
         item -= (int)blocks;
     }
     const int64_t usable = usable_keys(a, seq);
@@ -110,18 +129,85 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     const uint32_t end = min(key_end, begin + (uint32_t)a.chunk_len);
     if (chunk > 0 && begin >= end) return;
 
+    // Staging: thread -> token `row` of a tile, quarter `quarter` of its dims.  Codes are loaded a tile ahead of their
+    // unpacking and pages another tile ahead of that.
+    const int64_t* table = a.tables + (int64_t)s * a.width;
+    const int row = threadIdx.x >> 2, quarter = threadIdx.x & 3;
+    const auto page_of = [&](uint32_t t0) {
+        return table[min(a.div.page(t0 + row), (uint32_t)a.width - 1u)];
+    };
+    const auto load = [&](Staged<D>& x, uint32_t t0, int64_t page) {
+        const uint32_t token = t0 + row;
+        x.there = token < end && page >= 0 && page < a.num_blocks;
+        const uint32_t place = x.there ? token - a.div.page(token) * a.div.size : 0u;
+        const int64_t at = ((x.there ? page : 0) * a.kv_heads + kv_head) * a.record;
+#pragma unroll
+        for (int plane = 0; plane < 2; ++plane) {
+            const uint8_t* record = (plane ? a.value : a.key) + at;
+            const uint8_t* from = record + place * (D / 2) + quarter * (D / 8);
+            if constexpr (S::kChunks % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < S::kChunks; i += 4) {
+                    const u32x4 w = *reinterpret_cast<const u32x4*>(from + 4 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x.codes[plane][i + j] = w[j];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::kChunks; ++i) x.codes[plane][i] = reinterpret_cast<const uint32_t*>(from)[i];
+            }
+#pragma unroll
+            for (int i = 0; i < S::kScales; ++i)
+                x.scales[plane][i] = record[a.div.size * (D / 2) + place * (D / kBlockDims) +
+                                            (quarter * (D / 4) + 8 * i * S::kPer) / kBlockDims];
+        }
+    };
+    const TileAddress<D> stage_at(row, quarter * S::kChunks);
+    const auto unpack = [&](Staged<D>& x, int buffer) {
+        // A NaN block of the values must not reach rows that do not see its key, as 0 * NaN would: it is staged as
+        // zeros, and the key's score is NaN instead.  Absent tokens are zeros.
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < S::kScales; ++i) nan |= x.scales[1][i] == 255u;
+        nan = (__ballot(nan) >> (lane & ~3)) & 15;
+        if (__any(!x.there || nan)) {
+#pragma unroll
+            for (int plane = 0; plane < 2; ++plane) {
+#pragma unroll
+                for (int i = 0; i < S::kChunks; ++i)
+                    x.codes[plane][i] = x.there && !(plane && nan) ? x.codes[plane][i] : 0u;
+#pragma unroll
+                for (int i = 0; i < S::kScales; ++i)
+                    x.scales[plane][i] = x.there && !(plane && nan) ? x.scales[plane][i] : 127u;
+            }
+        }
+        if (quarter == 0) present[buffer][row] = x.there ? nan ? 2 : 1 : 0;
+#pragma unroll
+        for (int i = 0; i < S::kChunks; ++i) {
+            const int at = stage_at.chunk(i);
+            *reinterpret_cast<u32x4*>(tiles[buffer][0] + at) =
+                values_of<T>(x.codes[0][i], scale_of(x.scales[0][i / S::kPer]));
+            *reinterpret_cast<u32x4*>(tiles[buffer][1] + at) =
+                values_of<Half>(x.codes[1][i], scale_of(x.scales[1][i / S::kPer]));
+        }
+    };
+    Staged<D> staged;
+    int64_t page = page_of(begin);
+    load(staged, begin, page);
+    page = page_of(begin + kKeys);
+
     // This lane's rows: column r of two blocks of 16.
     int64_t head[2];
     int32_t limit[2];  // last visible key, -1 for rows without any
     u32x4 q[2][S::kChunks];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        const int64_t row = row0 + wave * 32 + c * 16 + r;
-        const bool live = row < rows;
-        const int64_t token = live ? row / a.group : 0;
+        const int64_t qrow = row0 + wave * 32 + c * 16 + r;
+        const bool live = qrow < rows;
+        const int64_t token = live ? qrow / a.group : 0;
         const int64_t pos = seq.start + token;
         limit[c] = live && pos < usable ? (int32_t)pos : -1;
-        head[c] = live ? (seq.row0 + token) * a.q_heads + (int64_t)kv_head * a.group + row % a.group : -1;
+        head[c] = live ? (seq.row0 + token) * a.q_heads + (int64_t)kv_head * a.group + qrow % a.group : -1;
 #pragma unroll
         for (int i = 0; i < S::kChunks; ++i)
             q[c][i] = live ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + head[c] * D +
@@ -134,87 +220,46 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
 #pragma unroll
         for (int n = 0; n < S::kDimTiles; ++n) acc[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     float ref[2] = {kRefNone, kRefNone}, sum[2] = {0.f, 0.f};
-    const int64_t* table = a.tables + (int64_t)s * a.width;
-    const TileAddress<D> read_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
+    TileAddress<D> key_at(r, g * S::kChunks), value_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
 
-    for (uint32_t t0 = begin; t0 < end; t0 += kKeys) {
-        __syncthreads();  // the last tile has been read
-        {
-            const int row = threadIdx.x >> 2, part = threadIdx.x & 3;
-            const uint32_t token = t0 + row;
-            uint32_t codes[2][S::kChunks], scales[2][S::kScales];
-            bool there = token < end;
-            if (there) {
-                const uint32_t block = a.div.page(token);
-                const int64_t page = table[block];
-                there = page >= 0 && page < a.num_blocks;
-                if (there) {
-                    const uint32_t place = token - block * a.div.size;
-                    const int64_t at = (page * a.kv_heads + kv_head) * a.record;
-#pragma unroll
-                    for (int plane = 0; plane < 2; ++plane) {
-                        const uint8_t* record = (plane ? a.value : a.key) + at;
-                        const uint8_t* from = record + place * (D / 2) + part * (D / 8);
-#pragma unroll
-                        for (int i = 0; i < S::kChunks; ++i)
-                            codes[plane][i] = reinterpret_cast<const uint32_t*>(from)[i];
-#pragma unroll
-                        for (int i = 0; i < S::kScales; ++i)
-                            scales[plane][i] = record[a.div.size * (D / 2) + place * (D / kBlockDims) +
-                                                      (part * (D / 4) + 8 * i * S::kPer) / kBlockDims];
-                    }
-                }
-            }
-            if (!there) {
-#pragma unroll
-                for (int plane = 0; plane < 2; ++plane) {
-#pragma unroll
-                    for (int i = 0; i < S::kChunks; ++i) codes[plane][i] = 0u;
-#pragma unroll
-                    for (int i = 0; i < S::kScales; ++i) scales[plane][i] = 127u;
-                }
-            }
-            // A NaN block of the values must not reach rows that do not see its key, as 0 * NaN would: it is staged as
-            // zeros, and the key's score is NaN instead.
-            bool nan = false;
-#pragma unroll
-            for (int i = 0; i < S::kScales; ++i) {
-                nan |= scales[1][i] == 255u;
-                scales[1][i] = scales[1][i] == 255u ? 0u : scales[1][i];
-            }
-            nan = (__ballot(nan) >> (lane & ~3)) & 15;
-            if (part == 0) present[row] = there ? nan ? 2 : 1 : 0;
-#pragma unroll
-            for (int i = 0; i < S::kChunks; ++i) {
-                const int at = TileLayout<D>::at(row, part * S::kChunks + i);
-                *reinterpret_cast<u32x4*>(keys + at) = values_of<T>(codes[0][i], scale_of(scales[0][i / S::kPer]));
-                *reinterpret_cast<u32x4*>(values + at) = values_of<Half>(codes[1][i], scale_of(scales[1][i / S::kPer]));
-            }
-        }
-        __syncthreads();
-        float x[2][16];
+    if (begin < end) {
+        unpack(staged, 0);
+        load(staged, begin + kKeys, page);
+        page = page_of(begin + 2 * kKeys);
+        lds_barrier();
+    }
+    int buffer = 0;
+#pragma unroll 1
+    for (uint32_t t0 = begin; t0 < end; t0 += kKeys, buffer ^= 1) {
+        key_at.forget();
+        value_at.forget();
+        const uint8_t* keys = tiles[buffer][0];
+        const uint8_t* values = tiles[buffer][1];
+        f32x4 x[2][4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
+            x[0][k] = x[1][k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < S::kChunks; ++i) {
-                const u32x4 kt = *reinterpret_cast<const u32x4*>(
-                    keys + TileLayout<D>::at(16 * k + r, g * S::kChunks + i));
-                c0 = T::mfma16x16x32(kt, q[0][i], c0);
-                c1 = T::mfma16x16x32(kt, q[1][i], c1);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[0][4 * k + j] = c0[j] * a.scale;
-                x[1][4 * k + j] = c1[j] * a.scale;
+                const u32x4 kt = *reinterpret_cast<const u32x4*>(keys + 16 * k * 2 * D + key_at.chunk(i));
+                x[0][k] = T::mfma16x16x32(kt, q[0][i], x[0][k]);
+                x[1][k] = T::mfma16x16x32(kt, q[1][i], x[1][k]);
             }
         }
-        const int state = present[lane];
+        const int state = present[buffer][lane];
+        // The next tile, while these scores go through the softmax.
+        if (t0 + kKeys < end) {
+            unpack(staged, buffer ^ 1);
+            load(staged, t0 + 2 * kKeys, page);
+            page = page_of(t0 + 3 * kKeys);
+        }
         const uint64_t mask = __ballot(state != 0), nans = __ballot(state == 2);
         if (nans) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-                if ((nans >> (16 * (k >> 2) + 4 * g + (k & 3))) & 1) x[0][k] = x[1][k] = __builtin_nanf("");
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if ((nans >> (16 * k + 4 * g + j)) & 1) x[0][k][j] = x[1][k][j] = __builtin_nanf("");
         }
         if (mask != ~uint64_t(0) || (int64_t)t0 + kKeys - 1 > first_pos) {
 #pragma unroll
@@ -225,16 +270,18 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
                     const bool there = (mask >> key) & 1;
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
-                        if (!there || (int32_t)(t0 + key) > limit[c]) x[c][4 * k + j] = kNegInf;
+                        if (!there || (int32_t)(t0 + key) > limit[c]) x[c][k][j] = kNegInf;
                 }
         }
         u32x4 weights[2][2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            float top = x[c][0];
+            float top = x[c][0][0];
 #pragma unroll
-            for (int j = 1; j < 16; ++j) top = fmaxf(top, x[c][j]);
-            top = row4_max(top);
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) top = fmaxf(top, x[c][k][j]);
+            top = row4_max(top) * a.scale;
             if (__any(top > ref[c] + kRefSlack)) {
                 const float moved = top > ref[c] + kRefSlack ? top - kRefBelow : ref[c];
                 const float by = fast_exp2(ref[c] - moved);
@@ -244,23 +291,26 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
                 for (int n = 0; n < S::kDimTiles; ++n) acc[c][n] *= by;
             }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                x[c][j] = fast_exp2(x[c][j] - ref[c]);
-                sum[c] += x[c][j];
+            for (int k = 0; k < 4; ++k) {
+                float p[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[j] = fast_exp2(__builtin_fmaf(x[c][k][j], a.scale, -ref[c]));
+                    sum[c] += p[j];
+                }
+                weights[c][k >> 1][2 * (k & 1)] = Half::pack(p[0], p[1]);
+                weights[c][k >> 1][2 * (k & 1) + 1] = Half::pack(p[2], p[3]);
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) weights[c][h][j] = Half::pack(x[c][8 * h + 2 * j], x[c][8 * h + 2 * j + 1]);
         }
 #pragma unroll
         for (int n = 0; n < S::kDimTiles; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const u32x4 vt = value_operand<D>(values + 32 * h * 2 * D, read_at.chunk(2 * n));
+                const u32x4 vt = value_operand<D>(values + 32 * h * 2 * D, value_at.chunk(2 * n));
                 acc[0][n] = Half::mfma16x16x32(vt, weights[0][h], acc[0][n]);
                 acc[1][n] = Half::mfma16x16x32(vt, weights[1][h], acc[1][n]);
             }
+        lds_barrier();
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
