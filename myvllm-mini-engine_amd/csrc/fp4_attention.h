@@ -32,14 +32,22 @@ constexpr float kRefNone = -3.0e38f;  // no score yet: below every finite one
 
 constexpr int kTileKeys = 32;
 
-// Byte address inside a tile of rows of 2 * D bytes: 16-byte chunks are
-// XORed with the row, so that 16 rows of one chunk fall into different banks
-// (both for writes of whole rows and for transposing reads).
+// Byte address inside a tile of rows of 2 * D bytes.  16-byte chunks are XORed
+// with a number of their row that puts these into different banks: 16 rows of
+// one chunk (or rows 0-3 and 12-15 of one and 4-11 of the next: the order in
+// which 16-byte reads are served), the chunk pairs of 8 consecutive rows that
+// a transposing read takes, and 4 rows of every fourth chunk.  Rows whose
+// length is a multiple of 256 bytes start in the same bank, of 128 bytes in
+// one of two, of 64 bytes in one of four.
 template <int D>
 struct TileLayout {
     static constexpr int kChunks = D / 8;
-    static constexpr int kMask = (kChunks & -kChunks) < 16 ? (kChunks & -kChunks) - 1 : 15;
-    __device__ static inline int at(int row, int chunk) { return row * 2 * D + ((chunk ^ (row & kMask)) << 4); }
+    __device__ static inline constexpr int number(int row) {
+        if (kChunks % 16 == 0) return 2 * (row & 7) | ((row >> 1) & 1);
+        if (kChunks % 8 == 0) return 2 * ((row >> 1) & 3) | ((row >> 2) & 1);
+        return 2 * ((row >> 2) & 1) | ((row >> 3) & 1);
+    }
+    __device__ static inline int at(int row, int chunk) { return row * 2 * D + ((chunk ^ number(row)) << 4); }
 };
 
 // A lane's place in a tile, for accesses at chunks `first + i` of its row.  For
@@ -54,9 +62,9 @@ struct TileAddress {
         base = (kPow2 ? TileLayout<D>::at(row, first) : row * 2 * D) + bytes;
     }
     __device__ inline void forget() { asm volatile("" : "+v"(base)); }
-    __device__ inline int chunk(int i) const {  // first is a multiple of the power of two above i, or i of the one above it
+    __device__ inline int chunk(int i) const {  // i and first have no bits in common
         if constexpr (kPow2) return base ^ (i << 4);
-        return base + (((first + i) ^ (row & TileLayout<D>::kMask)) << 4);
+        return base + (((first + i) ^ TileLayout<D>::number(row)) << 4);
     }
 };
 

@@ -28,6 +28,7 @@ struct PrefillArgs {
     float* partial;  // [total_tokens, q_heads, chunks, D], then [total_tokens, q_heads, chunks, 2]
     int64_t stats;
     int64_t num_blocks, record, total_tokens;
+    uint64_t page_bytes;
     int num_seqs, kv_heads, q_heads, group, width;
     int items;       // work-groups per kv head and chunk; the last one clears rows that no sequence owns
     int chunks, chunk_len;
@@ -85,6 +86,49 @@ struct Staged {
     bool there;
 };
 
+// The scores of one 16-row block in a tile become weights; accumulators follow the reference when it moves.
+template <int D>
+__device__ inline void exact_weights(const f32x4 (&x)[4], u32x4 (&weights)[2], float scale, float& ref, f32x4& sum,
+                                     f32x4 (&acc)[D / 16]) {
+    float top = x[0][0];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, x[k][j]);
+    top = row4_max(top) * scale;
+    const float moved = top > ref + kRefSlack ? top - kRefBelow : ref;
+    const float by = fast_exp2(ref - moved);
+    ref = moved;
+    sum *= by;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) acc[n] *= by;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = fast_exp2(__builtin_fmaf(x[k][j], scale, -ref));
+        weights[k >> 1][2 * (k & 1)] = Half::pack(p[0], p[1]);
+        weights[k >> 1][2 * (k & 1) + 1] = Half::pack(p[2], p[3]);
+    }
+}
+// The same against the reference as it is; false where a weight passed fp16 (or is NaN), which the one above settles.
+__device__ inline bool quick_weights(const f32x4 (&x)[4], u32x4 (&weights)[2], float scale, float ref) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = fast_exp2(__builtin_fmaf(x[k][j], scale, -ref));
+        const uint32_t lo = Half::pack(p[0], p[1]), hi = Half::pack(p[2], p[3]);
+        weights[k >> 1][2 * (k & 1)] = lo;
+        weights[k >> 1][2 * (k & 1) + 1] = hi;
+        most = __builtin_elementwise_max(most, __builtin_elementwise_max(__builtin_bit_cast(u16x2, lo),
+                                                                         __builtin_bit_cast(u16x2, hi)));
+    }
+    return max(most[0], most[1]) < 0x7c00;
+}
+
 // Barrier of the work-group for LDS alone: loads from memory stay in flight.
 __device__ inline void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -92,12 +136,13 @@ __device__ inline void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <typename T, int D>
+template <typename T, int D, int RUN>
 __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_kernel(PrefillArgs a) {
     using S = Shape<D>;
     constexpr int kPlane = kKeys * 2 * D;
     __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][kPlane];  // [buffer][keys, values]
-    __shared__ uint8_t present[2][kKeys];
+    __shared__ uint8_t present[2][kKeys];       // 1: there, 2: there and its value has a NaN
+    __shared__ __attribute__((aligned(4))) uint8_t odd[2][4];  // per wave's 16 tokens: whether any is not 1
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv_head = blockIdx.x % a.kv_heads, chunk = blockIdx.x / a.kv_heads % a.chunks;
@@ -129,22 +174,32 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     const uint32_t end = min(key_end, begin + (uint32_t)a.chunk_len);
     if (chunk > 0 && begin >= end) return;
 
-    // Staging: thread -> token `row` of a tile, quarter `quarter` of its dims.  Codes are loaded a tile ahead of their
-    // unpacking and pages another tile ahead of that.
+    // Staging: thread -> token `row` of a tile, quarter `quarter` of its dims; a wave has 16 consecutive tokens.  RUN 16
+    // (block sizes that are multiples of 16): they lie in one page at consecutive places, looked up once per wave.
+    // Codes are loaded a tile ahead of their unpacking, and pages another tile ahead of that.
     const int64_t* table = a.tables + (int64_t)s * a.width;
     const int row = threadIdx.x >> 2, quarter = threadIdx.x & 3;
+    const uint32_t looked = RUN == 16 ? 16 * wave : row;  // the token of the tile that is looked up
     const auto page_of = [&](uint32_t t0) {
-        return table[min(a.div.page(t0 + row), (uint32_t)a.width - 1u)];
+        const int64_t* entry = table + min(a.div.page(t0 + looked), (uint32_t)a.width - 1u);
+        return RUN == 16 ? uniform_load(entry) : *entry;
     };
+    uint32_t code_at = (RUN == 16 ? (row & 15) * (D / 2) : 0) + quarter * (D / 8);
+    uint32_t scale_at[S::kScales];
+#pragma unroll
+    for (int i = 0; i < S::kScales; ++i)
+        scale_at[i] = (RUN == 16 ? (row & 15) * (D / kBlockDims) : 0) + (quarter * (D / 4) + 8 * i * S::kPer) / kBlockDims;
     const auto load = [&](Staged<D>& x, uint32_t t0, int64_t page) {
-        const uint32_t token = t0 + row;
-        x.there = token < end && page >= 0 && page < a.num_blocks;
-        const uint32_t place = x.there ? token - a.div.page(token) * a.div.size : 0u;
-        const int64_t at = ((x.there ? page : 0) * a.kv_heads + kv_head) * a.record;
+        const uint32_t token = t0 + looked;
+        const bool found = token < end && (uint64_t)page < (uint64_t)a.num_blocks;
+        x.there = found && t0 + row < end;
+        const uint32_t place = found ? token - a.div.page(token) * a.div.size : 0u;
+        const int64_t at = kv_head * a.record + (int64_t)((uint64_t)(uint32_t)(found ? page : 0) * a.page_bytes) + place * (D / 2);
+        const uint32_t to_scales = a.div.size * (D / 2) - place * (D / 2 - D / kBlockDims);
 #pragma unroll
         for (int plane = 0; plane < 2; ++plane) {
-            const uint8_t* record = (plane ? a.value : a.key) + at;
-            const uint8_t* from = record + place * (D / 2) + quarter * (D / 8);
+            const uint8_t* base = (plane ? a.value : a.key) + at;
+            const uint8_t* from = base + code_at;
             if constexpr (S::kChunks % 4 == 0) {
 #pragma unroll
                 for (int i = 0; i < S::kChunks; i += 4) {
@@ -157,31 +212,30 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
                 for (int i = 0; i < S::kChunks; ++i) x.codes[plane][i] = reinterpret_cast<const uint32_t*>(from)[i];
             }
 #pragma unroll
-            for (int i = 0; i < S::kScales; ++i)
-                x.scales[plane][i] = record[a.div.size * (D / 2) + place * (D / kBlockDims) +
-                                            (quarter * (D / 4) + 8 * i * S::kPer) / kBlockDims];
+            for (int i = 0; i < S::kScales; ++i) x.scales[plane][i] = base[scale_at[i] + to_scales];
         }
     };
-    const TileAddress<D> stage_at(row, quarter * S::kChunks);
+    TileAddress<D> stage_at(row, quarter * S::kChunks);
     const auto unpack = [&](Staged<D>& x, int buffer) {
         // A NaN block of the values must not reach rows that do not see its key, as 0 * NaN would: it is staged as
         // zeros, and the key's score is NaN instead.  Absent tokens are zeros.
         bool nan = false;
 #pragma unroll
         for (int i = 0; i < S::kScales; ++i) nan |= x.scales[1][i] == 255u;
-        nan = (__ballot(nan) >> (lane & ~3)) & 15;
-        if (__any(!x.there || nan)) {
+        const bool some = __any(!x.there || nan);
+        if (some) {
+            nan = (__ballot(nan) >> (lane & ~3)) & 15;
 #pragma unroll
             for (int plane = 0; plane < 2; ++plane) {
+                const bool keep = x.there && !(plane && nan);
 #pragma unroll
-                for (int i = 0; i < S::kChunks; ++i)
-                    x.codes[plane][i] = x.there && !(plane && nan) ? x.codes[plane][i] : 0u;
+                for (int i = 0; i < S::kChunks; ++i) x.codes[plane][i] = keep ? x.codes[plane][i] : 0u;
 #pragma unroll
-                for (int i = 0; i < S::kScales; ++i)
-                    x.scales[plane][i] = x.there && !(plane && nan) ? x.scales[plane][i] : 127u;
+                for (int i = 0; i < S::kScales; ++i) x.scales[plane][i] = keep ? x.scales[plane][i] : 127u;
             }
+            if (quarter == 0) present[buffer][row] = x.there ? nan ? 2 : 1 : 0;
         }
-        if (quarter == 0) present[buffer][row] = x.there ? nan ? 2 : 1 : 0;
+        if (lane == 0) odd[buffer][wave] = some;
 #pragma unroll
         for (int i = 0; i < S::kChunks; ++i) {
             const int at = stage_at.chunk(i);
@@ -211,7 +265,7 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
 #pragma unroll
         for (int i = 0; i < S::kChunks; ++i)
             q[c][i] = live ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + head[c] * D +
-                                                             g * (D / 4) + 8 * i)
+                                                             32 * i + 8 * g)
                            : u32x4{0u, 0u, 0u, 0u};
     }
     f32x4 acc[2][S::kDimTiles];
@@ -219,8 +273,9 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int n = 0; n < S::kDimTiles; ++n) acc[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float ref[2] = {kRefNone, kRefNone}, sum[2] = {0.f, 0.f};
-    TileAddress<D> key_at(r, g * S::kChunks), value_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
+    float ref[2] = {kRefNone, kRefNone};
+    f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // each element is the sum of all keys' weights
+    TileAddress<D> key_at(r, g), value_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
 
     if (begin < end) {
         unpack(staged, 0);
@@ -233,6 +288,10 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     for (uint32_t t0 = begin; t0 < end; t0 += kKeys, buffer ^= 1) {
         key_at.forget();
         value_at.forget();
+        stage_at.forget();
+        asm volatile("" : "+v"(code_at));
+#pragma unroll
+        for (int i = 0; i < S::kScales; ++i) asm volatile("" : "+v"(scale_at[i]));
         const uint8_t* keys = tiles[buffer][0];
         const uint8_t* values = tiles[buffer][1];
         f32x4 x[2][4];
@@ -241,25 +300,29 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
             x[0][k] = x[1][k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < S::kChunks; ++i) {
-                const u32x4 kt = *reinterpret_cast<const u32x4*>(keys + 16 * k * 2 * D + key_at.chunk(i));
+                const u32x4 kt = *reinterpret_cast<const u32x4*>(keys + 16 * k * 2 * D + key_at.chunk(4 * i));
                 x[0][k] = T::mfma16x16x32(kt, q[0][i], x[0][k]);
                 x[1][k] = T::mfma16x16x32(kt, q[1][i], x[1][k]);
             }
         }
-        const int state = present[buffer][lane];
-        // The next tile, while these scores go through the softmax.
-        if (t0 + kKeys < end) {
-            unpack(staged, buffer ^ 1);
-            load(staged, t0 + 2 * kKeys, page);
-            page = page_of(t0 + 3 * kKeys);
-        }
-        const uint64_t mask = __ballot(state != 0), nans = __ballot(state == 2);
-        if (nans) {
+        const uint32_t odds = (uint32_t)__builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(odd[buffer]));
+        uint64_t mask = ~uint64_t(0);
+        if (odds) {
+            // (Only waves with something odd wrote their tokens' states.)
+            const int state = (odds >> (8 * (lane >> 4))) & 0xff ? present[buffer][lane] : 1;
+            mask = __ballot(state != 0);
+            const uint64_t nans = __ballot(state == 2);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if ((nans >> (16 * k + 4 * g + j)) & 1) x[0][k][j] = x[1][k][j] = __builtin_nanf("");
+        }
+        // The next tile, while these scores go through the softmax.
+        if (t0 + kKeys < end) {
+            unpack(staged, buffer ^ 1);
+            load(staged, t0 + 2 * kKeys, page);
+            page = page_of(t0 + 3 * kKeys);
         }
         if (mask != ~uint64_t(0) || (int64_t)t0 + kKeys - 1 > first_pos) {
 #pragma unroll
@@ -276,30 +339,13 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         u32x4 weights[2][2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            float top = x[c][0][0];
+            if (__any(!quick_weights(x[c], weights[c], a.scale, ref[c])))
+                exact_weights<D>(x[c], weights[c], a.scale, ref[c], sum[c], acc[c]);
+            // The sums by a product with ones: the matrix cores have room where the vector units do not.
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, x[c][k][j]);
-            top = row4_max(top) * a.scale;
-            if (__any(top > ref[c] + kRefSlack)) {
-                const float moved = top > ref[c] + kRefSlack ? top - kRefBelow : ref[c];
-                const float by = fast_exp2(ref[c] - moved);
-                ref[c] = moved;
-                sum[c] *= by;
-#pragma unroll
-                for (int n = 0; n < S::kDimTiles; ++n) acc[c][n] *= by;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float p[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    p[j] = fast_exp2(__builtin_fmaf(x[c][k][j], a.scale, -ref[c]));
-                    sum[c] += p[j];
-                }
-                weights[c][k >> 1][2 * (k & 1)] = Half::pack(p[0], p[1]);
-                weights[c][k >> 1][2 * (k & 1) + 1] = Half::pack(p[2], p[3]);
+            for (int h = 0; h < 2; ++h) {
+                constexpr uint32_t kOnes = 0x3c003c00u;
+                sum[c] = Half::mfma16x16x32(u32x4{kOnes, kOnes, kOnes, kOnes}, weights[c][h], sum[c]);
             }
         }
 #pragma unroll
@@ -314,7 +360,7 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        const float total = row4_sum(sum[c]);
+        const float total = sum[c][0];
         if (head[c] < 0) continue;
         if (a.chunks == 1) {
             const float by = 1.f / total;
@@ -398,8 +444,9 @@ Plan plan(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, in
 
 template <typename T, int D>
 int launch(const PrefillArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((fp4_prefill_kernel<T, D>), dim3((unsigned)((int64_t)a.items * a.chunks * a.kv_heads)),
-                       dim3(kThreads), 0, s, a);
+    const dim3 grid((unsigned)((int64_t)a.items * a.chunks * a.kv_heads)), block(kThreads);
+    if (a.div.size % 16 == 0) hipLaunchKernelGGL((fp4_prefill_kernel<T, D, 16>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((fp4_prefill_kernel<T, D, 1>), grid, block, 0, s, a);
     if (int rc = check_launch("packed prefill")) return rc;
     if (a.chunks == 1) return MVME_OK;
     hipLaunchKernelGGL((fp4_prefill_merge_kernel<T, D>), dim3((unsigned)(a.total_tokens * a.q_heads)), dim3(64), 0, s,
@@ -454,7 +501,8 @@ extern "C" int mvme_fp4_paged_prefill_attention(void* out, const void* q, const 
     if (!prefill_shape(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width))
         return fail(MVME_EINVAL, "too many packed query rows");
     const int64_t record = record_bytes(block_size, head_dim);
-    if (num_blocks > (int64_t(1) << 62) / record / kv_heads) return fail(MVME_EINVAL, "KV cache too large");
+    if (num_blocks > 2147483647 || num_blocks > (int64_t(1) << 62) / record / kv_heads)
+        return fail(MVME_EINVAL, "KV cache too large");
     if (chunk_tokens < 0) return fail(MVME_EINVAL, "chunk_tokens must not be negative");
     if (total_tokens == 0) return MVME_OK;
     if (!out || !q || !key_cache || !value_cache || !cu_seqlens_q || !query_starts || !block_tables || !context_lens)
@@ -481,6 +529,7 @@ extern "C" int mvme_fp4_paged_prefill_attention(void* out, const void* q, const 
     a.stats = total_tokens * q_heads * p.chunks * head_dim;
     a.num_blocks = num_blocks;
     a.record = record;
+    a.page_bytes = (uint64_t)(record * kv_heads);
     a.total_tokens = total_tokens;
     a.num_seqs = (int)num_seqs;
     a.kv_heads = (int)kv_heads;
