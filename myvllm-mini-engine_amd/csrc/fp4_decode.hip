@@ -270,7 +270,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, Shape<D>::kMinWaves) void fp
         return s;
     };
 
-    TileAddress<D> write_at(r, g * S::kChunks), read_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
+    TileAddress<D, 16> write_at(r, g * S::kChunks), read_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
     LaneAt<D, RUN> lane_at(r, g);
     uint8_t* tile_lds = tiles[wave];
     // A tile's registers are refilled as soon as they are used up: keys after
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, Shape<D>::kMinWaves) void fp
             // A wave reads only what it wrote: the LDS queue is in order, no barrier.
 #pragma unroll
             for (int n = 0; n < S::kDimTiles; ++n) {
-                const u32x4 vt = value_operand<D>(tile_lds, read_at.chunk(2 * n));
+                const u32x4 vt = value_operand(tile_lds, read_at.chunk(2 * n), read_at.chunk(2 * n) + 16 * 2 * D);
                 acc[n] = Half::mfma16x16x32(vt, weights, acc[n]);
             }
             now = next;

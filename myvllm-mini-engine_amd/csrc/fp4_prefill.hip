@@ -16,6 +16,8 @@ constexpr int kThreads = 256;
 constexpr int kRows = 128;   // query rows of a work-group
 constexpr int kKeys = 64;    // keys of a tile
 
+constexpr int kMfma = 0x8, kDsRead = 0x100;  // kinds of instructions for the scheduler
+
 struct PrefillArgs {
     void* out;
     const void* q;
@@ -41,9 +43,19 @@ struct Shape {
     static constexpr int kChunks = D / 32;
     static constexpr int kPer = D % 128 == 0 ? 4 : D == 64 || D == 192 ? 2 : 1;
     static constexpr int kScales = kChunks / kPer;
-    static constexpr int kDimTiles = D / 16;
+    static constexpr int kBlocks = D / 32;   // 32-dim blocks of the output
+    static constexpr int kSteps = D / 16;    // score products per 32 keys
     static constexpr int kMinWaves = D <= 128 ? 2 : 1;
 };
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <typename T>
+__device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (T::kId == MVME_FP16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
 
 struct Seq {
     int64_t row0, rows, start, len;
@@ -86,47 +98,45 @@ struct Staged {
     bool there;
 };
 
-// The scores of one 16-row block in a tile become weights; accumulators follow the reference when it moves.
-template <int D>
-__device__ inline void exact_weights(const f32x4 (&x)[4], u32x4 (&weights)[2], float scale, float& ref, f32x4& sum,
-                                     f32x4 (&acc)[D / 16]) {
+// The scores of a tile become weights, four products' operands, and add to the sum.  Against the reference as it is; false
+// where a weight passed fp16 (or is NaN): nothing but `weights` is written then.
+__device__ inline bool quick_weights(const f32x16 (&x)[2], u32x4 (&weights)[4], float scale, float ref) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float p0 = fast_exp2(__builtin_fmaf(x[m >> 1][8 * (m & 1) + 2 * j], scale, -ref));
+            const float p1 = fast_exp2(__builtin_fmaf(x[m >> 1][8 * (m & 1) + 2 * j + 1], scale, -ref));
+            weights[m][j] = Half::pack(p0, p1);
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, weights[m][j]));
+        }
+    return max(most[0], most[1]) < 0x7c00;
+}
+// The same after moving the reference to the scores; accumulators follow.
+template <int BLOCKS>
+__device__ inline void exact_weights(const f32x16 (&x)[2], u32x4 (&weights)[4], float scale, float& ref, float& sum,
+                                     f32x16 (&acc)[BLOCKS]) {
     float top = x[0][0];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, x[k][j]);
-    top = row4_max(top) * scale;
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i >> 4][i & 15]);
+    top = pair32_max(top) * scale;
     const float moved = top > ref + kRefSlack ? top - kRefBelow : ref;
     const float by = fast_exp2(ref - moved);
     ref = moved;
     sum *= by;
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n) acc[n] *= by;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float p[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = fast_exp2(__builtin_fmaf(x[k][j], scale, -ref));
-        weights[k >> 1][2 * (k & 1)] = Half::pack(p[0], p[1]);
-        weights[k >> 1][2 * (k & 1) + 1] = Half::pack(p[2], p[3]);
-    }
+    for (int n = 0; n < BLOCKS; ++n) acc[n] *= by;
+    quick_weights(x, weights, scale, ref);
 }
-// The same against the reference as it is; false where a weight passed fp16 (or is NaN), which the one above settles.
-__device__ inline bool quick_weights(const f32x4 (&x)[4], u32x4 (&weights)[2], float scale, float ref) {
-    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-    u16x2 most = {0, 0};
+// Sum of the weights, as rounded.
+__device__ inline float add_weights(const u32x4 (&weights)[4], float sum) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        float p[4];
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = fast_exp2(__builtin_fmaf(x[k][j], scale, -ref));
-        const uint32_t lo = Half::pack(p[0], p[1]), hi = Half::pack(p[2], p[3]);
-        weights[k >> 1][2 * (k & 1)] = lo;
-        weights[k >> 1][2 * (k & 1) + 1] = hi;
-        most = __builtin_elementwise_max(most, __builtin_elementwise_max(__builtin_bit_cast(u16x2, lo),
-                                                                         __builtin_bit_cast(u16x2, hi)));
-    }
-    return max(most[0], most[1]) < 0x7c00;
+        for (int j = 0; j < 4; ++j) sum = Half::dot2(weights[m][j], 0x3c003c00u, sum);
+    return sum;
 }
 
 // Barrier of the work-group for LDS alone: loads from memory stay in flight.
@@ -143,7 +153,7 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     __shared__ __attribute__((aligned(16))) uint8_t tiles[2][2][kPlane];  // [buffer][keys, values]
     __shared__ uint8_t present[2][kKeys];       // 1: there, 2: there and its value has a NaN
     __shared__ __attribute__((aligned(4))) uint8_t odd[2][4];  // per wave's 16 tokens: whether any is not 1
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, column = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv_head = blockIdx.x % a.kv_heads, chunk = blockIdx.x / a.kv_heads % a.chunks;
     int item = blockIdx.x / a.kv_heads / a.chunks;
@@ -178,7 +188,8 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     // (block sizes that are multiples of 16): they lie in one page at consecutive places, looked up once per wave.
     // Codes are loaded a tile ahead of their unpacking, and pages another tile ahead of that.
     const int64_t* table = a.tables + (int64_t)s * a.width;
-    const int row = threadIdx.x >> 2, quarter = threadIdx.x & 3;
+    // (The order of the tokens in a wave puts four that share a bank into one 16-byte access: TileLayout.)
+    const int row = 16 * wave + 4 * ((lane >> 2) & 3) + (lane >> 4), quarter = lane & 3;
     const uint32_t looked = RUN == 16 ? 16 * wave : row;  // the token of the tile that is looked up
     const auto page_of = [&](uint32_t t0) {
         const int64_t* entry = table + min(a.div.page(t0 + looked), (uint32_t)a.width - 1u);
@@ -215,7 +226,7 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
             for (int i = 0; i < S::kScales; ++i) x.scales[plane][i] = base[scale_at[i] + to_scales];
         }
     };
-    TileAddress<D> stage_at(row, quarter * S::kChunks);
+    TileAddress<D, 32> stage_at(row, quarter * S::kChunks);
     const auto unpack = [&](Staged<D>& x, int buffer) {
         // A NaN block of the values must not reach rows that do not see its key, as 0 * NaN would: it is staged as
         // zeros, and the key's score is NaN instead.  Absent tokens are zeros.
@@ -250,32 +261,25 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     load(staged, begin, page);
     page = page_of(begin + kKeys);
 
-    // This lane's rows: column r of two blocks of 16.
-    int64_t head[2];
-    int32_t limit[2];  // last visible key, -1 for rows without any
-    u32x4 q[2][S::kChunks];
+    // This lane's row.
+    const int64_t qrow = row0 + wave * 32 + column;
+    const bool live = qrow < rows;
+    const int64_t token = live ? qrow / a.group : 0;
+    const int32_t limit = live && seq.start + token < usable ? (int32_t)(seq.start + token) : -1;  // last visible key
+    const int64_t head = (seq.row0 + token) * a.q_heads + (int64_t)kv_head * a.group + (live ? qrow % a.group : 0);
+    u32x4 q[S::kSteps];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const int64_t qrow = row0 + wave * 32 + c * 16 + r;
-        const bool live = qrow < rows;
-        const int64_t token = live ? qrow / a.group : 0;
-        const int64_t pos = seq.start + token;
-        limit[c] = live && pos < usable ? (int32_t)pos : -1;
-        head[c] = live ? (seq.row0 + token) * a.q_heads + (int64_t)kv_head * a.group + qrow % a.group : -1;
+    for (int i = 0; i < S::kSteps; ++i)
+        q[i] = live ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + head * D + 16 * i + 8 * h)
+                    : u32x4{0u, 0u, 0u, 0u};
+    f32x16 acc[S::kBlocks];
 #pragma unroll
-        for (int i = 0; i < S::kChunks; ++i)
-            q[c][i] = live ? *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + head[c] * D +
-                                                             32 * i + 8 * g)
-                           : u32x4{0u, 0u, 0u, 0u};
-    }
-    f32x4 acc[2][S::kDimTiles];
+    for (int n = 0; n < S::kBlocks; ++n)
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int n = 0; n < S::kDimTiles; ++n) acc[c][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float ref[2] = {kRefNone, kRefNone};
-    f32x4 sum[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // each element is the sum of all keys' weights
-    TileAddress<D> key_at(r, g), value_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
+        for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+    float ref = kRefNone, sum = 0.f;
+    TileAddress<D, 32> key_at(column, h);
+    TileAddress<D, 32> value_at(4 * h + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), (lane & 1) * 8);
 
     if (begin < end) {
         unpack(staged, 0);
@@ -294,17 +298,23 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         for (int i = 0; i < S::kScales; ++i) asm volatile("" : "+v"(scale_at[i]));
         const uint8_t* keys = tiles[buffer][0];
         const uint8_t* values = tiles[buffer][1];
-        f32x4 x[2][4];
+        f32x16 x[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            x[0][k] = x[1][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 2; ++k) {
 #pragma unroll
-            for (int i = 0; i < S::kChunks; ++i) {
-                const u32x4 kt = *reinterpret_cast<const u32x4*>(keys + 16 * k * 2 * D + key_at.chunk(4 * i));
-                x[0][k] = T::mfma16x16x32(kt, q[0][i], x[0][k]);
-                x[1][k] = T::mfma16x16x32(kt, q[1][i], x[1][k]);
-            }
+            for (int i = 0; i < 16; ++i) x[k][i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::kSteps; ++i)
+                x[k] = mfma32<T>(*reinterpret_cast<const u32x4*>(keys + 32 * k * 2 * D + key_at.chunk(2 * i)), q[i], x[k]);
         }
+        // Reads run four products ahead.
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * S::kSteps - 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
         const uint32_t odds = (uint32_t)__builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(odd[buffer]));
         uint64_t mask = ~uint64_t(0);
         if (odds) {
@@ -313,10 +323,12 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
             mask = __ballot(state != 0);
             const uint64_t nans = __ballot(state == 2);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t bits = (uint32_t)(nans >> (32 * k)) >> (4 * h);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if ((nans >> (16 * k + 4 * g + j)) & 1) x[0][k][j] = x[1][k][j] = __builtin_nanf("");
+                for (int i = 0; i < 16; ++i)
+                    if ((bits >> (8 * (i >> 2) + (i & 3))) & 1) x[k][i] = __builtin_nanf("");
+            }
         }
         // The next tile, while these scores go through the softmax.
         if (t0 + kKeys < end) {
@@ -325,59 +337,53 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
             page = page_of(t0 + 3 * kKeys);
         }
         if (mask != ~uint64_t(0) || (int64_t)t0 + kKeys - 1 > first_pos) {
+            const int32_t seen = limit - (int32_t)t0 - 4 * h;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t bits = (uint32_t)(mask >> (32 * k)) >> (4 * h);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int key = 16 * k + 4 * g + j;
-                    const bool there = (mask >> key) & 1;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        if (!there || (int32_t)(t0 + key) > limit[c]) x[c][k][j] = kNegInf;
+                for (int i = 0; i < 16; ++i) {
+                    const int key = 8 * (i >> 2) + (i & 3);
+                    if (!((bits >> key) & 1) || 32 * k + key > seen) x[k][i] = kNegInf;
                 }
-        }
-        u32x4 weights[2][2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (__any(!quick_weights(x[c], weights[c], a.scale, ref[c])))
-                exact_weights<D>(x[c], weights[c], a.scale, ref[c], sum[c], acc[c]);
-            // The sums by a product with ones: the matrix cores have room where the vector units do not.
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                constexpr uint32_t kOnes = 0x3c003c00u;
-                sum[c] = Half::mfma16x16x32(u32x4{kOnes, kOnes, kOnes, kOnes}, weights[c][h], sum[c]);
             }
         }
+        u32x4 weights[4];
+        if (__any(!quick_weights(x, weights, a.scale, ref))) exact_weights(x, weights, a.scale, ref, sum, acc);
+        sum = add_weights(weights, sum);
 #pragma unroll
-        for (int n = 0; n < S::kDimTiles; ++n)
+        for (int n = 0; n < S::kBlocks; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 vt = value_operand<D>(values + 32 * h * 2 * D, value_at.chunk(2 * n));
-                acc[0][n] = Half::mfma16x16x32(vt, weights[0][h], acc[0][n]);
-                acc[1][n] = Half::mfma16x16x32(vt, weights[1][h], acc[1][n]);
-            }
+            for (int m = 0; m < 4; ++m)
+                // (Eight rows on, the row's number differs in bit 1.)
+                acc[n] = mfma32<Half>(value_operand(values + 16 * m * 2 * D, value_at.chunk(4 * n),
+                                                    value_at.chunk(4 * n, 2) + 8 * 2 * D), weights[m], acc[n]);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 1);
+#pragma unroll
+        for (int i = 0; i < 4 * S::kBlocks - 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 1);
         lds_barrier();
     }
+    const float total = swap32_add(sum, sum);  // the other half of the keys is with the lane 32 away
+    if (!live) return;
+    const int64_t at = head * a.chunks + chunk;
+    const float by = 1.f / total;
+    const bool zero = limit < 0 || total == 0.f;  // a row that sees no key
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const float total = sum[c][0];
-        if (head[c] < 0) continue;
-        if (a.chunks == 1) {
-            const float by = 1.f / total;
-            const bool zero = limit[c] < 0 || total == 0.f;  // a row that sees no key
+    for (int n = 0; n < S::kBlocks; ++n)
 #pragma unroll
-            for (int n = 0; n < S::kDimTiles; ++n)
-                store4<T, D>(a, head[c], 16 * n + 4 * g, zero ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[c][n] * by);
-        } else {
-            const int64_t at = head[c] * a.chunks + chunk;
-#pragma unroll
-            for (int n = 0; n < S::kDimTiles; ++n)
-                *reinterpret_cast<f32x4*>(a.partial + at * D + 16 * n + 4 * g) = acc[c][n];
-            if (g == 0) {
-                a.partial[a.stats + at * 2] = ref[c];
-                a.partial[a.stats + at * 2 + 1] = total;
-            }
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 v = {acc[n][4 * i], acc[n][4 * i + 1], acc[n][4 * i + 2], acc[n][4 * i + 3]};
+            const int d = 32 * n + 8 * i + 4 * h;
+            if (a.chunks == 1) store4<T, D>(a, head, d, zero ? f32x4{0.f, 0.f, 0.f, 0.f} : v * by);
+            else *reinterpret_cast<f32x4*>(a.partial + at * D + d) = v;
         }
+    if (a.chunks > 1 && h == 0) {
+        a.partial[a.stats + at * 2] = ref;
+        a.partial[a.stats + at * 2 + 1] = total;
     }
 }
 
