@@ -98,26 +98,18 @@ struct Staged {
     bool there;
 };
 
-// The scores of a tile become weights, four products' operands, and add to the sum.  Against the reference as it is; false
-// where a weight passed fp16 (or is NaN): nothing but `weights` is written then.
-__device__ inline bool quick_weights(const f32x16 (&x)[2], u32x4 (&weights)[4], float scale, float ref) {
-    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-    u16x2 most = {0, 0};
+constexpr float kLargest = 15.999f;  // log2 of a weight that fp16 holds (65519 is the last to round down)
+// Whether no score of the tile gives a weight past fp16 against the reference (a NaN does not count).
+__device__ inline bool weights_fit(const f32x16 (&x)[2], float scale, float ref) {
+    float top = x[0][0];
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float p0 = fast_exp2(__builtin_fmaf(x[m >> 1][8 * (m & 1) + 2 * j], scale, -ref));
-            const float p1 = fast_exp2(__builtin_fmaf(x[m >> 1][8 * (m & 1) + 2 * j + 1], scale, -ref));
-            weights[m][j] = Half::pack(p0, p1);
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, weights[m][j]));
-        }
-    return max(most[0], most[1]) < 0x7c00;
+    for (int i = 1; i < 31; i += 2) top = fmaxf(fmaxf(top, x[i >> 4][i & 15]), x[(i + 1) >> 4][(i + 1) & 15]);
+    top = fmaxf(top, x[1][15]);
+    return __builtin_fmaf(top, scale, -ref) <= kLargest;
 }
-// The same after moving the reference to the scores; accumulators follow.
+// Moves the reference to the scores; sum and accumulators follow.
 template <int BLOCKS>
-__device__ inline void exact_weights(const f32x16 (&x)[2], u32x4 (&weights)[4], float scale, float& ref, float& sum,
-                                     f32x16 (&acc)[BLOCKS]) {
+__device__ inline void move_reference(const f32x16 (&x)[2], float scale, float& ref, float& sum, f32x16 (&acc)[BLOCKS]) {
     float top = x[0][0];
 #pragma unroll
     for (int i = 0; i < 32; ++i) top = fmaxf(top, x[i >> 4][i & 15]);
@@ -128,7 +120,17 @@ __device__ inline void exact_weights(const f32x16 (&x)[2], u32x4 (&weights)[4], 
     sum *= by;
 #pragma unroll
     for (int n = 0; n < BLOCKS; ++n) acc[n] *= by;
-    quick_weights(x, weights, scale, ref);
+}
+// The scores of a tile become weights, four products' operands.
+__device__ inline void weigh(const f32x16 (&x)[2], u32x4 (&weights)[4], float scale, float ref) {
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float p0 = fast_exp2(__builtin_fmaf(x[m >> 1][8 * (m & 1) + 2 * j], scale, -ref));
+            const float p1 = fast_exp2(__builtin_fmaf(x[m >> 1][8 * (m & 1) + 2 * j + 1], scale, -ref));
+            weights[m][j] = Half::pack(p0, p1);
+        }
 }
 // Sum of the weights, as rounded.
 __device__ inline float add_weights(const u32x4 (&weights)[4], float sum) {
@@ -349,7 +351,8 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
             }
         }
         u32x4 weights[4];
-        if (__any(!quick_weights(x, weights, a.scale, ref))) exact_weights(x, weights, a.scale, ref, sum, acc);
+        if (__any(!weights_fit(x, a.scale, ref))) move_reference(x, a.scale, ref, sum, acc);
+        weigh(x, weights, a.scale, ref);
         sum = add_weights(weights, sum);
 #pragma unroll
         for (int n = 0; n < S::kBlocks; ++n)

@@ -243,6 +243,39 @@ def test_prefill_nan_behind_the_mask_stays_there(plane, chunk):
     assert got[60:, 2:].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [32, 128, 256])
+def test_a_key_far_above_the_earlier_ones_at_every_place(dtype, dim):
+    """One key whose score is hundreds above all before it: 130 sequences, another place in each, for prefill rows
+    before, at and behind it, and for decode.
+
+    The bounds of ``attention`` count what is relative to a probability. Here most are below fp16's range: its
+    smallest step is 2^-24, so rounding is off by up to 2^-25 there, and the largest probability is held as 2^8 or
+    more (the reference of the exponentials stays 8 or more below the largest score). Per key this is 2^-33 of the
+    largest and so of their sum: 2^-33 * n * max|v| in the sum over the values, and the same again by way of the
+    sum of n probabilities that divides it, since the output is at most max|v|.
+    """
+    gen = torch.Generator().manual_seed(13)
+    block, tokens, count = 16, 192, 130
+    tables, pages = f4.tables_of(gen, (tokens,) * count, block)
+    rows = torch.randn(pages, 1, block, dim, generator=gen)
+    place = torch.arange(count) + 50
+    page = tables[torch.arange(count), place // block]
+    rows[page, 0, place % block] = 40.0
+    kc, vc = f4.packed(rows.to(dtype)), f4.packed(torch.randn(pages, 1, block, dim, generator=gen).to(dtype))
+    lens = torch.full((count,), tokens)
+    query = torch.rand(count, 1, dim, generator=gen).to(dtype)
+    args = [query, kc, vc, tables, lens]
+    floor = 2 * 2.0 ** -33 * tokens * f4.cache_values(vc, block, dim).abs().max()
+    want, bound = f4.decode_oracle(*args, block)
+    f4.assert_within(run_decode(args, block), want, bound + floor)
+    lens = place + 3  # rows at place - 1 .. place + 2
+    query = torch.rand(4 * count, 1, dim, generator=gen).to(dtype)
+    args = [query, kc, vc, torch.arange(count + 1) * 4, lens - 4, tables, lens]
+    want, bound = f4.prefill_oracle(*args, block)
+    f4.assert_within(run_prefill(args, block), want, bound + floor)
+
+
 def test_prefill_many_sequences():
     gen = torch.Generator().manual_seed(11)
     new = torch.randint(0, 9, (150,), generator=gen).tolist()
