@@ -121,24 +121,13 @@ __device__ inline void move_reference(const f32x16 (&x)[2], float scale, float& 
 #pragma unroll
     for (int n = 0; n < BLOCKS; ++n) acc[n] *= by;
 }
-// The scores of a tile become weights, four products' operands.
-__device__ inline void weigh(const f32x16 (&x)[2], u32x4 (&weights)[4], float scale, float ref) {
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float p0 = fast_exp2(__builtin_fmaf(x[m >> 1][8 * (m & 1) + 2 * j], scale, -ref));
-            const float p1 = fast_exp2(__builtin_fmaf(x[m >> 1][8 * (m & 1) + 2 * j + 1], scale, -ref));
-            weights[m][j] = Half::pack(p0, p1);
-        }
-}
-// Sum of the weights, as rounded.
-__device__ inline float add_weights(const u32x4 (&weights)[4], float sum) {
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum = Half::dot2(weights[m][j], 0x3c003c00u, sum);
-    return sum;
+// Pair i of a tile's scores becomes weights, as operands of four products, and adds to the sum as rounded.
+__device__ inline void weigh(const f32x16 (&x)[2], int i, u32x4 (&weights)[4], float& sum, float scale, float ref) {
+    const float p0 = fast_exp2(__builtin_fmaf(x[i >> 3][2 * (i & 7)], scale, -ref));
+    const float p1 = fast_exp2(__builtin_fmaf(x[i >> 3][2 * (i & 7) + 1], scale, -ref));
+    const uint32_t pair = Half::pack(p0, p1);
+    weights[i >> 2][i & 3] = pair;
+    sum = Half::dot2(pair, 0x3c003c00u, sum);
 }
 
 // Barrier of the work-group for LDS alone: loads from memory stay in flight.
@@ -352,22 +341,30 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         }
         u32x4 weights[4];
         if (__any(!weights_fit(x, a.scale, ref))) move_reference(x, a.scale, ref, sum, acc);
-        weigh(x, weights, a.scale, ref);
-        sum = add_weights(weights, sum);
+        // Sixteen keys at a time: their weights are made beside the products of the sixteen before them.
+        const auto operand_of = [&](int i) {  // sixteen keys i / kBlocks of 32 dims i % kBlocks
+            // (Eight rows on, the row's number differs in bit 1.)
+            const int n = i % S::kBlocks;
+            return value_operand(values + 16 * (i / S::kBlocks) * 2 * D, value_at.chunk(4 * n),
+                                 value_at.chunk(4 * n, 2) + 8 * 2 * D);
+        };
+        constexpr int kProducts = 4 * S::kBlocks, kAhead = kProducts < 4 ? kProducts : 4;
+        u32x4 operand[kAhead];
 #pragma unroll
-        for (int n = 0; n < S::kBlocks; ++n)
+        for (int i = 0; i < kAhead; ++i) operand[i] = operand_of(i);
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-                // (Eight rows on, the row's number differs in bit 1.)
-                acc[n] = mfma32<Half>(value_operand(values + 16 * m * 2 * D, value_at.chunk(4 * n),
-                                                    value_at.chunk(4 * n, 2) + 8 * 2 * D), weights[m], acc[n]);
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 8, 1);
+        for (int j = 0; j < 4; ++j) weigh(x, j, weights, sum, a.scale, ref);
 #pragma unroll
-        for (int i = 0; i < 4 * S::kBlocks - 4; ++i) {
-            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
-            __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
+        for (int i = 0; i < kProducts; ++i) {
+            const int m = i / S::kBlocks, n = i % S::kBlocks;
+            acc[n] = mfma32<Half>(operand[i % kAhead], weights[m], acc[n]);
+            if (i + kAhead < kProducts) operand[i % kAhead] = operand_of(i + kAhead);
+            if (m < 3)
+#pragma unroll
+                for (int j = 4 * n / S::kBlocks; j < 4 * (n + 1) / S::kBlocks; ++j)
+                    weigh(x, 4 * (m + 1) + j, weights, sum, a.scale, ref);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 1);
         lds_barrier();
     }
     const float total = swap32_add(sum, sum);  // the other half of the keys is with the lane 32 away
