@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         }
     };
     TileAddress<D, 32> stage_at(row, quarter * S::kChunks);
-    const auto unpack = [&](Staged<D>& x, int buffer) {
+    const auto prepare = [&](Staged<D>& x, int buffer) {
         // A NaN block of the values must not reach rows that do not see its key, as 0 * NaN would: it is staged as
         // zeros, and the key's score is NaN instead.  Absent tokens are zeros.
         bool nan = false;
@@ -238,14 +238,12 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
             if (quarter == 0) present[buffer][row] = x.there ? nan ? 2 : 1 : 0;
         }
         if (lane == 0) odd[buffer][wave] = some;
-#pragma unroll
-        for (int i = 0; i < S::kChunks; ++i) {
-            const int at = stage_at.chunk(i);
-            *reinterpret_cast<u32x4*>(tiles[buffer][0] + at) =
-                values_of<T>(x.codes[0][i], scale_of(x.scales[0][i / S::kPer]));
-            *reinterpret_cast<u32x4*>(tiles[buffer][1] + at) =
-                values_of<Half>(x.codes[1][i], scale_of(x.scales[1][i / S::kPer]));
-        }
+    };
+    const auto unpack = [&](const Staged<D>& x, int i, int buffer) {  // eight dims, of the key or behind all of it the value
+        const int plane = i / S::kChunks, n = i % S::kChunks;
+        const float scale = scale_of(x.scales[plane][n / S::kPer]);
+        *reinterpret_cast<u32x4*>(tiles[buffer][plane] + stage_at.chunk(n)) =
+            plane ? values_of<Half>(x.codes[plane][n], scale) : values_of<T>(x.codes[plane][n], scale);
     };
     Staged<D> staged;
     int64_t page = page_of(begin);
@@ -273,7 +271,9 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     TileAddress<D, 32> value_at(4 * h + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), (lane & 1) * 8);
 
     if (begin < end) {
-        unpack(staged, 0);
+        prepare(staged, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * S::kChunks; ++i) unpack(staged, i, 0);
         load(staged, begin + kKeys, page);
         page = page_of(begin + 2 * kKeys);
         lds_barrier();
@@ -289,23 +289,32 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         for (int i = 0; i < S::kScales; ++i) asm volatile("" : "+v"(scale_at[i]));
         const uint8_t* keys = tiles[buffer][0];
         const uint8_t* values = tiles[buffer][1];
+        // The scores, and the next tile's unpacking (behind the last tile: of zeros) beside them.
+        prepare(staged, buffer ^ 1);
         f32x16 x[2];
+        {
+            constexpr int kProducts = 2 * S::kSteps, kAhead = 4, kWords = 2 * S::kChunks;
+            const auto operand_of = [&](int i) {
+                return *reinterpret_cast<const u32x4*>(keys + 32 * (i / S::kSteps) * 2 * D + key_at.chunk(2 * (i % S::kSteps)));
+            };
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+            for (int i = 0; i < 16; ++i) x[0][i] = x[1][i] = 0.f;
+            u32x4 operand[kAhead];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[k][i] = 0.f;
+            for (int i = 0; i < kAhead; ++i) operand[i] = operand_of(i);
 #pragma unroll
-            for (int i = 0; i < S::kSteps; ++i)
-                x[k] = mfma32<T>(*reinterpret_cast<const u32x4*>(keys + 32 * k * 2 * D + key_at.chunk(2 * i)), q[i], x[k]);
+            for (int i = 0; i < kProducts; ++i) {
+                x[i / S::kSteps] = mfma32<T>(operand[i % kAhead], q[i % S::kSteps], x[i / S::kSteps]);
+                if (i + kAhead < kProducts) operand[i % kAhead] = operand_of(i + kAhead);
+#pragma unroll
+                for (int n = i * kWords / kProducts; n < (i + 1) * kWords / kProducts; ++n) unpack(staged, n, buffer ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        // Reads run four products ahead.
-        __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
-#pragma unroll
-        for (int i = 0; i < 2 * S::kSteps - 4; ++i) {
-            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+        if (t0 + kKeys < end) {
+            load(staged, t0 + 2 * kKeys, page);
+            page = page_of(t0 + 3 * kKeys);
         }
-        __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
         const uint32_t odds = (uint32_t)__builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(odd[buffer]));
         uint64_t mask = ~uint64_t(0);
         if (odds) {
@@ -320,12 +329,6 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
                 for (int i = 0; i < 16; ++i)
                     if ((bits >> (8 * (i >> 2) + (i & 3))) & 1) x[k][i] = __builtin_nanf("");
             }
-        }
-        // The next tile, while these scores go through the softmax.
-        if (t0 + kKeys < end) {
-            unpack(staged, buffer ^ 1);
-            load(staged, t0 + 2 * kKeys, page);
-            page = page_of(t0 + 3 * kKeys);
         }
         if (mask != ~uint64_t(0) || (int64_t)t0 + kKeys - 1 > first_pos) {
             const int32_t seen = limit - (int32_t)t0 - 4 * h;
