@@ -6,6 +6,9 @@
 // Tiles of 64 keys are unpacked once into LDS (keys in the query's type,
 // values in fp16) and used by all rows.  Chunks of split calls are joined by a
 // second kernel.
+#include <algorithm>
+#include <cmath>
+
 #include "fp4_attention.h"
 
 namespace mvme {
@@ -29,6 +32,7 @@ struct PrefillArgs {
     const int64_t* lens;
     float* partial;  // [total_tokens, q_heads, chunks, D], then [total_tokens, q_heads, chunks, 2]
     int64_t stats;
+    int32_t* counts; // [total_tokens, q_heads]: chunks that a row sees, -1 for rows that no sequence owns
     int64_t num_blocks, record, total_tokens;
     uint64_t page_bytes;
     int num_seqs, kv_heads, q_heads, group, width;
@@ -87,6 +91,7 @@ __device__ void clear_rows(const PrefillArgs& a, int kv_head) {
     for (int64_t i = threadIdx.x; i < count; i += kThreads) {
         const int64_t n = i / width, token = n < first ? n : last + n - first;
         static_cast<uint16_t*>(a.out)[(token * a.q_heads + (int64_t)kv_head * a.group) * D + i % width] = 0;
+        if (a.chunks > 1 && i % D == 0) a.counts[token * a.q_heads + (int64_t)kv_head * a.group + i % width / D] = -1;
     }
 }
 
@@ -152,19 +157,31 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         if (chunk == 0) clear_rows<D>(a, kv_head);
         return;
     }
-    // The sequence and the row block that `item` is: a sequence's blocks from the last, which sees most keys.
-    Seq seq;
+    // The sequence and the row block that `item` is: a sequence's blocks from the last, which sees most keys.  Sixty-four
+    // sequences at a time, one per lane.
     int s = 0;
-    for (;; ++s) {
-        if (s == a.num_seqs) return;
-        seq = sequence(a, s);
-        const int64_t blocks = (seq.rows * a.group + kRows - 1) / kRows;
-        if (item < blocks) {
-            item = (int)blocks - 1 - item;
+    for (;; s += 64) {
+        if (s >= a.num_seqs) return;
+        const int own = min(s + lane, a.num_seqs - 1);
+        const int64_t lo = min(max(a.cu[own], (int64_t)0), a.total_tokens);
+        const int64_t hi = min(max(a.cu[own + 1], lo), a.total_tokens);
+        const int blocks = s + lane < a.num_seqs ? (int)(((hi - lo) * a.group + kRows - 1) / kRows) : 0;
+        int behind = blocks;  // of the lanes up to this one
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) {
+            const int other = __shfl_up(behind, i);
+            if (lane >= i) behind += other;
+        }
+        const uint64_t found = __ballot(behind > item);
+        if (found) {
+            const int at = __builtin_ctzll(found);
+            s += at;
+            item = __builtin_amdgcn_readlane(behind, at) - 1 - item;
             break;
         }
-        item -= (int)blocks;
+        item -= __builtin_amdgcn_readlane(behind, 63);
     }
+    const Seq seq = sequence(a, s);
     const int64_t usable = usable_keys(a, seq);
     const int64_t row0 = (int64_t)item * kRows, rows = seq.rows * a.group;
     // Keys of this work-group: up to the last row's position, in its chunk.
@@ -387,36 +404,33 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     if (a.chunks > 1 && h == 0) {
         a.partial[a.stats + at * 2] = ref;
         a.partial[a.stats + at * 2 + 1] = total;
+        if (chunk == 0) a.counts[head] = limit < 0 ? 0 : limit / a.chunk_len + 1;
     }
 }
 
-// Joins the key chunks of one packed row and query head.
+template <int D>
+constexpr int kMergeRows = kThreads / (D / 4);
+// Joins the key chunks of packed rows and query heads: four dims per thread.
 template <typename T, int D>
-__global__ __launch_bounds__(64) void fp4_prefill_merge_kernel(PrefillArgs a) {
-    const int64_t head = blockIdx.x, token = head / a.q_heads;
-    int lo = 0, hi = a.num_seqs;  // the first sequence that ends behind the row
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (a.cu[mid + 1] <= token) lo = mid + 1;
-        else hi = mid;
+__global__ __launch_bounds__(kThreads) void fp4_prefill_merge_kernel(PrefillArgs a) {
+    const int64_t head = (int64_t)blockIdx.x * kMergeRows<D> + threadIdx.x / (D / 4);
+    const int d = threadIdx.x % (D / 4) * 4;
+    if ((int)threadIdx.x >= kMergeRows<D> * (D / 4) || head >= a.total_tokens * a.q_heads) return;
+    const int chunks = a.counts[head];
+    if (chunks < 0) return;  // cleared by the first kernel
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2* stats = reinterpret_cast<const f32x2*>(a.partial + a.stats) + head * a.chunks;
+    const float* partial = a.partial + head * a.chunks * D + d;
+    float top = kRefNone, total = 0.f;
+    for (int c = 0; c < chunks; ++c) top = fmaxf(top, stats[c][0]);
+    f32x4 value = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int c = 0; c < chunks; ++c) {
+        const float by = fast_exp2(stats[c][0] - top);
+        total += by * stats[c][1];
+        value += by * *reinterpret_cast<const f32x4*>(partial + (int64_t)c * D);
     }
-    if (lo == a.num_seqs || token < a.cu[lo]) return;  // no sequence's row: cleared by the first kernel
-    const Seq seq = sequence(a, lo);
-    const int64_t pos = seq.start + token - seq.row0;
-    const int chunks = pos < usable_keys(a, seq) ? (int)(pos / a.chunk_len) + 1 : 0;
-    const float* stats = a.partial + a.stats + head * a.chunks * 2;
-    const float* partial = a.partial + head * a.chunks * D;
-    float top = kRefNone;
-    for (int c = 0; c < chunks; ++c) top = fmaxf(top, stats[2 * c]);
-    for (int d = threadIdx.x; d < D; d += 64) {
-        float total = 0.f, value = 0.f;
-        for (int c = 0; c < chunks; ++c) {
-            const float by = fast_exp2(stats[2 * c] - top);
-            total += by * stats[2 * c + 1];
-            value += by * partial[(int64_t)c * D + d];
-        }
-        static_cast<uint16_t*>(a.out)[head * D + d] = T::from_float(total != 0.f ? value / total : 0.f);
-    }
+    store4<T, D>(a, head, d, total != 0.f ? value * (1.f / total) : f32x4{0.f, 0.f, 0.f, 0.f});
 }
 
 bool attention_dim(int64_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
@@ -433,18 +447,34 @@ struct Plan {
     int64_t items, chunks, chunk_len;
 };
 
-Plan plan(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, int64_t block_size, int64_t width,
-          int64_t chunk_tokens) {
+// Splits the keys where the row blocks are too few for the chip, by an estimate in microseconds: a tile takes a work-group
+// kTileAlone where it has a compute unit to itself and kTileBoth where two share it (128 dims, where these were measured),
+// and the pieces have to be joined.
+constexpr double kCus = 256, kTileAlone = 1.45, kTileBoth = 2.1, kMerge = 4, kMergeRate = 4e6;
+constexpr int64_t kMostChunks = 64, kLeastKeys = 256;
+
+Plan plan(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t block_size,
+          int64_t width, int64_t chunk_tokens) {
     const int64_t capacity = block_size * width, group = q_heads / kv_heads;
     // Row blocks: full ones, at most one partial per sequence, and the one that clears.
     const int64_t items = total * group / kRows + num_seqs + 1;
     int64_t len = capacity;
     if (chunk_tokens > 0) {
         len = chunk_tokens;
-    } else if (items * kv_heads < 512) {
-        const int64_t want = 512 / (items * kv_heads) + 1;
-        len = (capacity + want - 1) / want;
-        if (len < 256) len = 256;
+    } else {
+        // (Half of the partial ones, for the estimate; a sequence has one at least.)
+        const double groups = (double)(std::max(total * group / kRows + num_seqs / 2, num_seqs) * kv_heads);
+        const double rows = (double)(total * q_heads), tiles = (double)((capacity + kKeys - 1) / kKeys);
+        double best = 0;
+        for (int64_t n = 1; n <= kMostChunks && (n - 1) * kLeastKeys < capacity; ++n) {
+            const double fill = groups * n / kCus;
+            if (n > 1 && fill - groups / kCus >= 2) break;  // full already
+            const double time = (fill <= 1 ? kTileAlone : kTileBoth * std::max(fill / 2, 1.)) * std::ceil(tiles / n) +
+                                (n > 1 ? kMerge + rows * n * head_dim * 8 / kMergeRate : 0);
+            if (n > 1 && time >= best) continue;
+            best = time;
+            len = (capacity + n - 1) / n;
+        }
     }
     if (len > capacity) len = capacity;
     len = (len + kKeys - 1) / kKeys * kKeys;
@@ -458,8 +488,8 @@ int launch(const PrefillArgs& a, hipStream_t s) {
     else hipLaunchKernelGGL((fp4_prefill_kernel<T, D, 1>), grid, block, 0, s, a);
     if (int rc = check_launch("packed prefill")) return rc;
     if (a.chunks == 1) return MVME_OK;
-    hipLaunchKernelGGL((fp4_prefill_merge_kernel<T, D>), dim3((unsigned)(a.total_tokens * a.q_heads)), dim3(64), 0, s,
-                       a);
+    hipLaunchKernelGGL((fp4_prefill_merge_kernel<T, D>), dim3((unsigned)((a.total_tokens * a.q_heads - 1) / kMergeRows<D> + 1)),
+                       dim3(kThreads), 0, s, a);
     return check_launch("packed prefill merge");
 }
 
@@ -486,9 +516,9 @@ extern "C" size_t mvme_fp4_paged_prefill_workspace_size(int64_t num_seqs, int64_
                                                         int64_t kv_heads, int64_t head_dim, int64_t block_size,
                                                         int64_t table_width, int64_t chunk_tokens) {
     if (!prefill_shape(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width)) return 0;
-    const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, block_size, table_width, chunk_tokens);
+    const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width, chunk_tokens);
     return p.chunks == 1 ? 0
-                         : (size_t)(total_tokens * q_heads) * (size_t)p.chunks * (size_t)(head_dim + 2) * sizeof(float);
+                         : (size_t)(total_tokens * q_heads) * ((size_t)p.chunks * (size_t)(head_dim + 2) + 1) * sizeof(float);
 }
 
 extern "C" int mvme_fp4_paged_prefill_attention(void* out, const void* q, const void* key_cache,
@@ -518,7 +548,7 @@ extern "C" int mvme_fp4_paged_prefill_attention(void* out, const void* q, const 
         return fail(MVME_EINVAL, "packed prefill: null pointer");
     if (!aligned(q, 16) || !aligned(key_cache, 16) || !aligned(value_cache, 16) || !aligned(out, 8))
         return fail(MVME_EINVAL, "packed prefill: queries and caches must be 16-byte, the output 8-byte aligned");
-    const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, block_size, table_width, chunk_tokens);
+    const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width, chunk_tokens);
     if (p.chunks > 2147483647 / kv_heads / p.items) return fail(MVME_EINVAL, "too many packed query rows");
     const size_t need = mvme_fp4_paged_prefill_workspace_size(num_seqs, total_tokens, q_heads, kv_heads, head_dim,
                                                               block_size, table_width, chunk_tokens);
@@ -536,6 +566,7 @@ extern "C" int mvme_fp4_paged_prefill_attention(void* out, const void* q, const 
     a.lens = context_lens;
     a.partial = static_cast<float*>(workspace);
     a.stats = total_tokens * q_heads * p.chunks * head_dim;
+    a.counts = reinterpret_cast<int32_t*>(a.partial + a.stats + total_tokens * q_heads * p.chunks * 2);
     a.num_blocks = num_blocks;
     a.record = record;
     a.page_bytes = (uint64_t)(record * kv_heads);
