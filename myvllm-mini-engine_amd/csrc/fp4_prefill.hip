@@ -447,10 +447,17 @@ struct Plan {
     int64_t items, chunks, chunk_len;
 };
 
-// Splits the keys where the row blocks are too few for the chip, by an estimate in microseconds: a tile takes a work-group
-// kTileAlone where it has a compute unit to itself and kTileBoth where two share it (128 dims, where these were measured),
-// and the pieces have to be joined.
-constexpr double kCus = 256, kTileAlone = 1.45, kTileBoth = 2.1, kMerge = 4, kMergeRate = 4e6;
+// Splits the keys where the row blocks are too few for the chip, by an estimate in microseconds.  A work-group with a
+// compute unit to itself takes a tile in 1.00, 1.15, 1.45, 1.5, 2.5 and 3.1 us at 32, 64, 96, 128, 192 and 256 dims, two
+// on one unit in 1.4 times as long each; from 192 dims on LDS holds one.  Joining takes a launch and its traffic.
+// 8 x 128 tokens behind 4096 keys (128 dims): 48 us in four pieces, 99 us whole, 67 us in sixteen; two sequences of 2048
+// tokens (256 dims): 239 us whole, 363 us in pieces of 768.
+constexpr double kCus = 256, kMerge = 4, kMergeRate = 8e6;
+double tile_time(int64_t head_dim, double fill) {  // fill: work-groups per compute unit
+    const double alone = head_dim <= 128 ? 0.85 + (double)head_dim / 200 : 0.65 + (double)head_dim / 105;
+    const double both = head_dim <= 128 ? 1.4 : 2;
+    return alone * (fill <= 1 ? 1 : fill <= 2 ? 1 + (both - 1) * (fill - 1) : both * fill / 2);
+}
 constexpr int64_t kMostChunks = 64, kLeastKeys = 256;
 
 Plan plan(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t block_size,
@@ -462,14 +469,14 @@ Plan plan(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, in
     if (chunk_tokens > 0) {
         len = chunk_tokens;
     } else {
-        // (Half of the partial ones, for the estimate; a sequence has one at least.)
-        const double groups = (double)(std::max(total * group / kRows + num_seqs / 2, num_seqs) * kv_heads);
+        // (A quarter of the partial ones, for the estimate; a sequence has one at least.)
+        const double groups = (double)(std::max(total * group / kRows + num_seqs / 4, num_seqs) * kv_heads);
         const double rows = (double)(total * q_heads), tiles = (double)((capacity + kKeys - 1) / kKeys);
         double best = 0;
         for (int64_t n = 1; n <= kMostChunks && (n - 1) * kLeastKeys < capacity; ++n) {
             const double fill = groups * n / kCus;
             if (n > 1 && fill - groups / kCus >= 2) break;  // full already
-            const double time = (fill <= 1 ? kTileAlone : kTileBoth * std::max(fill / 2, 1.)) * std::ceil(tiles / n) +
+            const double time = tile_time(head_dim, fill) * std::ceil(tiles / n) +
                                 (n > 1 ? kMerge + rows * n * head_dim * 8 / kMergeRate : 0);
             if (n > 1 && time >= best) continue;
             best = time;
