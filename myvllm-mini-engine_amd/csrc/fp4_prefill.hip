@@ -142,6 +142,70 @@ __device__ inline void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// Sum over the lanes up to this one.
+__device__ inline int lane_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // from 1, 2, 4, 8 lanes before, in rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last lane of the row before, to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31, to rows 2 and 3
+    return x;
+}
+// Which of the lanes' row blocks, counted through, is `item`: its lane, and `item` from that lane's first.  -1: behind all.
+__device__ inline int find_lane(int blocks, int& item) {
+    const int scan = lane_scan(blocks);
+    const uint64_t behind = __ballot(scan > item);
+    if (!behind) return -1;
+    const int at = __builtin_ctzll(behind);
+    item -= __builtin_amdgcn_readlane(scan - blocks, at);
+    return at;
+}
+__device__ inline int row_blocks(const PrefillArgs& a, int s) {
+    const int64_t lo = min(max(a.cu[s], (int64_t)0), a.total_tokens);
+    const int64_t hi = min(max(a.cu[s + 1], lo), a.total_tokens);
+    return (int)(((hi - lo) * a.group + kRows - 1) / kRows);
+}
+// The sequence s and its row block that `item` becomes, from sequence to sequence; a sequence's blocks from the last,
+// which sees most keys.  False behind all blocks.
+__device__ inline bool find_in_order(const PrefillArgs& a, int lane, int& item, int& s) {
+    for (s = 0; s < a.num_seqs; s += 64) {
+        const int blocks = s + lane < a.num_seqs ? row_blocks(a, s + lane) : 0;
+        const int at = find_lane(blocks, item);
+        if (at >= 0) {
+            s += at;
+            item = __builtin_amdgcn_readlane(blocks, at) - 1 - item;
+            return true;
+        }
+        item -= __builtin_amdgcn_readlane(lane_scan(blocks), 63);
+    }
+    return false;
+}
+// The same for up to 64 sequences with the blocks that see most keys first, to a tile: they take longest, and the short
+// ones fill what the chip has free at the end.
+__device__ inline bool find_longest_first(const PrefillArgs& a, int lane, int& item, int& s) {
+    const int own = min(lane, a.num_seqs - 1);
+    const int blocks = lane < a.num_seqs ? row_blocks(a, own) : 0;
+    const int start = (int)min(max(a.starts[own], (int64_t)0), kMaxCapacity);
+    // Blocks of this lane's sequence that see keys at 64 * tile and behind; none at `top` (positions past the tables are
+    // with the last tile before it).
+    const int half = 1 << (31 - __builtin_clz((int)(a.width * a.div.size / kKeys) | 1)), top = 2 * half;
+    const auto from = [&](int tile) {
+        const int64_t before = (int64_t)(tile * kKeys - start) * a.group / kRows;
+        return tile == top ? 0 : (int)max(blocks - max(before, (int64_t)0), (int64_t)0);
+    };
+    const auto all = [&](int n) { return __builtin_amdgcn_readlane(lane_scan(n), 63); };
+    if (item >= all(blocks)) return false;
+    int tile = 0;  // the last with more than `item` blocks
+    for (int step = half; step > 0; step /= 2)
+        if (all(from(tile + step)) > item) tile += step;
+    const int longer = from(tile + 1), here = from(tile) - longer;
+    item -= all(longer);
+    s = find_lane(here, item);
+    item = __builtin_amdgcn_readlane(blocks - longer, s) - 1 - item;
+    return s >= 0;
+}
+
 template <typename T, int D, int RUN>
 __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_kernel(PrefillArgs a) {
     using S = Shape<D>;
@@ -157,30 +221,8 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
         if (chunk == 0) clear_rows<D>(a, kv_head);
         return;
     }
-    // The sequence and the row block that `item` is: a sequence's blocks from the last, which sees most keys.  Sixty-four
-    // sequences at a time, one per lane.
-    int s = 0;
-    for (;; s += 64) {
-        if (s >= a.num_seqs) return;
-        const int own = min(s + lane, a.num_seqs - 1);
-        const int64_t lo = min(max(a.cu[own], (int64_t)0), a.total_tokens);
-        const int64_t hi = min(max(a.cu[own + 1], lo), a.total_tokens);
-        const int blocks = s + lane < a.num_seqs ? (int)(((hi - lo) * a.group + kRows - 1) / kRows) : 0;
-        int behind = blocks;  // of the lanes up to this one
-#pragma unroll
-        for (int i = 1; i < 64; i *= 2) {
-            const int other = __shfl_up(behind, i);
-            if (lane >= i) behind += other;
-        }
-        const uint64_t found = __ballot(behind > item);
-        if (found) {
-            const int at = __builtin_ctzll(found);
-            s += at;
-            item = __builtin_amdgcn_readlane(behind, at) - 1 - item;
-            break;
-        }
-        item -= __builtin_amdgcn_readlane(behind, 63);
-    }
+    int s;
+    if (!(a.num_seqs <= 64 ? find_longest_first(a, lane, item, s) : find_in_order(a, lane, item, s))) return;
     const Seq seq = sequence(a, s);
     const int64_t usable = usable_keys(a, seq);
     const int64_t row0 = (int64_t)item * kRows, rows = seq.rows * a.group;
