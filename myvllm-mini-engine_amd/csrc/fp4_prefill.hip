@@ -38,7 +38,7 @@ struct PrefillArgs {
     int num_seqs, kv_heads, q_heads, group, width;
     int items;       // work-groups per kv head and chunk; the last one clears rows that no sequence owns
     int chunks, chunk_len;
-    BlockDiv div;
+    BlockDiv div, group_div;
     float scale;     // log2(e) / sqrt(D)
 };
 
@@ -191,8 +191,8 @@ __device__ inline bool find_longest_first(const PrefillArgs& a, int lane, int& i
     // with the last tile before it).
     const int half = 1 << (31 - __builtin_clz((int)(a.width * a.div.size / kKeys) | 1)), top = 2 * half;
     const auto from = [&](int tile) {
-        const int64_t before = (int64_t)(tile * kKeys - start) * a.group / kRows;
-        return tile == top ? 0 : (int)max(blocks - max(before, (int64_t)0), (int64_t)0);
+        const uint64_t before = (uint64_t)(uint32_t)max(tile * kKeys - start, 0) * (uint32_t)a.group / kRows;
+        return tile == top ? 0 : blocks - (int)min(before, (uint64_t)blocks);
     };
     const auto all = [&](int n) { return __builtin_amdgcn_readlane(lane_scan(n), 63); };
     if (item >= all(blocks)) return false;
@@ -225,10 +225,11 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     if (!(a.num_seqs <= 64 ? find_longest_first(a, lane, item, s) : find_in_order(a, lane, item, s))) return;
     const Seq seq = sequence(a, s);
     const int64_t usable = usable_keys(a, seq);
-    const int64_t row0 = (int64_t)item * kRows, rows = seq.rows * a.group;
+    // (Rows are counted in 32 bits: all tokens' query heads are below 2^31.)
+    const uint32_t row0 = (uint32_t)item * kRows, rows = (uint32_t)seq.rows * a.group;
     // Keys of this work-group: up to the last row's position, in its chunk.
-    const int64_t last_token = (min(row0 + kRows, rows) - 1) / a.group;
-    const int64_t first_pos = seq.start + row0 / a.group;
+    const uint32_t last_token = a.group_div.page(min(row0 + kRows, rows) - 1);
+    const int64_t first_pos = seq.start + a.group_div.page(row0);
     const uint32_t key_end = (uint32_t)min(usable, max(seq.start + last_token + 1, (int64_t)0));
     const uint32_t begin = (uint32_t)chunk * a.chunk_len;
     const uint32_t end = min(key_end, begin + (uint32_t)a.chunk_len);
@@ -310,11 +311,11 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     page = page_of(begin + kKeys);
 
     // This lane's row.
-    const int64_t qrow = row0 + wave * 32 + column;
+    const uint32_t qrow = row0 + wave * 32 + column;
     const bool live = qrow < rows;
-    const int64_t token = live ? qrow / a.group : 0;
+    const uint32_t token = live ? a.group_div.page(qrow) : 0u;
     const int32_t limit = live && seq.start + token < usable ? (int32_t)(seq.start + token) : -1;  // last visible key
-    const int64_t head = (seq.row0 + token) * a.q_heads + (int64_t)kv_head * a.group + (live ? qrow % a.group : 0);
+    const int64_t head = (seq.row0 + token) * a.q_heads + (int64_t)kv_head * a.group + (live ? qrow - token * a.group : 0u);
     u32x4 q[S::kSteps];
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i)
@@ -629,6 +630,7 @@ extern "C" int mvme_fp4_paged_prefill_attention(void* out, const void* q, const 
     a.chunks = (int)p.chunks;
     a.chunk_len = (int)p.chunk_len;
     a.div = make_block_div(block_size);
+    a.group_div = make_block_div(a.group);
     a.scale = kLog2e / __builtin_sqrtf((float)head_dim);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return dtype == MVME_FP16 ? launch_dim<Half>(a, head_dim, s) : launch_dim<BFloat16>(a, head_dim, s);
