@@ -32,30 +32,37 @@ struct DecodeArgs {
     float scale;     // log2(e) / sqrt(D)
 };
 
+// Waves of a work-group: four work-groups fit a CU up to 128 dims and so overlap each other's joins (64 ragged sequences
+// of up to 4096 tokens: 38.9 us; eight waves 47.4, two 39.1).
+constexpr int kWaves = 4;
+constexpr int kRound = kWaves * kTileKeys;  // keys of a round
+
 template <int D>
 struct Shape {
-    static constexpr int kWaves = D <= 128 ? 8 : 4;
     static constexpr int kChunks = D / 32;           // score products per 16 keys; dwords of codes per lane
     static constexpr int kPer = D % 128 == 0 ? 4 : D == 64 || D == 192 ? 2 : 1;  // chunks that share a scale
     static constexpr int kScales = kChunks / kPer;
     static constexpr int kDimTiles = D / 16;
     static constexpr int kTileBytes = kTileKeys * 2 * D;  // fp16 rows of a tile; as large as a wave's accumulators
     static constexpr int kMinWaves = D <= 128 ? 4 : 2;
-    static constexpr int kRound = kWaves * kTileKeys;     // keys of a round
 };
 
 // The walk's order: sequences, their units, a unit's rounds.
 template <int D>
 __device__ inline int rounds_of(const DecodeArgs& a, int64_t len) {
     const bool usable = len > 0 && len <= (int64_t)a.width * a.div.size;
-    return usable ? (int)(((uint32_t)len - 1) / Shape<D>::kRound) + 1 : 0;
+    return usable ? (int)(((uint32_t)len - 1) / kRound) + 1 : 0;
 }
 
 __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ inline int64_t length_of(const DecodeArgs& a, int seq) { return seq < a.batch ? a.lens[seq] : 0; }
 
-// Shares of the walk, in rounds.  Every wave computes the same, lane-parallel over the sequences; the first 64 lengths
-// stay in registers.
+// Shares of the walk, in rounds, have two where that still gives every CU one: more pieces cost the join more than they save
+// (8192 tokens, 8 kv heads: 9.3 us in shares of two, 10.7 of one), fewer leave the CUs unevenly loaded (16 ragged sequences
+// of up to 4096: 16.0 us, 19.7 in shares of four).
+constexpr int kCus = 256, kLeastShare = 2;
+
+// The walk.  Every wave computes the same, lane-parallel over the sequences; the first 64 lengths stay in registers.
 template <int D>
 struct Walk {
     int64_t len;  // of sequence `lane`
@@ -69,7 +76,7 @@ struct Walk {
         for (int s0 = kWave; s0 < a.batch; s0 += kWave)
             total += lane_value(wave_incl_scan(rounds_of<D>(a, length_of(a, s0 + lane))), kWave - 1);
         total *= units;
-        share = a.share > 0 ? a.share : (total + a.groups - 1) / a.groups;
+        share = a.share > 0 ? a.share : max((total + a.groups - 1) / a.groups, min((total + kCus - 1) / kCus, kLeastShare));
     }
     // The sequence that owns round `round` (< total), the round it begins at, its rounds per unit and its length.
     __device__ inline void find(const DecodeArgs& a, int round, int& seq, int& base, int& rounds, uint32_t& tokens) const {
@@ -220,10 +227,10 @@ __device__ inline void load_query(u32x4 (&q)[Shape<D>::kChunks], const DecodeArg
 }
 
 template <typename T, int D, int RUN>
-__global__ __launch_bounds__(64 * Shape<D>::kWaves, Shape<D>::kMinWaves) void fp4_decode_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, Shape<D>::kMinWaves) void fp4_decode_kernel(DecodeArgs a) {
     using S = Shape<D>;
-    __shared__ __attribute__((aligned(16))) uint8_t tiles[S::kWaves][S::kTileBytes];
-    __shared__ float stats[S::kWaves][2][16];
+    __shared__ __attribute__((aligned(16))) uint8_t tiles[kWaves][S::kTileBytes];
+    __shared__ float stats[kWaves][2][16];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -263,8 +270,8 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, Shape<D>::kMinWaves) void fp
         s.seq = uniform(s.seq);
         s.kv_head = uniform(unit / a.head_tiles);
         s.tile = uniform(unit) - s.kv_head * a.head_tiles;
-        s.begin = (uint32_t)uniform(from * S::kRound);
-        s.end = (uint32_t)uniform((int)min(tokens, (uint32_t)(from + n) * S::kRound));
+        s.begin = (uint32_t)uniform(from * kRound);
+        s.end = (uint32_t)uniform((int)min(tokens, (uint32_t)(from + n) * kRound));
         s.slot = uniform(s.slot);
         s.rounds = uniform(n);
         return s;
@@ -301,13 +308,13 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, Shape<D>::kMinWaves) void fp
         float ref = kRefNone, sum = 0.f;
         const bool idle = t0 >= seg.end;  // no tile of this segment for this wave
 #pragma unroll 1
-        for (; t0 < seg.end; t0 += S::kRound) {
-            const bool more = t0 + S::kRound < seg.end;
+        for (; t0 < seg.end; t0 += kRound) {
+            const bool more = t0 + kRound < seg.end;
             write_at.forget();
             read_at.forget();
             lane_at.forget();
             Where<D, RUN> next = now;
-            if (more) next = find_tile(seg, t0 + S::kRound);
+            if (more) next = find_tile(seg, t0 + kRound);
             else if (ahead.rounds) next = find_tile(ahead, ahead.begin + wave * kTileKeys);
             // Scores.
             f32x4 x[2];
@@ -396,14 +403,14 @@ __global__ __launch_bounds__(64 * Shape<D>::kWaves, Shape<D>::kMinWaves) void fp
         }
         __syncthreads();
         const int64_t first_head = (int64_t)seg.seq * a.q_heads + seg.kv_head * a.group + seg.tile * 16;
-        for (int i = threadIdx.x; i < heads * D; i += 64 * S::kWaves) {
+        for (int i = threadIdx.x; i < heads * D; i += 64 * kWaves) {
             const int h = i / D, d = i - h * D;
             float top = stats[0][0][h];
 #pragma unroll
-            for (int w = 1; w < S::kWaves; ++w) top = fmaxf(top, stats[w][0][h]);
+            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, stats[w][0][h]);
             float total = 0.f, value = 0.f;
 #pragma unroll
-            for (int w = 0; w < S::kWaves; ++w) {
+            for (int w = 0; w < kWaves; ++w) {
                 const float by = fast_exp2(stats[w][0][h] - top);
                 total += by * stats[w][1][h];
                 value += by * reinterpret_cast<const float*>(tiles[w])[i];
@@ -452,6 +459,7 @@ __global__ __launch_bounds__(kMergeThreads) void fp4_merge_kernel(DecodeArgs a) 
     f32x4 value = {0.f, 0.f, 0.f, 0.f};
     float ref = kRefNone, sum = 0.f;
     if (group < kGroups) {
+#pragma unroll 4
         for (int i = first + group; i <= last; i += kGroups) {
             // A piece that begins its share is in the share's first slot.
             const int64_t slot = (int64_t)i * 2 + (i == first && at > first * walk.share ? 1 : 0);
@@ -489,8 +497,11 @@ struct Plan {
     int64_t share;   // rounds of a share (0: by the lengths)
 };
 
-constexpr int64_t kWalkGroups = 512;   // two per CU: what LDS and registers hold at once
-constexpr int64_t kManyUnits = 2048;
+constexpr int64_t kWalkGroups = 1024;  // four per CU: what registers hold at once up to 128 dims
+// Units go out whole where they are short: up to 512 tokens the join costs more than it shares out (64 sequences of 512: 9.6
+// us whole, 13.9 shared), and up to 2048 where they fill the chip (128 ragged sequences: 35.7 us whole, 42.3 shared; one
+// long among short ones takes 17 us alone).
+constexpr int64_t kShortRounds = 4, kManyUnits = 1024, kManyRounds = 16;
 constexpr int64_t kMostRounds = int64_t(1) << 30;
 
 bool attention_dim(int64_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
@@ -503,24 +514,22 @@ bool decode_shape(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head
 }
 
 // From shapes alone (lengths stay on the device).
-Plan plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t block_size, int64_t width,
-          int64_t partition_tokens) {
-    const int64_t capacity = block_size * width, round = head_dim <= 128 ? 256 : 128;
+Plan plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t block_size, int64_t width, int64_t partition_tokens) {
+    const int64_t capacity = block_size * width;
     const int64_t units = batch * kv_heads * ((q_heads / kv_heads + 15) / 16);
-    const int64_t rounds = (capacity - 1) / round + 1;  // of a unit, at most
+    const int64_t rounds = (capacity - 1) / kRound + 1;  // of a unit, at most
     if (partition_tokens > 0) {
-        const int64_t share = (partition_tokens + round - 1) / round;
+        const int64_t share = (partition_tokens + kRound - 1) / kRound;
         if (share >= rounds && partition_tokens >= capacity) return {0, 0};
         return {(units * rounds - 1) / share + 1, share};
     }
-    // Units of one round have nothing to share; many units level each other out.
-    if (rounds == 1 || units >= kManyUnits) return {0, 0};
+    if (rounds <= kShortRounds || (units >= kManyUnits && rounds <= kManyRounds)) return {0, 0};
     return {units * rounds < kWalkGroups ? units * rounds : kWalkGroups, 0};
 }
 
 template <typename T, int D>
 int launch(const DecodeArgs& a, int64_t units, hipStream_t s) {
-    const dim3 grid((unsigned)(a.groups ? a.groups : units)), block(64 * Shape<D>::kWaves);
+    const dim3 grid((unsigned)(a.groups ? a.groups : units)), block(64 * kWaves);
     if (a.div.size % 32 == 0) hipLaunchKernelGGL((fp4_decode_kernel<T, D, 32>), grid, block, 0, s, a);
     else if (a.div.size % 16 == 0) hipLaunchKernelGGL((fp4_decode_kernel<T, D, 16>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((fp4_decode_kernel<T, D, 1>), grid, block, 0, s, a);
@@ -553,7 +562,7 @@ extern "C" size_t mvme_fp4_paged_attention_workspace_size(int64_t batch, int64_t
                                                           int64_t head_dim, int64_t block_size, int64_t table_width,
                                                           int64_t partition_tokens) {
     if (!decode_shape(batch, q_heads, kv_heads, head_dim, block_size, table_width)) return 0;
-    const Plan p = plan(batch, q_heads, kv_heads, head_dim, block_size, table_width, partition_tokens);
+    const Plan p = plan(batch, q_heads, kv_heads, block_size, table_width, partition_tokens);
     // Two pieces of up to 16 heads a share.
     return (size_t)p.groups * 2 * 16 * (size_t)(head_dim + 2) * sizeof(float);
 }
@@ -581,7 +590,7 @@ extern "C" int mvme_fp4_paged_attention(void* out, const void* query, const void
     if (!aligned(query, 16) || !aligned(key_cache, 16) || !aligned(value_cache, 16) || !aligned(out, 2))
         return fail(MVME_EINVAL, "packed decode: query and caches must be 16-byte aligned");
     if (partition_tokens < 0) return fail(MVME_EINVAL, "partition_tokens must not be negative");
-    const Plan p = plan(batch, q_heads, kv_heads, head_dim, block_size, table_width, partition_tokens);
+    const Plan p = plan(batch, q_heads, kv_heads, block_size, table_width, partition_tokens);
     const int64_t tiles = (q_heads / kv_heads + 15) / 16, units = batch * kv_heads * tiles;
     if (p.groups > kMostRounds || units > 2147483647) return fail(MVME_EINVAL, "too many partitions");
     const size_t need = mvme_fp4_paged_attention_workspace_size(batch, q_heads, kv_heads, head_dim, block_size,
