@@ -77,7 +77,7 @@ int mvme_fp4_gather(void* key_out, void* value_out, const void* key_cache, const
  * Bytes of device workspace mvme_fp4_paged_attention needs for these shapes
  * (0 when no sequence is split).  Pure host function.  partition_tokens: 0
  * selects the library's plan, > 0 partitions of that many tokens (rounded up
- * to whole tiles of 32).
+ * to whole rounds of 128).  At most 34 MB with the library's plan.
  */
 size_t mvme_fp4_paged_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                int64_t block_size, int64_t table_width, int64_t partition_tokens);
@@ -88,9 +88,10 @@ size_t mvme_fp4_paged_attention_workspace_size(int64_t batch, int64_t q_heads, i
  * 1/sqrt(head_dim), sequences of length <= 0 or beyond the table's capacity
  * produce zeros, pages out of range are skipped.  Query and output are fp16
  * or bf16 [batch, q_heads, head_dim]; scores, softmax statistics and
- * accumulators are fp32, probabilities are rounded to fp16 (11 bits, exponent
- * range used from 2^-24 to 2^14 around the running maximum) for the value
- * product.
+ * accumulators are fp32.  Probabilities are rounded to fp16 for the value
+ * product, relative to a reference that keeps the largest between 2^8 and
+ * 2^16: they have 11 bits from 2^-22 of the largest on and are lost below
+ * 2^-33 of it.
  */
 int mvme_fp4_paged_attention(void* out, const void* query, const void* key_cache, const void* value_cache,
                              const int64_t* block_tables, const int64_t* context_lens,
@@ -99,7 +100,12 @@ int mvme_fp4_paged_attention(void* out, const void* query, const void* key_cache
                              int64_t partition_tokens, int dtype,
                              void* workspace, size_t workspace_bytes, void* stream);
 
-/* Bytes of device workspace mvme_fp4_paged_prefill_attention needs (0 when no keys are split).  Pure host function. */
+/*
+ * Bytes of device workspace mvme_fp4_paged_prefill_attention needs (0 when no
+ * keys are split).  Pure host function.  chunk_tokens: 0 selects the
+ * library's plan, > 0 chunks of that many keys (rounded up to whole tiles of
+ * 64).
+ */
 size_t mvme_fp4_paged_prefill_workspace_size(int64_t num_seqs, int64_t total_tokens, int64_t q_heads,
                                              int64_t kv_heads, int64_t head_dim, int64_t block_size,
                                              int64_t table_width, int64_t chunk_tokens);

@@ -22,10 +22,12 @@ namespace fp4 {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// Probabilities are exp2(x - reference) with the reference kept 8 below the
-// largest score seen when it was set, and moved when a score passes it by 14:
-// fp16 then holds every probability down to 2^-24 - 8 of the largest with
-// full 11 bits from 2^-22 on, and none overflows.
+// Probabilities are exp2(x - reference) with the reference set 8 below the
+// largest score, and moved when a score passes it by 14 (prefill looks when
+// one passes fp16, at 16).  They are rounded to fp16 for the value product
+// (half the products of fp32, and every value of the cache is exact in it):
+// 11 bits from 2^-22 of the largest on, nothing below 2^-33 of it, and none
+// overflows.  Their sums and the accumulators are fp32.
 constexpr float kRefBelow = 8.f;
 constexpr float kRefSlack = 14.f;
 constexpr float kRefNone = -3.0e38f;  // no score yet: below every finite one

@@ -13,6 +13,7 @@ namespace fp4 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kPieces = 2;  // of eight dims that a lane gathers: their slots and codes are in flight together
 
 enum SlotMode { kSlots = 0, kBatch = 1, kRange = 2 };
 
@@ -104,9 +105,10 @@ __global__ __launch_bounds__(kThreads) void fp4_write_kernel(RowArgs a) {
     if (i >= a.lanes) return;
     const int plane = blockIdx.y;
     const Place p = place_of(a, i);
+    // (The row is loaded beside its slot, and for nothing where that does not exist.)
+    const u32x4 x = load_row<VEC16>(a.rows[plane] + p.t * a.row_stride[plane] + (p.head * a.dim + p.chunk * 8) * 2);
     int64_t page, place;
     if (!locate<MODE>(a, p.t, page, place)) return;
-    const u32x4 x = load_row<VEC16>(a.rows[plane] + p.t * a.row_stride[plane] + (p.head * a.dim + p.chunk * 8) * 2);
     uint32_t most = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) most = max(most, max(x[k] & 0x7fffu, (x[k] >> 16) & 0x7fffu));
@@ -129,27 +131,36 @@ __global__ __launch_bounds__(kThreads) void fp4_write_kernel(RowArgs a) {
 
 template <typename T, int MODE, bool VEC16>
 __global__ __launch_bounds__(kThreads) void fp4_gather_kernel(RowArgs a) {
-    const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
-    if (i >= a.lanes) return;
+    const uint32_t first = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
     const int plane = blockIdx.y;
-    const Place p = place_of(a, i);
-    int64_t page, place;
-    u32x4 x = {0u, 0u, 0u, 0u};
-    if (locate<MODE>(a, p.t, page, place)) {
-        const uint8_t* record = a.cache[plane] + (page * a.kv_heads + p.head) * a.record;
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(record + place * (a.dim / 2) + p.chunk * 4);
-        const uint32_t byte = record[a.block_size * (a.dim / 2) + place * (a.dim / kBlockDims) + p.chunk / 4];
-        x = values_of<T>(w, scale_of(byte));
-    }
-    uint8_t* to = a.rows[plane] + p.t * a.row_stride[plane] + (p.head * a.dim + p.chunk * 8) * 2;
-    if constexpr (VEC16) {
-        *reinterpret_cast<u32x4*>(to) = x;
-    } else {
-        uint16_t* h = reinterpret_cast<uint16_t*>(to);
+    Place p[kPieces];
+    bool there[kPieces];
+    uint32_t codes[kPieces], byte[kPieces];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            h[2 * k] = (uint16_t)x[k];
-            h[2 * k + 1] = (uint16_t)(x[k] >> 16);
+    for (int n = 0; n < kPieces; ++n) {
+        p[n] = place_of(a, min(first + n * kThreads, a.lanes - 1));
+        int64_t page, place;
+        there[n] = locate<MODE>(a, p[n].t, page, place);
+        const uint8_t* record = a.cache[plane] + ((there[n] ? page : 0) * a.kv_heads + p[n].head) * a.record;
+        if (!there[n]) place = 0;
+        codes[n] = *reinterpret_cast<const uint32_t*>(record + place * (a.dim / 2) + p[n].chunk * 4);
+        byte[n] = record[a.block_size * (a.dim / 2) + place * (a.dim / kBlockDims) + p[n].chunk / 4];
+    }
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+        if (first + n * kThreads >= a.lanes) return;
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (there[n]) x = values_of<T>(codes[n], scale_of(byte[n]));
+        uint8_t* to = a.rows[plane] + p[n].t * a.row_stride[plane] + (p[n].head * a.dim + p[n].chunk * 8) * 2;
+        if constexpr (VEC16) {
+            *reinterpret_cast<u32x4*>(to) = x;
+        } else {
+            uint16_t* h = reinterpret_cast<uint16_t*>(to);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                h[2 * k] = (uint16_t)x[k];
+                h[2 * k + 1] = (uint16_t)(x[k] >> 16);
+            }
         }
     }
 }
@@ -214,7 +225,7 @@ int launch_write(const RowArgs& a, int dtype, void* stream) {
 template <int MODE>
 int launch_gather(const RowArgs& a, int dtype, void* stream) {
     if (a.lanes == 0) return MVME_OK;
-    const dim3 grid((a.lanes - 1) / kThreads + 1, 2), block(kThreads);
+    const dim3 grid((a.lanes - 1) / (kThreads * kPieces) + 1, 2), block(kThreads);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool vec = vector_rows(a);
     if (dtype == MVME_FP16) {
