@@ -471,7 +471,8 @@ __global__ __launch_bounds__(kThreads) void fp4_prefill_merge_kernel(PrefillArgs
     const int64_t head = (int64_t)blockIdx.x * kMergeRows<D> + threadIdx.x / (D / 4);
     const int d = threadIdx.x % (D / 4) * 4;
     if ((int)threadIdx.x >= kMergeRows<D> * (D / 4) || head >= a.total_tokens * a.q_heads) return;
-    const int chunks = a.counts[head];
+    // (Bounded, for rows that nothing counted: offsets that fall name more row blocks than there are work-groups.)
+    const int chunks = min(a.counts[head], a.chunks);
     if (chunks < 0) return;  // cleared by the first kernel
     typedef float f32x2 __attribute__((ext_vector_type(2)));
     const f32x2* stats = reinterpret_cast<const f32x2*>(a.partial + a.stats) + head * a.chunks;

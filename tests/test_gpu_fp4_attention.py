@@ -230,6 +230,17 @@ def test_prefill_offsets_out_of_order_stay_in_bounds():
 
 
 @pytest.mark.parametrize("chunk", [0, 64])
+def test_prefill_offsets_that_fall_name_too_many_rows(chunk):
+    """More row blocks than work-groups: what rows get is open, but every access stays in bounds."""
+    args, block = prefill_case((300,) + (0,) * 8, (9,) * 9, torch.bfloat16)
+    args[3] = torch.tensor([0, 300] * 5)
+    args[6] = torch.full((9,), int(args[6].max()))
+    out = run_prefill(args, block, validate=False, chunk_tokens=chunk)
+    torch.cuda.synchronize()
+    assert out.shape == args[0].shape
+
+
+@pytest.mark.parametrize("chunk", [0, 64])
 @pytest.mark.parametrize("plane", [1, 2])
 def test_prefill_nan_behind_the_mask_stays_there(plane, chunk):
     """A NaN block reaches the rows that see its key and no other (in particular not as 0 * NaN)."""
