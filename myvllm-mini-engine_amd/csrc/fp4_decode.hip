@@ -507,8 +507,10 @@ struct Plan {
 
 constexpr int64_t kWalkGroups = 1024;  // four per CU: what registers hold at once up to 128 dims
 // Units go out whole where they are short: up to 512 tokens the join costs more than it shares out (64 sequences of 512: 9.6
-// us whole, 13.9 shared), and up to 2048 where they fill the chip (128 ragged sequences: 35.7 us whole, 42.3 shared; one
-// long among short ones takes 17 us alone).
+// us whole, 13.9 shared), and where they are many for their length: up to 2048 tokens from 1024 units on (128 ragged
+// sequences: 35.7 us whole, 42.3 shared), 4096 from 2048 on (256 ragged ones: 125 us, 154), and so on; 512 units of up to
+// 4096 are shared (33.9 us, 45.2 whole).  What one long sequence among short ones takes alone, 1.06 us per 128 tokens, is
+// then at most what a CU has to do anyway.
 constexpr int64_t kShortRounds = 4, kManyUnits = 1024, kManyRounds = 16;
 constexpr int64_t kMostRounds = int64_t(1) << 30;
 
@@ -529,9 +531,11 @@ Plan plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t block_size, 
     if (partition_tokens > 0) {
         const int64_t share = (partition_tokens + kRound - 1) / kRound;
         if (share >= rounds && partition_tokens >= capacity) return {0, 0};
-        return {(units * rounds - 1) / share + 1, share};
+        // (Rounds are counted in 32 bits; the call refuses more.)
+        return {units * rounds > kMostRounds ? kMostRounds + 1 : (units * rounds - 1) / share + 1, share};
     }
-    if (rounds <= kShortRounds || (units >= kManyUnits && rounds <= kManyRounds)) return {0, 0};
+    if (rounds <= kShortRounds || units * rounds > kMostRounds || rounds <= units / kManyUnits * kManyRounds)
+        return {0, 0};
     return {units * rounds < kWalkGroups ? units * rounds : kWalkGroups, 0};
 }
 

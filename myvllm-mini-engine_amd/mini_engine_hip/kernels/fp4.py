@@ -278,6 +278,9 @@ def paged_attention_fp4(query, key_cache, value_cache, block_tables, context_len
     if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device
                             or not out.is_contiguous()):
         raise ValueError("output buffer must match the query")
+    if out is not None and any(ext.share_bytes(out, tensor) for tensor in (
+            query, key_cache, value_cache, block_tables, context_lens, workspace) if tensor is not None):
+        raise ValueError("output buffer must not overlap the inputs or the workspace")
     if validate:
         for length, table in zip(context_lens.tolist(), block_tables.tolist()):
             if not 0 < length <= width * block_size:
@@ -288,8 +291,6 @@ def paged_attention_fp4(query, key_cache, value_cache, block_tables, context_len
     query = _dense(query)
     if out is None:
         out = torch.empty_like(query)
-    elif ext.share_bytes(out, query):
-        raise ValueError("output buffer must not overlap the query")
     lib = ext.load_hip_extension()
     need = lib.fp4_workspace_size(batch, q_heads, kv_heads, head_dim, block_size, width, partition_tokens)
     ws_ptr, ws_bytes, workspace = _workspace(workspace, need, query.device)

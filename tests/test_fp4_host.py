@@ -170,6 +170,29 @@ def test_attention_refuses():
     prefill("physical page", q, kc, vc, cu, starts, ids(0, -1, 2, 3).view(2, 2), lens, block)
 
 
+def test_rounds_that_pass_32_bits(lib):
+    """A million short sequences in tables of a million tokens: whole units by default, no partitions on request."""
+    shape = (1 << 20, 8, 8, 128, 16, 65536)
+    assert lib.fp4_workspace_size(*shape, 0) == 0
+    with pytest.raises(RuntimeError, match="too many partitions"):
+        lib.call("mvme_fp4_paged_attention", *[4096] * 6, *shape[:4], 64, *shape[4:], 1 << 19, 0, 4096, 1 << 40, None)
+    assert lib.fp4_workspace_size(64, 8, 8, 128, 16, 65536, 0) > 0
+
+
+def test_output_must_not_share_bytes_with_inputs():
+    kc, vc, _, _, block = packed_inputs()
+    query, tables, lens = torch.randn(2, 4, 64).half(), ids(0, 1, 2, 3).view(2, 2), ids(8, 3)
+    size = 2 * 4 * 64
+    for cache in (kc, vc):
+        with pytest.raises(ValueError, match="overlap"):
+            paged_attention_fp4(query, kc, vc, tables, lens, block,
+                                out=cache.view(-1)[:2 * size].view(torch.float16).view(2, 4, 64))
+    shared = torch.empty(4 * size, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="overlap"):
+        paged_attention_fp4(query, kc, vc, tables, lens, block, workspace=shared,
+                            out=shared[:2 * size].view(torch.float16).view(2, 4, 64))
+
+
 def test_page_operators_refuse():
     cache = torch.zeros(2, 5, 4, 8)
 
