@@ -297,6 +297,16 @@ def test_prefill_many_sequences():
     f4.assert_within(run_prefill(args, block), *f4.prefill_oracle(*args, block))
 
 
+@pytest.mark.parametrize("chunk", [0, 64])
+@pytest.mark.parametrize("count", [2, 63, 64, 65, 129])
+def test_prefill_sequence_counts(count, chunk):
+    """Row blocks are handed out in two ways, up to 64 sequences and above; some have none, some several."""
+    new = [(7 * i * i + 3 * i) % 11 * (i % 5 > 0) + 150 * (i % 40 == 1) for i in range(count)]
+    prior = [(13 * i) % 170 for i in range(count)]
+    args, block = prefill_case(tuple(new), tuple(prior), torch.bfloat16, heads=4, kv=1, dim=32)
+    f4.assert_within(run_prefill(args, block, validate=False, chunk_tokens=chunk), *f4.prefill_oracle(*args, block))
+
+
 def test_prefill_of_single_rows_equals_decode():
     """One new token per sequence is a decode step: both kernels are within their bounds of each other."""
     args, block = decode_case((1, 300, 77), torch.bfloat16)
