@@ -9,7 +9,7 @@
 //
 // Bound by those bytes for many rows, by a launch and the chain from slot to
 // store for few: 16384 tokens of 8 heads of 128 written and read back in 37.6
-// us (152 MB: 4.05 TB/s, a large copy reaches 4.76), 32 tokens in 5.7 us.
+// us (152 MB: 4.05 TB/s, a large copy reaches 4.76), 32 tokens in 5.1 us.
 #include "fp4_cache.h"
 
 namespace mvme {
@@ -17,9 +17,9 @@ namespace fp4 {
 namespace {
 
 constexpr int kThreads = 256;
-// Pieces of eight dims per lane, whose loads are in flight together (16384 tokens: 42.7 us with one, 37.6 with two, 38.3 with
-// four; 32 tokens 5.2, 5.7 and 7.3).
-constexpr int kPieces = 2;
+// Pieces of eight dims per lane: two, whose loads are in flight together, where there are more than the chip's lanes take at
+// once, else one (16384 tokens: 39.7 us with one, 37.6 with two, 38.3 with four; 32 tokens: 5.1, 5.7 and 7.3).
+constexpr uint32_t kManyLanes = 256 * 2048;
 
 enum SlotMode { kSlots = 0, kBatch = 1, kRange = 2 };
 
@@ -104,16 +104,16 @@ __device__ inline uint32_t codes_into(uint32_t w, uint32_t pair, float scale) {
         return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, pair), scale, SEL);
 }
 
-template <typename T, int MODE, bool VEC16>
+template <typename T, int MODE, bool VEC16, int PIECES>
 __global__ __launch_bounds__(kThreads) void fp4_write_kernel(RowArgs a) {
-    const uint32_t first = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
+    const uint32_t first = blockIdx.x * (kThreads * PIECES) + threadIdx.x;
     const int plane = blockIdx.y;
-    Place p[kPieces];
-    u32x4 rows[kPieces];
-    int64_t page[kPieces], place[kPieces];
-    bool there[kPieces];
+    Place p[PIECES];
+    u32x4 rows[PIECES];
+    int64_t page[PIECES], place[PIECES];
+    bool there[PIECES];
 #pragma unroll
-    for (int n = 0; n < kPieces; ++n) {
+    for (int n = 0; n < PIECES; ++n) {
         // Whole quads are behind the end together: lanes is a multiple of 4.
         const uint32_t i = first + n * kThreads;
         p[n] = place_of(a, min(i, a.lanes - 1));
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void fp4_write_kernel(RowArgs a) {
         there[n] = locate<MODE>(a, p[n].t, page[n], place[n]) && i < a.lanes;
     }
 #pragma unroll
-    for (int n = 0; n < kPieces; ++n) {
+    for (int n = 0; n < PIECES; ++n) {
         if (!there[n]) continue;
         const u32x4 x = rows[n];
         uint32_t most = 0;
@@ -146,15 +146,15 @@ __global__ __launch_bounds__(kThreads) void fp4_write_kernel(RowArgs a) {
     }
 }
 
-template <typename T, int MODE, bool VEC16>
+template <typename T, int MODE, bool VEC16, int PIECES>
 __global__ __launch_bounds__(kThreads) void fp4_gather_kernel(RowArgs a) {
-    const uint32_t first = blockIdx.x * (kThreads * kPieces) + threadIdx.x;
+    const uint32_t first = blockIdx.x * (kThreads * PIECES) + threadIdx.x;
     const int plane = blockIdx.y;
-    Place p[kPieces];
-    bool there[kPieces];
-    uint32_t codes[kPieces], byte[kPieces];
+    Place p[PIECES];
+    bool there[PIECES];
+    uint32_t codes[PIECES], byte[PIECES];
 #pragma unroll
-    for (int n = 0; n < kPieces; ++n) {
+    for (int n = 0; n < PIECES; ++n) {
         p[n] = place_of(a, min(first + n * kThreads, a.lanes - 1));
         int64_t page, place;
         there[n] = locate<MODE>(a, p[n].t, page, place);
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kThreads) void fp4_gather_kernel(RowArgs a) {
         byte[n] = record[a.block_size * (a.dim / 2) + place * (a.dim / kBlockDims) + p[n].chunk / 4];
     }
 #pragma unroll
-    for (int n = 0; n < kPieces; ++n) {
+    for (int n = 0; n < PIECES; ++n) {
         if (first + n * kThreads >= a.lanes) return;
         u32x4 x = {0u, 0u, 0u, 0u};
         if (there[n]) x = values_of<T>(codes[n], scale_of(byte[n]));
@@ -223,36 +223,46 @@ bool vector_rows(const RowArgs& a) {
     return aligned(a.rows[0], 16) && aligned(a.rows[1], 16) && a.row_stride[0] % 16 == 0 && a.row_stride[1] % 16 == 0;
 }
 
-template <int MODE>
-int launch_write(const RowArgs& a, int dtype, void* stream) {
-    if (a.lanes == 0) return MVME_OK;
-    const dim3 grid((a.lanes - 1) / (kThreads * kPieces) + 1, 2), block(kThreads);
+template <int MODE, int PIECES>
+int launch_write_pieces(const RowArgs& a, int dtype, void* stream) {
+    const dim3 grid((a.lanes - 1) / (kThreads * PIECES) + 1, 2), block(kThreads);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool vec = vector_rows(a);
     if (dtype == MVME_FP16) {
-        if (vec) hipLaunchKernelGGL((fp4_write_kernel<Half, MODE, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((fp4_write_kernel<Half, MODE, false>), grid, block, 0, s, a);
+        if (vec) hipLaunchKernelGGL((fp4_write_kernel<Half, MODE, true, PIECES>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((fp4_write_kernel<Half, MODE, false, PIECES>), grid, block, 0, s, a);
     } else {
-        if (vec) hipLaunchKernelGGL((fp4_write_kernel<BFloat16, MODE, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((fp4_write_kernel<BFloat16, MODE, false>), grid, block, 0, s, a);
+        if (vec) hipLaunchKernelGGL((fp4_write_kernel<BFloat16, MODE, true, PIECES>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((fp4_write_kernel<BFloat16, MODE, false, PIECES>), grid, block, 0, s, a);
     }
     return check_launch("packed KV write");
 }
-
 template <int MODE>
-int launch_gather(const RowArgs& a, int dtype, void* stream) {
+int launch_write(const RowArgs& a, int dtype, void* stream) {
     if (a.lanes == 0) return MVME_OK;
-    const dim3 grid((a.lanes - 1) / (kThreads * kPieces) + 1, 2), block(kThreads);
+    return a.lanes > kManyLanes ? launch_write_pieces<MODE, 2>(a, dtype, stream)
+                                : launch_write_pieces<MODE, 1>(a, dtype, stream);
+}
+
+template <int MODE, int PIECES>
+int launch_gather_pieces(const RowArgs& a, int dtype, void* stream) {
+    const dim3 grid((a.lanes - 1) / (kThreads * PIECES) + 1, 2), block(kThreads);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool vec = vector_rows(a);
     if (dtype == MVME_FP16) {
-        if (vec) hipLaunchKernelGGL((fp4_gather_kernel<Half, MODE, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((fp4_gather_kernel<Half, MODE, false>), grid, block, 0, s, a);
+        if (vec) hipLaunchKernelGGL((fp4_gather_kernel<Half, MODE, true, PIECES>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((fp4_gather_kernel<Half, MODE, false, PIECES>), grid, block, 0, s, a);
     } else {
-        if (vec) hipLaunchKernelGGL((fp4_gather_kernel<BFloat16, MODE, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((fp4_gather_kernel<BFloat16, MODE, false>), grid, block, 0, s, a);
+        if (vec) hipLaunchKernelGGL((fp4_gather_kernel<BFloat16, MODE, true, PIECES>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((fp4_gather_kernel<BFloat16, MODE, false, PIECES>), grid, block, 0, s, a);
     }
     return check_launch("packed KV gather");
+}
+template <int MODE>
+int launch_gather(const RowArgs& a, int dtype, void* stream) {
+    if (a.lanes == 0) return MVME_OK;
+    return a.lanes > kManyLanes ? launch_gather_pieces<MODE, 2>(a, dtype, stream)
+                                : launch_gather_pieces<MODE, 1>(a, dtype, stream);
 }
 
 }  // namespace

@@ -88,6 +88,37 @@ def test_write_and_read_back(dtype, dim, block, heads):
         assert torch.equal(v.cpu().double(), f4.values(*f4.quantise(value)))
 
 
+@pytest.mark.parametrize("strided", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_rows_than_the_chip_takes_at_once(dtype, strided):
+    """Lanes with two pieces, the last ones with one; slots that do not exist among them."""
+    gen = torch.Generator().manual_seed(8)
+    tokens, heads, dim, block, pages = 769, 57, 96, 7, 120
+    key, value = (torch.randn(tokens, heads, dim, generator=gen).to(dtype) for _ in range(2))
+    slots = torch.randperm(pages * block, generator=gen)[:tokens]
+    slots[5::50] = -1
+    slots[9::50] = pages * block + 3
+    exists = (slots >= 0) & (slots < pages * block)
+    sources = [x.to(DEV) for x in (key, value)]
+    if strided:  # rows that start at odd places
+        sources = [torch.nn.functional.pad(x.view(tokens, -1), (1, 0))[:, 1:].view(tokens, heads, dim) for x in sources]
+    kc, vc = caches(pages, heads, block, dim)
+    before = kc.clone()
+    write_kv_cache_slots_fp4(kc, vc, slots.to(DEV), *sources, block, validate=False)
+    assert torch.equal(kc.cpu(), written(before, key, slots, block))
+    assert torch.equal(vc.cpu(), written(before, value, slots, block))
+    k, v = gather_kv_cache_slots_fp4(kc, vc, slots.to(DEV), block, dim, dtype, validate=False)
+    for got, rows in ((k, key), (v, value)):
+        assert torch.equal(got.cpu().double(), f4.values(*f4.quantise(rows)) * exists.view(-1, 1, 1))
+    tables = torch.arange(pages, device=DEV).view(1, pages).expand(tokens, pages).contiguous()
+    again = caches(pages, heads, block, dim)
+    write_kv_cache_batch_fp4(*again, tables, slots.to(DEV), *sources, block, validate=False)
+    assert torch.equal(again[0], kc) and torch.equal(again[1], vc)
+    k, _ = gather_kv_cache_fp4(kc, vc, tables[0].contiguous(), pages * block, block, dim, dtype)
+    # (Slots that nothing wrote hold the fill, whose scale 2^38 no written block has: past 65504 fp16 reads infinity.)
+    assert torch.equal(k.cpu(), f4.cache_values(kc.cpu(), block, dim).flatten(0, 1).to(dtype))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_strided_and_unaligned_rows(dtype):
     """Slices of a fused projection, an odd token stride, rows that start two bytes off, and a view that is copied."""
