@@ -194,7 +194,8 @@ __device__ inline bool find_in_order(const PrefillArgs& a, int lane, int& item, 
     return false;
 }
 // The same for up to 64 sequences with the blocks that see most keys first, to a tile: they take longest, and the short
-// ones fill what the chip has free at the end.
+// ones fill what the chip has free at the end (12 mixed sequences 42.5 us, in order 49.1; 32 x 256 tokens behind 4096 keys
+// 188 and 240; equal blocks pay 1 us for the search).  One wave has a lane for each of 64 sequences; more go in order.
 __device__ inline bool find_longest_first(const PrefillArgs& a, int lane, int& item, int& s) {
     const int own = min(lane, a.num_seqs - 1);
     const int blocks = lane < a.num_seqs ? row_blocks(a, own) : 0;
