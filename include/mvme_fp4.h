@@ -91,7 +91,7 @@ size_t mvme_fp4_paged_attention_workspace_size(int64_t batch, int64_t q_heads, i
  * accumulators are fp32.  Probabilities are rounded to fp16 for the value
  * product, relative to a reference that keeps the largest between 2^8 and
  * 2^16: they have 11 bits from 2^-22 of the largest on and are lost below
- * 2^-33 of it.
+ * 2^-33 of it.  The sum that divides is of the rounded ones.
  */
 int mvme_fp4_paged_attention(void* out, const void* query, const void* key_cache, const void* value_cache,
                              const int64_t* block_tables, const int64_t* context_lens,

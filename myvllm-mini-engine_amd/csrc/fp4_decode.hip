@@ -375,13 +375,13 @@ __global__ __launch_bounds__(64 * kWaves, Shape<D>::kMinWaves) void fp4_decode_k
             for (int s = 0; s < 2; ++s) {
                 float p[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    p[j] = fast_exp2(__builtin_fmaf(x[s][j], a.scale, -ref));
-                    sum += p[j];
-                }
+                for (int j = 0; j < 4; ++j) p[j] = fast_exp2(__builtin_fmaf(x[s][j], a.scale, -ref));
                 weights[2 * s] = Half::pack(p[0], p[1]);
                 weights[2 * s + 1] = Half::pack(p[2], p[3]);
             }
+            // The sum is of the weights as rounded: what a rounding adds to the values' product it adds to the divisor.
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum = Half::dot2(weights[i], 0x3c003c00u, sum);
             // A wave reads only what it wrote: the LDS queue is in order, no barrier.
 #pragma unroll
             for (int n = 0; n < S::kDimTiles; ++n) {

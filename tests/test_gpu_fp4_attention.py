@@ -371,3 +371,45 @@ def test_graph_replays_follow_their_inputs():
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(captured, eager))
+
+
+# ---------------------------------------------------------------------------
+# Rounded probabilities and their sum
+# ---------------------------------------------------------------------------
+def equal_values_case(n, heads, dim, seed):
+    """n keys of which the first is another than the equal rest, every value 4, one kv head."""
+    gen = torch.Generator().manual_seed(seed)
+    tables, pages = f4.tables_of(gen, (n,), 16)
+    keys = torch.zeros(pages, 1, 16, dim) + torch.randn(dim, generator=gen)
+    keys[tables[0, 0], 0, 0] = torch.randn(dim, generator=gen)
+    kc, vc = f4.packed(keys.half()), f4.packed(torch.full((pages, 1, 16, dim), 4.0).half())
+    return torch.randn(1, heads, dim, generator=gen).half(), kc, vc, tables, torch.tensor([n])
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_average_of_equal_values_is_that_value(dim):
+    """Whatever a probability is rounded to, the sum that divides counts it as rounded: 200 queries, 32 keys.
+
+    What is left is the error of fp32 sums of 32 terms, 2^-24 * 64 at most, and fp16 has its next value 2^-11 below 4.
+    """
+    query, kc, vc, tables, lens = equal_values_case(32, 200, dim, dim)
+    assert (run_decode([query, kc, vc, tables, lens], 16) == 4).all()
+    assert (run_prefill([query, kc, vc, torch.tensor([0, 1]), lens - 1, tables, lens], 16) == 4).all()
+
+
+def test_average_of_equal_values_with_most_keys_far_below_one():
+    """8191 keys at 2^-23 of the first, which fp16 holds as subnormals: they count in both sums, or in neither.
+
+    A lane adds at most 2048 pairs to the sum and 512 products to the values, each off by 2^-24 of it: 2^-12.7 in
+    all, and from 2^-12 on the result would round to the value below 4.  Lost on one side alone they would be 2^-10.
+    """
+    n, dim = 8192, 64
+    gen = torch.Generator().manual_seed(1)
+    tables, pages = f4.tables_of(gen, (n,), 16)
+    keys = torch.zeros(pages, 1, 16, dim)
+    keys[tables[0, 0], 0, 0] = 2.0
+    kc, vc = f4.packed(keys.half()), f4.packed(torch.full((pages, 1, 16, dim), 4.0).half())
+    query, lens = torch.ones(1, 1, dim).half(), torch.tensor([n])
+    assert (run_decode([query, kc, vc, tables, lens], 16, partition_tokens=n) == 4).all()
+    args = [query, kc, vc, torch.tensor([0, 1]), lens - 1, tables, lens]
+    assert (run_prefill(args, 16, chunk_tokens=n) == 4).all()
