@@ -14,6 +14,10 @@ namespace mvme {
 
 constexpr int kWave = 64;
 
+// Threads of one launch along x.  The runtime counts them in 32 bits: a larger
+// grid is not refused, it runs what is left modulo 2^32.
+constexpr int64_t kMostThreads = 4294967295;
+
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

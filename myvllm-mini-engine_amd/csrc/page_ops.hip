@@ -21,6 +21,7 @@ struct PageArgs {
     int64_t num_planes, num_pages, page_bytes, moves;
     int64_t pieces;     // work-groups per page and plane
     int64_t copies;     // work-groups that copy; the others renumber
+    int64_t first;      // work-group that a launch begins with
     int64_t* tables;
     int64_t entries;
 };
@@ -64,7 +65,7 @@ __device__ inline void renumber(const PageArgs& a, int64_t group) {
 
 template <typename Unit>
 __global__ __launch_bounds__(kThreads) void move_pages_kernel(PageArgs a) {
-    const int64_t group = blockIdx.x;
+    const int64_t group = a.first + blockIdx.x;
     if (group < a.copies) copy_piece<Unit>(a, group);
     else renumber(a, group - a.copies);
 }
@@ -96,12 +97,18 @@ int move_pages(void* planes, int64_t num_planes, int64_t num_pages, int64_t page
     if (a.pieces > 2147483647 / num_planes / moves || num_planes * moves * a.pieces > 2147483647 - renumbers)
         return fail(MVME_EINVAL, "too many pages to move in one call");
     a.copies = num_planes * moves * a.pieces;
-    const dim3 grid((unsigned)(a.copies + renumbers)), block(kThreads);
+    // One launch, unless there are more work-groups than it can have (millions of small pages).
+    constexpr int64_t kMostGroups = kMostThreads / kThreads;
+    const int64_t groups = a.copies + renumbers;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (unit == 16) hipLaunchKernelGGL((move_pages_kernel<u32x4>), grid, block, 0, s, a);
-    else if (unit == 4) hipLaunchKernelGGL((move_pages_kernel<uint32_t>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((move_pages_kernel<uint8_t>), grid, block, 0, s, a);
-    return check_launch("page move");
+    for (; a.first < groups; a.first += kMostGroups) {
+        const dim3 grid((unsigned)(groups - a.first < kMostGroups ? groups - a.first : kMostGroups)), block(kThreads);
+        if (unit == 16) hipLaunchKernelGGL((move_pages_kernel<u32x4>), grid, block, 0, s, a);
+        else if (unit == 4) hipLaunchKernelGGL((move_pages_kernel<uint32_t>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((move_pages_kernel<uint8_t>), grid, block, 0, s, a);
+        if (int rc = check_launch("page move")) return rc;
+    }
+    return MVME_OK;
 }
 
 }  // namespace

@@ -230,3 +230,15 @@ def test_packed_pool_serves_forked_requests(dtype):
     assert step > 8
     k, v = pool.gather(1, host.table("b"), at, dtype)
     assert torch.equal(k.cpu().double(), history["b"][1][0][:at]) and torch.equal(v.cpu().double(), history["b"][1][1][:at])
+
+
+def test_more_pages_than_one_launch_has_work_groups():
+    """A work-group a page and plane, 2^24 + 10 of them: a launch has at most 2^24 - 1 of 256 threads."""
+    moves = (1 << 23) + 5
+    cache = torch.randint(0, 256, (2, 2 * moves + 3, 16), dtype=torch.uint8, device=DEV)
+    want = cache.clone()
+    want[:, :moves] = cache[:, moves + 3:]
+    dst = torch.arange(moves, device=DEV)
+    tables = torch.tensor([[0, moves + 3, 2 * moves + 2, -1, moves + 1]], device=DEV)
+    compact_kv_pages(cache, dst + moves + 3, dst, tables, page_dim=1, validate=False)
+    assert torch.equal(cache, want) and tables.tolist() == [[0, 0, moves - 1, -1, moves + 1]]
