@@ -604,7 +604,9 @@ extern "C" int mvme_fp4_paged_attention(void* out, const void* query, const void
     if (partition_tokens < 0) return fail(MVME_EINVAL, "partition_tokens must not be negative");
     const Plan p = plan(batch, q_heads, kv_heads, block_size, table_width, partition_tokens);
     const int64_t tiles = (q_heads / kv_heads + 15) / 16, units = batch * kv_heads * tiles;
-    if (p.groups > kMostRounds || units > 2147483647) return fail(MVME_EINVAL, "too many partitions");
+    if (units > kMostThreads / (64 * kWaves)) return fail(MVME_EINVAL, "batch/head product too large");
+    if (p.groups > kMostThreads / (64 * kWaves) || (p.groups && batch * q_heads > kMostThreads / kMergeThreads))
+        return fail(MVME_EINVAL, "too many partitions");
     const size_t need = mvme_fp4_paged_attention_workspace_size(batch, q_heads, kv_heads, head_dim, block_size,
                                                                 table_width, partition_tokens);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))

@@ -613,7 +613,9 @@ extern "C" int mvme_fp4_paged_prefill_attention(void* out, const void* q, const 
     if (!aligned(q, 16) || !aligned(key_cache, 16) || !aligned(value_cache, 16) || !aligned(out, 8))
         return fail(MVME_EINVAL, "packed prefill: queries and caches must be 16-byte, the output 8-byte aligned");
     const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width, chunk_tokens);
-    if (p.chunks > 2147483647 / kv_heads / p.items) return fail(MVME_EINVAL, "too many packed query rows");
+    if (p.chunks > kMostThreads / kThreads / kv_heads / p.items ||
+        (p.chunks > 1 && (total_tokens * q_heads - 1) / (kThreads / (head_dim / 4)) >= kMostThreads / kThreads))
+        return fail(MVME_EINVAL, "too many packed query rows");
     const size_t need = mvme_fp4_paged_prefill_workspace_size(num_seqs, total_tokens, q_heads, kv_heads, head_dim,
                                                               block_size, table_width, chunk_tokens);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))

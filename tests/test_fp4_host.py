@@ -301,3 +301,25 @@ def test_c_entry_points_refuse_before_launch(lib):
                           ({"size": 1 << 40, "pages": 1 << 20, "moves": 1 << 20}, "too many")):
         assert move(**args) == ext.EINVAL and message in lib.last_error(), (args, lib.last_error())
     assert move(moves=0, src=None, dst=None) == ext.OK
+
+
+def test_launches_that_do_not_fit_are_refused(lib):
+    """A launch has at most 2^32 - 1 threads; what would need more, and so run short, is refused before it starts."""
+    def decode(match, batch, heads, kv, dim, block, width, part):
+        with pytest.raises(RuntimeError, match=match):
+            lib.call("mvme_fp4_paged_attention", *[4096] * 6, batch, heads, kv, dim, 64, block, width, part, 0, 4096,
+                     1 << 60, None)
+
+    decode("head product too large", 1 << 24, 1, 1, 64, 16, 1, 0)       # a work-group of 256 threads per sequence
+    decode("head product too large", 1 << 20, 256, 1, 64, 16, 1, 0)     # ... and 16 heads
+    decode("too many partitions", 1 << 12, 1, 1, 64, 16, 1 << 16, 128)  # 2^25 rounds of 128 tokens
+    decode("too many partitions", 1 << 21, 8, 1, 64, 16, 16, 128)       # the join has one per head
+
+    def prefill(seqs, total, heads, kv, dim, width, chunk):
+        with pytest.raises(RuntimeError, match="too many packed query rows"):
+            lib.call("mvme_fp4_paged_prefill_attention", *[4096] * 8, seqs, total, heads, kv, dim, 64, 16, width, chunk,
+                     0, 4096, 1 << 60, None)
+
+    prefill(1 << 24, 1 << 24, 1, 1, 64, 1, 0)
+    prefill(1, 1 << 20, 16, 1, 64, 1 << 16, 64)     # 2^17 row blocks, 2^14 chunks
+    prefill(1, 1 << 20, 128, 1, 256, 8, 64)         # 2^25 joining work-groups of four rows
