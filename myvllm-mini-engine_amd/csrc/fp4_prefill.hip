@@ -460,7 +460,8 @@ __global__ __launch_bounds__(kThreads, Shape<D>::kMinWaves) void fp4_prefill_ker
     if (a.chunks > 1 && h == 0) {
         a.partial[a.stats + at * 2] = ref;
         a.partial[a.stats + at * 2 + 1] = total;
-        if (chunk == 0) a.counts[head] = limit < 0 ? 0 : limit / a.chunk_len + 1;
+        // (Starts that cannot be make any limit of themselves, but leave no keys.)
+        if (chunk == 0) a.counts[head] = limit < 0 || end == 0 ? 0 : limit / a.chunk_len + 1;
     }
 }
 

@@ -413,3 +413,14 @@ def test_average_of_equal_values_with_most_keys_far_below_one():
     assert (run_decode([query, kc, vc, tables, lens], 16, partition_tokens=n) == 4).all()
     args = [query, kc, vc, torch.tensor([0, 1]), lens - 1, tables, lens]
     assert (run_prefill(args, 16, chunk_tokens=n) == 4).all()
+
+
+@pytest.mark.parametrize("start", [70 - (1 << 32), (1 << 32) + 70, -(1 << 63), (1 << 63) - 1, -1])
+def test_prefill_starts_that_cannot_be_see_no_keys(start):
+    """Nor do their rows take anything from the workspace: 70 alone would be a key of the second chunk."""
+    args, block = prefill_case((40, 20), (200, 100), torch.bfloat16)
+    args[4][0] = start
+    workspace = torch.ones(fp4_prefill_workspace_bytes(2, 60, 4, 2, 128, block, args[5].shape[1], 64) // 4, device=DEV)
+    got = run_prefill(args, block, validate=False, chunk_tokens=64, workspace=workspace)
+    f4.assert_within(got, *f4.prefill_oracle(*args, block))
+    assert not got[:40].any() and got[40:].any()
