@@ -529,8 +529,8 @@ Plan plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t block_size, 
     const int64_t units = batch * kv_heads * ((q_heads / kv_heads + 15) / 16);
     const int64_t rounds = (capacity - 1) / kRound + 1;  // of a unit, at most
     if (partition_tokens > 0) {
+        if (partition_tokens >= capacity) return {0, 0};  // (before it is added to: it may be any number)
         const int64_t share = (partition_tokens + kRound - 1) / kRound;
-        if (share >= rounds && partition_tokens >= capacity) return {0, 0};
         // (Rounds are counted in 32 bits; the call refuses more.)
         return {units * rounds > kMostRounds ? kMostRounds + 1 : (units * rounds - 1) / share + 1, share};
     }

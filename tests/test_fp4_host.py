@@ -323,3 +323,10 @@ def test_launches_that_do_not_fit_are_refused(lib):
     prefill(1 << 24, 1 << 24, 1, 1, 64, 1, 0)
     prefill(1, 1 << 20, 16, 1, 64, 1 << 16, 64)     # 2^17 row blocks, 2^14 chunks
     prefill(1, 1 << 20, 128, 1, 256, 8, 64)         # 2^25 joining work-groups of four rows
+
+
+@pytest.mark.parametrize("tokens", [2 ** 63 - 1, 2 ** 63 - 127, 2 ** 63 - 128, 1024])
+def test_partitions_and_chunks_of_any_size_leave_one(lib, tokens):
+    """Sizes from the table's capacity on split nothing, up to the largest number that the calls take."""
+    assert lib.fp4_workspace_size(2, 16, 8, 128, 16, 64, tokens) == 0
+    assert lib.fp4_prefill_workspace_size(2, 40, 16, 8, 128, 16, 64, tokens) == 0
