@@ -91,7 +91,8 @@ class PagePool:
         """Give ``new_request`` the first ``token_count`` tokens of a request.
 
         Whole pages are shared; a partly written last page is copied, since both
-        requests write on behind it.  Returns (the new table, page copies).
+        requests write on behind it.  The new table ends with that page:
+        ``extend`` gives it more.  Returns (the new table, page copies).
         """
         if new_request in self._owned:
             raise ValueError(f"request already owns blocks: {new_request}")
@@ -104,6 +105,15 @@ class PagePool:
             self._refs[page] += 1
         self._owned[new_request] = table[:whole] + copy
         return list(self._owned[new_request]), [(table[whole], page) for page in copy]
+
+    def extend(self, request_id: str, token_count: int) -> list[int]:
+        """Give a request the private pages that ``token_count`` tokens need beyond its table, if any.
+
+        Returns its table.  Where the pages run out, nothing has changed.
+        """
+        table = self._owned[request_id]
+        table += self._take(max(0, self.blocks_required(token_count) - len(table)))
+        return list(table)
 
     def make_writable(self, request_id: str, index: int):
         """Before writing into page ``index`` of a table: a page that others hold too is replaced by a copy.

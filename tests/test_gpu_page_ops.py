@@ -242,3 +242,51 @@ def test_more_pages_than_one_launch_has_work_groups():
     tables = torch.tensor([[0, moves + 3, 2 * moves + 2, -1, moves + 1]], device=DEV)
     compact_kv_pages(cache, dst + moves + 3, dst, tables, page_dim=1, validate=False)
     assert torch.equal(cache, want) and tables.tolist() == [[0, 0, moves - 1, -1, moves + 1]]
+
+
+@pytest.mark.parametrize("at", [32, 37])
+def test_branches_of_a_fork_decode_pages_beyond_it(at):
+    """A fork at a page boundary and behind one: both branches write 40 tokens, three new pages each, and every step
+    is within the bounds of float64 on the rows written."""
+    block, kv, heads, dim, steps, dtype = 16, 2, 4, 64, 40, torch.bfloat16
+    gen = torch.Generator().manual_seed(at)
+    pool, host = KVCachePoolFP4(1, 16, block, kv, dim), PagePool(16, block, order=list(range(15, -1, -1)))
+    host.allocate("filler", 3 * block)
+    table = host.allocate("a", at)
+    prompt = [torch.randn(at, kv, dim, generator=gen).to(dtype) for _ in range(2)]
+    pool.write_hip(0, table, 0, prompt[0].to(DEV), prompt[1].to(DEV))
+    _, moves = host.fork("a", "b", at)
+    assert len(moves) == (1 if at % block else 0)
+    pool.copy_pages(moves)
+    requests = ["a", "b"]
+    history = {r: [f4.values(*f4.quantise(x)) for x in prompt] for r in requests}
+    ran = 0
+    for step in range(steps):
+        length = at + step + 1
+        for request in requests:
+            host.extend(request, length)
+            _, moves = host.make_writable(request, (length - 1) // block)
+            assert not moves  # what a branch writes behind the fork is its own
+        tables = torch.tensor([host.table(r) for r in requests], device=DEV)
+        if step == 20:
+            host.free("filler")
+            moves = host.compact()
+            assert moves
+            pool.compact_pages(moves, tables)
+            assert tables.tolist() == [host.table(r) for r in requests]
+        new = [torch.randn(2, kv, dim, generator=gen).to(dtype) for _ in range(2)]
+        lens = torch.tensor([length] * 2, device=DEV)
+        write_kv_cache_batch_fp4(*pool.layer(0), tables, lens - 1, new[0].to(DEV), new[1].to(DEV), block)
+        query = torch.randn(2, heads, dim, generator=gen).to(dtype)
+        got = paged_attention_fp4(query.to(DEV), *pool.layer(0), tables, lens, block)
+        for row, request in enumerate(requests):
+            history[request] = [torch.cat((old, f4.values(*f4.quantise(x[row:row + 1]))))
+                                for old, x in zip(history[request], new)]
+            k, v = history[request]
+            for h in range(heads):
+                f4.assert_within(got[row, h], *f4.attention(query[row, h].double(), k[:, h // 2], v[:, h // 2]))
+        ran += 1
+    assert ran == steps and all(len(host.table(r)) == -(-(at + steps) // block) for r in requests)
+    for request in requests:
+        for rows, want in zip(pool.gather(0, host.table(request), at + steps, dtype), history[request]):
+            assert torch.equal(rows.cpu().double(), want)

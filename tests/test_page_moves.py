@@ -131,3 +131,49 @@ def test_random_life_of_a_pool(seed):
         except MemoryError:
             pass
         model.check()
+
+
+def test_extension_appends_private_pages():
+    pool = PagePool(8, 4)
+    table = pool.allocate("a", 6)
+    assert pool.extend("a", 8) == table and pool.extend("a", 0) == table
+    child, _ = pool.fork("a", "b", 8)  # whole pages: not one token fits behind them
+    assert child == table
+    grown = pool.extend("b", 9)
+    assert grown[:2] == table and len(grown) == 3 and pool.refcount(grown[2]) == 1 and pool.table("b") == grown
+    assert pool.table("a") == table
+    assert len(pool.extend("a", 20)) == 5 and pool.free_blocks == 2
+    for args, error in ((("b", 24), MemoryError), (("b", -1), ValueError), (("x", 4), KeyError)):
+        with pytest.raises(error):
+            pool.extend(*args)
+        assert pool.table("b") == grown and pool.free_blocks == 2
+    pool.free("a")
+    pool.free("b")
+    assert pool.free_blocks == 8
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_branches_grow_past_their_fork(seed):
+    """Forks at any length, page boundaries among them; every branch then writes on, through compactions too."""
+    rng = random.Random(seed)
+    size = rng.choice([1, 3, 4])
+    pool = PagePool(120, size, order=rng.sample(range(120), 120))
+    model = Model(pool)
+    pool.allocate("r0", size)
+    model.text["r0"] = []
+    for step in range(300):
+        request = rng.choice(list(model.text))
+        text = model.text[request]
+        if step % 12 == 11 and len(model.text) < 6:
+            count = rng.choice([0, len(text), len(text) // size * size, rng.randint(0, len(text))])
+            child = f"r{step}"
+            _, moves = pool.fork(request, child, count)
+            model.run(moves)
+            model.text[child] = text[:count]
+        elif step % 31 == 30:
+            model.run(pool.compact())
+        elif len(text) < 15 * size:
+            pool.extend(request, len(text) + 1)
+            model.write(request, rng.random())
+        model.check()
+    assert min(len(text) for text in model.text.values()) > size and len(model.text) == 6
