@@ -244,7 +244,8 @@ def paged_attention_fp4(query, key_cache, value_cache, block_tables, context_len
     returns [B, Hq, D] in the query's type.  ``validate=False`` reads no
     metadata on the host (graph capture); sequences whose length is not
     positive or passes the table give zeros and pages out of range are
-    skipped.  ``partition_tokens`` (0 = library plan) splits sequences over
+    skipped.  A NaN block of a value reaches its own 32 dims of the output.
+    ``partition_tokens`` (0 = library plan) splits sequences over
     work-groups; ``out`` / ``workspace`` may supply the buffers.
     """
     _backend(backend, "decode")
@@ -334,8 +335,9 @@ def paged_prefill_attention_fp4(q, key_cache, value_cache, cu_seqlens_q, query_s
     ``[cu_seqlens_q[s], cu_seqlens_q[s + 1])``, row i of it sits at position
     ``query_starts[s] + i`` and sees the keys up to it; the chunk's own keys
     are read from the cache, so they are written first.  Rows that see no key
-    and rows behind the last sequence are zeros.  ``validate=False`` reads no
-    metadata on the host.  ``chunk_tokens`` (0 = library plan) splits keys over
+    and rows behind the last sequence are zeros.  A NaN block, of a value too,
+    makes the rows that see its key NaN in all dims (decode keeps a value's to
+    its 32).  ``validate=False`` reads no metadata on the host.  ``chunk_tokens`` (0 = library plan) splits keys over
     work-groups; ``workspace`` may supply the buffer for it.
     """
     _backend(backend, "prefill")

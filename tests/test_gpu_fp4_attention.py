@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import fp4_cases as f4
+from mini_engine_hip.kernels import hip_extension as ext
 from mini_engine_hip.kernels.fp4 import (fp4_prefill_workspace_bytes, fp4_workspace_bytes, paged_attention_fp4,
                                          paged_prefill_attention_fp4)
 
@@ -114,6 +115,18 @@ def test_decode_nan_blocks_reach_the_sequences_that_hold_them():
     args[1] = f4.join(code, byte)
     got = run_decode(args, block)
     assert got[1, :2].isnan().all() and not got[1, 2:].isnan().any()
+
+
+def test_decode_keeps_a_nan_value_block_to_its_dims():
+    args, block = decode_case((70, 70), torch.float16, heads=4, kv=2, dim=64)
+    clean = run_decode(args, block)
+    code, byte = f4.split(args[2], block, 64)
+    byte[args[3][0, 2], 1, 5, 1] = 255  # sequence 0, kv head 1, token 37, dims 32 .. 63
+    args[2] = f4.join(code, byte)
+    got = run_decode(args, block)
+    assert got[0, 2:, 32:].isnan().all()
+    got[0, 2:, 32:] = clean[0, 2:, 32:]
+    assert torch.equal(got, clean)
 
 
 def test_decode_long_sequence_and_many_partitions():
@@ -238,6 +251,43 @@ def test_prefill_offsets_that_fall_name_too_many_rows(chunk):
     out = run_prefill(args, block, validate=False, chunk_tokens=chunk)
     torch.cuda.synchronize()
     assert out.shape == args[0].shape
+
+
+@pytest.mark.parametrize("chunk", [0, 64])
+@pytest.mark.parametrize("new,prior,cu", [((31, 20, 20), (9, 3, 10), (0, 50, 30, 71)),
+                                          ((31, 20, 20), (9, 3, 10), (0, 50, 1 << 40, 71)),
+                                          ((31, 20, 20), (9, 3, 10), (-5, 20, 60, 1 << 33)),
+                                          ((31, 20, 20), (9, 3, 10), (71, 71, 0, 3)),
+                                          ((300,) + (0,) * 8, (9,) * 9, (0, 300) * 5)])
+def test_prefill_writes_nothing_beside_its_buffers_whatever_the_offsets(new, prior, cu, chunk):
+    """Offsets out of order: the bytes around the output and the workspace stay, and rows with one owner
+    are right where there are no more row blocks than work-groups (all but the last case)."""
+    args, block = prefill_case(new, prior, torch.bfloat16)
+    args[3] = torch.tensor(cu)
+    query, kc, vc, offsets, starts, tables, lens = [a.to(DEV) for a in args]
+    total, seqs = query.shape[0], len(new)
+    lib = ext.load_hip_extension()
+    need = lib.fp4_prefill_workspace_size(seqs, total, 4, 2, 128, block, tables.shape[1], chunk)
+    out = torch.full((2048 + total * 512 + 2048,), 77, dtype=torch.int16, device=DEV)
+    workspace = torch.full((4096 + need + 4096,), 77, dtype=torch.uint8, device=DEV)
+    lib.call("mvme_fp4_paged_prefill_attention", out[2048:].data_ptr(), query.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+             offsets.data_ptr(), starts.data_ptr(), tables.data_ptr(), lens.data_ptr(), seqs, total, 4, 2, 128,
+             kc.shape[0], block, tables.shape[1], chunk, ext.dtype_code(query.dtype), workspace[4096:].data_ptr(), need,
+             ext.current_stream(query.device))
+    torch.cuda.synchronize()
+    assert (out[:2048] == 77).all() and (out[2048 + total * 512:] == 77).all()
+    assert (workspace[:4096] == 77).all() and (workspace[4096 + need:] == 77).all()
+    clamped = [min(max(c, 0), total) for c in cu]
+    owners = torch.zeros(total, dtype=torch.int64)
+    for low, high in zip(clamped, clamped[1:]):
+        owners[low:max(low, high)] += 1
+    owners[:clamped[0]] += 1  # rows before the first and behind the last offset are cleared
+    owners[max(clamped[0], clamped[-1]):] += 1
+    if seqs == 3:
+        args[3] = torch.tensor(clamped)
+        want, bound = f4.prefill_oracle(*args, block)
+        got = out[2048:2048 + total * 512].view(torch.bfloat16).view(total, 4, 128).cpu()
+        f4.assert_within(got[owners == 1], want[owners == 1], bound[owners == 1])
 
 
 @pytest.mark.parametrize("chunk", [0, 64])
