@@ -47,6 +47,9 @@ inline bool valid_format(int64_t block_size, int64_t head_dim) {
            head_dim % kBlockDims == 0;
 }
 
+// Head dims that the attention kernels are built for.
+inline bool attention_dim(int64_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
+
 // A load by all lanes from one address that no kernel writes meanwhile, through the scalar cache.
 __device__ inline int64_t uniform_load(const int64_t* p) {
     return *(const __attribute__((address_space(4))) int64_t*)(uintptr_t)p;

@@ -514,8 +514,6 @@ constexpr int64_t kWalkGroups = 1024;  // four per CU: what registers hold at on
 constexpr int64_t kShortRounds = 4, kManyUnits = 1024, kManyRounds = 16;
 constexpr int64_t kMostRounds = int64_t(1) << 30;
 
-bool attention_dim(int64_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
-
 bool decode_shape(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t block_size,
                   int64_t width) {
     return batch > 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && attention_dim(head_dim) &&

@@ -31,8 +31,6 @@ constexpr int kThreads = 256;
 constexpr int kRows = 128;   // query rows of a work-group
 constexpr int kKeys = 64;    // keys of a tile
 
-constexpr int kMfma = 0x8, kDsRead = 0x100;  // kinds of instructions for the scheduler
-
 struct PrefillArgs {
     void* out;
     const void* q;
@@ -154,19 +152,9 @@ __device__ inline void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Sum over the lanes up to this one.
-__device__ inline int lane_scan(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // from 1, 2, 4, 8 lanes before, in rows of 16
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last lane of the row before, to rows 1 and 3
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // lane 31, to rows 2 and 3
-    return x;
-}
 // Which of the lanes' row blocks, counted through, is `item`: its lane, and `item` from that lane's first.  -1: behind all.
 __device__ inline int find_lane(int blocks, int& item) {
-    const int scan = lane_scan(blocks);
+    const int scan = wave_incl_scan(blocks);
     const uint64_t behind = __ballot(scan > item);
     if (!behind) return -1;
     const int at = __builtin_ctzll(behind);
@@ -189,7 +177,7 @@ __device__ inline bool find_in_order(const PrefillArgs& a, int lane, int& item, 
             item = __builtin_amdgcn_readlane(blocks, at) - 1 - item;
             return true;
         }
-        item -= __builtin_amdgcn_readlane(lane_scan(blocks), 63);
+        item -= __builtin_amdgcn_readlane(wave_incl_scan(blocks), 63);
     }
     return false;
 }
@@ -207,7 +195,7 @@ __device__ inline bool find_longest_first(const PrefillArgs& a, int lane, int& i
         const uint64_t before = (uint64_t)(uint32_t)max(tile * kKeys - start, 0) * (uint32_t)a.group / kRows;
         return tile == top ? 0 : blocks - (int)min(before, (uint64_t)blocks);
     };
-    const auto all = [&](int n) { return __builtin_amdgcn_readlane(lane_scan(n), 63); };
+    const auto all = [&](int n) { return __builtin_amdgcn_readlane(wave_incl_scan(n), 63); };
     if (item >= all(blocks)) return false;
     int tile = 0;  // the last with more than `item` blocks
     for (int step = half; step > 0; step /= 2)
@@ -490,8 +478,6 @@ __global__ __launch_bounds__(kThreads) void fp4_prefill_merge_kernel(PrefillArgs
     }
     store4<T, D>(a, head, d, total != 0.f ? value * (1.f / total) : f32x4{0.f, 0.f, 0.f, 0.f});
 }
-
-bool attention_dim(int64_t d) { return d == 32 || d == 64 || d == 96 || d == 128 || d == 192 || d == 256; }
 
 bool prefill_shape(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                    int64_t block_size, int64_t width) {
