@@ -91,7 +91,9 @@ size_t mvme_fp4_paged_attention_workspace_size(int64_t batch, int64_t q_heads, i
  * accumulators are fp32.  Probabilities are rounded to fp16 for the value
  * product, relative to a reference that keeps the largest between 2^8 and
  * 2^16: they have 11 bits from 2^-22 of the largest on and are lost below
- * 2^-33 of it.  The sum that divides is of the rounded ones.  A NaN block of a
+ * 2^-33 of it.  The sum that divides is of the rounded ones.  Scores (with
+ * their scale) are meant to stay below 1.1e7 in magnitude, where fp32 still
+ * has their differences; rows beyond may come out as NaN.  A NaN block of a
  * key makes a head's output NaN, one of a value the 32 dims that it holds.
  */
 int mvme_fp4_paged_attention(void* out, const void* query, const void* key_cache, const void* value_cache,
@@ -118,6 +120,8 @@ size_t mvme_fp4_paged_prefill_workspace_size(int64_t num_seqs, int64_t total_tok
  * keys of the chunk itself are read from the cache as well: they are written
  * first.  A NaN block of a key or a value makes all dims of the rows that see
  * its key NaN (decode: only the value's own 32 dims) and touches no others.
+ * Scores are bounded as for decode.  Rows that no sequence owns become zeros,
+ * by one work-group per kv head: leave few of them.
  */
 int mvme_fp4_paged_prefill_attention(void* out, const void* q, const void* key_cache, const void* value_cache,
                                      const int64_t* cu_seqlens_q, const int64_t* query_starts,

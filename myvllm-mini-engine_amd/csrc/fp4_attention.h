@@ -26,9 +26,11 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 // largest score, and moved when a score passes it by 14 (prefill looks when
 // one passes fp16, at 16).  They are rounded to fp16 for the value product
 // (half the products of fp32, and every value of the cache is exact in it):
-// 11 bits from 2^-22 of the largest on, nothing below 2^-33 of it, and none
-// overflows.  The accumulators and the sums that divide them are fp32, both of
-// the probabilities as rounded: what a rounding adds, it adds to both.
+// 11 bits from 2^-22 of the largest on, nothing below 2^-33 of it.  None
+// overflows while scores (in log2) are below 2^24 in magnitude; beyond, a step
+// of fp32 passes 1, and a weight can be as many powers of two off.  The
+// accumulators and the sums that divide them are fp32, both of the
+// probabilities as rounded: what a rounding adds, it adds to both.
 constexpr float kRefBelow = 8.f;
 constexpr float kRefSlack = 14.f;
 constexpr float kRefNone = -3.0e38f;  // no score yet: below every finite one

@@ -474,3 +474,37 @@ def test_prefill_starts_that_cannot_be_see_no_keys(start):
     got = run_prefill(args, block, validate=False, chunk_tokens=64, workspace=workspace)
     f4.assert_within(got, *f4.prefill_oracle(*args, block))
     assert not got[:40].any() and got[40:].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", [1, -1])
+def test_scores_up_to_nine_million(dtype, order):
+    """Keys at 1 and 1.5 times the powers of two up to 2^15, rising or falling: the largest score of a row is 8.9e6.
+
+    Where it is 100 or more above the next (fp32 sums are off by 2^-23 * 272 of it, the next is a quarter below),
+    no other key counts, and the output is its value.
+    """
+    gen = torch.Generator().manual_seed(17)
+    n, dim, block = 64, 128, 16
+    tables, pages = f4.tables_of(gen, (n,), block)
+    at = torch.arange(n)
+    size = (1.0 + 0.5 * (at % 2)) * torch.exp2(at // 2 - 16.0)
+    size = size if order == 1 else size.flip(0)
+    rows = torch.zeros(pages, 1, block, dim)
+    rows[tables[0, at // block], 0, at % block] = size[:, None].expand(n, dim)
+    kc, vc = f4.packed(rows.to(dtype)), f4.packed(torch.randn(pages, 1, block, dim, generator=gen).to(dtype))
+    values = f4.cache_values(vc, block, dim)[tables[0, at // block], at % block, 0]
+    scores = 16.0 * dim ** 0.5 * size
+    assert 8.8e6 < scores.max() < 9e6
+    best = torch.tensor([int(scores[:t + 1].argmax()) for t in range(n)])
+    clear = torch.tensor([t > 0 and scores[:t + 1].topk(2).values.diff().item() <= -100 for t in range(n)])
+    # Rising, the gap at t is 90 * 2^(t // 2 - 16) for odd t and half of it for even ones: 100 or more from t = 35 on.
+    assert clear.sum() == (29 if order == 1 else 63)
+    query = torch.full((n, 1, dim), 16.0).to(dtype)
+    wide = tables.expand(n, -1).contiguous()
+    got = run_decode([query, kc, vc, wide, at + 1], block).cpu().double()[:, 0]
+    assert torch.equal(got[clear], values[best[clear]])
+    for chunk in (0, 64):
+        args = [query, kc, vc, torch.tensor([0, n]), torch.tensor([0]), tables, torch.tensor([n])]
+        got = run_prefill(args, block, chunk_tokens=chunk).cpu().double()[:, 0]
+        assert torch.equal(got[clear], values[best[clear]])
