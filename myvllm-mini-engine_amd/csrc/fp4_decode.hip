@@ -12,9 +12,10 @@
 // sequences of up to 4096 tokens 39 us (22 us at 6.8 TB/s; the start and drain
 // of a work-group and the join are the rest), 4 x 65536 tokens 37 us (21 us),
 // one of 128 tokens 4.1 us (a launch and a chain of table, page and score
-// latency).  Matrix tiles of 16 heads x 32 keys: a lane's four-bit codes are
-// its score operand as they lie in memory, only values go through LDS, for the
-// transposition.
+// latency).  Times in this file are of calls back to back in a graph; from
+// Python the smallest takes 4.9-5.1.  Matrix tiles of 16 heads x 32 keys: a
+// lane's four-bit codes are its score operand as they lie in memory, only
+// values go through LDS, for the transposition.
 #include "fp4_attention.h"
 
 namespace mvme {
@@ -509,8 +510,9 @@ constexpr int64_t kWalkGroups = 1024;  // four per CU: what registers hold at on
 // Units go out whole where they are short: up to 512 tokens the join costs more than it shares out (64 sequences of 512: 9.6
 // us whole, 13.9 shared), and where they are many for their length: up to 2048 tokens from 1024 units on (128 ragged
 // sequences: 35.7 us whole, 42.3 shared), 4096 from 2048 on (256 ragged ones: 125 us, 154), and so on; 512 units of up to
-// 4096 are shared (33.9 us, 45.2 whole).  What one long sequence among short ones takes alone, 1.06 us per 128 tokens, is
-// then at most what a CU has to do anyway.
+// 4096 are shared (33.9 us, 45.2 whole).  The rule sees the tables' width and not the lengths.  Whole, one long sequence among
+// short ones is walked alone at 1.06 us per 128 tokens: one of 2048 tokens and 127 of 16 take 21 us, where sharing takes 14
+// (all 128 of 16 tokens: 5.7).  That much the rule gives up there for what it gains on batches of mostly long ones.
 constexpr int64_t kShortRounds = 4, kManyUnits = 1024, kManyRounds = 16;
 constexpr int64_t kMostRounds = int64_t(1) << 30;
 

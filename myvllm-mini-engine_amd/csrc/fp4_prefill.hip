@@ -11,13 +11,16 @@
 //
 // Per tile a wave has 1024 cycles of products (128 dims), as many of vector
 // work (exponentials, conversions, unpacking) and a quarter of 1300 cycles of
-// LDS traffic: none alone bounds it, so the loop runs them beside each other:
-// the next tile is unpacked between the score products, and the weights of 16
-// keys are made between the value products of the 16 before.  8192 tokens, 16
-// heads on 8, no prior keys: 269 us, 1.02 PFLOP/s of visible pairs (a large
-// library product reaches 1.40; 331 us with the scores of the next tile beside
-// the softmax of this one instead, 281 us with neither); 2 x 4096 tokens 143
-// us; 8 x 128 behind 4096 keys 48 us, of which the tile loop is 33.
+// LDS traffic: none alone bounds it, so the loop mixes them: the next tile is
+// unpacked between the score products, and the weights of 16 keys are made
+// between the value products of the 16 before.  By the counters the matrix pipe
+// works for 0.445 and the vector unit for 0.50 of the SIMDs' cycles, 0.95
+// together: mostly one of them at a time still.  8192 tokens, 16 heads on 8, no
+// prior keys: 269-274 us, 1.0 PFLOP/s of visible pairs (a large library product
+// reaches 1.40; 331 us with the scores of the next tile beside the softmax of
+// this one instead, 281 us with neither); 2 x 4096 tokens 142-146 us; 8 x 128
+// behind up to 4096 keys 48 us, of which the tile loop is 33.  (Calls back to
+// back.)
 #include <algorithm>
 #include <cmath>
 
@@ -91,7 +94,8 @@ __device__ inline void store4(const PrefillArgs& a, int64_t head, int d, f32x4 v
     *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + head * D + d) = w;
 }
 
-// Rows before the first and behind the last sequence: zeros.
+// Rows before the first and behind the last sequence: zeros.  Meant for few of them: one work-group per kv head, two bytes
+// at a time (3072 behind 1024 live ones, 16 heads of 128: the call takes 563 us instead of 31).
 template <int D>
 __device__ void clear_rows(const PrefillArgs& a, int kv_head) {
     const int64_t first = min(max(a.cu[0], (int64_t)0), a.total_tokens);
@@ -495,7 +499,9 @@ struct Plan {
 // compute unit to itself takes a tile in 1.00, 1.15, 1.45, 1.5, 2.5 and 3.1 us at 32, 64, 96, 128, 192 and 256 dims, two
 // on one unit in 1.4 times as long each; from 192 dims on LDS holds one.  Joining takes a launch and its traffic.
 // 8 x 128 tokens behind 4096 keys (128 dims): 48 us in four pieces, 99 us whole, 67 us in sixteen; two sequences of 2048
-// tokens (256 dims): 239 us whole, 363 us in pieces of 768.
+// tokens (256 dims): 239 us whole, 363 us in pieces of 768.  Chunks are shares of the table's capacity, since the lengths
+// stay on the device: in wider tables the same keys fall into fewer of them (8 x 128 in tables of 4096 tokens 48 us, 8192
+// 68, 16384 and more 117: all in the first).
 constexpr double kCus = 256, kMerge = 4, kMergeRate = 8e6;
 double tile_time(int64_t head_dim, double fill) {  // fill: work-groups per compute unit
     const double alone = head_dim <= 128 ? 0.85 + (double)head_dim / 200 : 0.65 + (double)head_dim / 105;

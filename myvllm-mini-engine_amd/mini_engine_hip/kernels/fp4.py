@@ -337,8 +337,11 @@ def paged_prefill_attention_fp4(q, key_cache, value_cache, cu_seqlens_q, query_s
     are read from the cache, so they are written first.  Rows that see no key
     and rows behind the last sequence are zeros.  A NaN block, of a value too,
     makes the rows that see its key NaN in all dims (decode keeps a value's to
-    its 32).  ``validate=False`` reads no metadata on the host.  ``chunk_tokens`` (0 = library plan) splits keys over
-    work-groups; ``workspace`` may supply the buffer for it.
+    its 32).  ``validate=False`` reads no metadata on the host.
+    ``chunk_tokens`` (0 = library plan) splits keys over work-groups;
+    ``workspace`` may supply the buffer for it.  The plan goes by the width of
+    ``block_tables``: pass them as wide as the longest context needs, and few
+    rows behind the last sequence (clearing them is slow).
     """
     _backend(backend, "prefill")
     if not validate and workspace is None:
