@@ -95,7 +95,7 @@ __device__ inline void store4(const PrefillArgs& a, int64_t head, int d, f32x4 v
 }
 
 // Rows before the first and behind the last sequence: zeros.  Meant for few of them: one work-group per kv head, two bytes
-// at a time (3072 behind 1024 live ones, 16 heads of 128: the call takes 563 us instead of 31).
+// at a time (1024 rows, 16 heads of 128: 31 us; padded to 4096 rows: 563 us).
 template <int D>
 __device__ void clear_rows(const PrefillArgs& a, int kv_head) {
     const int64_t first = min(max(a.cu[0], (int64_t)0), a.total_tokens);
