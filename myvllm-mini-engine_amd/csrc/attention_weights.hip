@@ -1,0 +1,182 @@
+// Decode attention that adds the weight each cached token receives to an
+// account: the narrow units of the shared-prefix walk, with their dot products
+// kept in a workspace until the divisor is known.
+#include "../../include/mvme_long.h"
+#include "long_attention.h"
+
+namespace mvme {
+namespace lng {
+namespace {
+
+template <typename T, int D, int RUN>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weighted_decode_kernel(Args a) {
+    __shared__ __attribute__((aligned(16))) NarrowLds<D> lds;
+    Walk w;
+    w.count(a);
+    const int all = w.total * a.kv_heads;
+    const int first = (int)min((int64_t)blockIdx.x * w.share, (int64_t)all);
+    const int stop = (int)min((int64_t)first + w.share, (int64_t)all);
+#pragma unroll 1
+    for (int at = first; at < stop;) {
+        const Segment s = find_segment(a, w, at, stop);
+        at += s.rounds;
+        narrow_segment<T, D, RUN, true>(a, s, lds);
+    }
+}
+
+constexpr int kAddKeys = 4 * kThreads;  // keys whose weights a work-group adds up
+
+// Joins the pieces, and adds weights: work-groups 0 .. batch * kv_heads - 1 do the first, the others take kAddKeys keys of
+// one sequence and kv head each.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void weighted_join_kernel(Args a, int blocks) {
+    const int units = a.batch * a.kv_heads;
+    if ((int)blockIdx.x < units) {
+        join_heads<T, D>(a, blockIdx.x / a.kv_heads, blockIdx.x % a.kv_heads);
+        return;
+    }
+    const int item = blockIdx.x - units, block = item % blocks, unit = item / blocks;
+    const int seq = unit / a.kv_heads, kv_head = unit % a.kv_heads;
+    const int len = Walk::length(a, seq);
+    if (block * kAddKeys >= len) return;
+    __shared__ float stats[kThreads][2];  // (reference, 1 / sum) of the heads at hand
+    Join j;
+    j.find(a, seq, kv_head);
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t head0 = (int64_t)seq * a.q_heads + kv_head * a.group;
+    float* out = a.weights + ((int64_t)seq * a.kv_heads + kv_head) * a.weight_row;
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
+    const int key = block * kAddKeys + threadIdx.x;
+    for (int h0 = 0; h0 < a.group; h0 += kThreads) {
+        const int heads = min(a.group - h0, kThreads);
+        __syncthreads();
+        for (int h = wave; h < heads; h += kWaves) {
+            Pieces p;
+            float ref = kRefNone, sum = 0.f;
+            if (j.pieces(a, h0 + h, p)) {
+                for (int i = lane; i < p.count; i += kWave) {
+                    const float* s;
+                    p.at(a, i, D, s);
+                    const float top = fmaxf(ref, s[0]);
+                    sum = sum * fast_exp2(ref - top) + s[1] * fast_exp2(s[0] - top);
+                    ref = top;
+                }
+                float top = ref;
+#pragma unroll
+                for (int m = 1; m < kWave; m *= 2) top = fmaxf(top, shfl_xor(top, m));
+                sum = group_sum<kWave>(sum * fast_exp2(ref - top));
+                ref = top;
+            } else {
+                ref = a.totals[(head0 + h0 + h) * 2];
+                sum = a.totals[(head0 + h0 + h) * 2 + 1];
+            }
+            if (lane == 0) {
+                stats[h][0] = ref;
+                stats[h][1] = sum != 0.f ? 1.f / sum : 0.f;
+            }
+        }
+        __syncthreads();
+        for (int h = 0; h < heads; ++h) {
+            const float ref = stats[h][0], by = stats[h][1];
+            const float* s = a.scores + (head0 + h0 + h) * a.score_row;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (key + i * kThreads < len)
+                    add[i] += fast_exp2(__builtin_fmaf(s[key + i * kThreads], a.scale, -ref)) * by;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (key + i * kThreads < len) out[key + i * kThreads] += add[i];
+}
+
+int work_groups(int64_t head_dim) { return head_dim <= 128 ? 512 : 256; }
+
+struct Sizes {
+    int64_t shares, slots, score_row;
+    int64_t floats;  // or -1: too many
+};
+Sizes sizes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t block_size, int64_t width) {
+    Sizes s{};
+    s.shares = work_groups(head_dim);
+    s.slots = kv_heads * batch * ((q_heads / kv_heads - 1) / kColumns + 1) + s.shares;
+    s.score_row = (block_size * width + 31) / 32 * 32;
+    s.floats = s.slots * kColumns * (head_dim + 2) + batch * q_heads * (2 + s.score_row) + 4;
+    return s;
+}
+
+template <typename T, int D>
+int launch(const Args& a, int blocks, hipStream_t s) {
+    const dim3 grid((unsigned)a.shares), block(kThreads);
+    if (a.div.size % 16 == 0) hipLaunchKernelGGL((weighted_decode_kernel<T, D, 16>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((weighted_decode_kernel<T, D, 1>), grid, block, 0, s, a);
+    if (int rc = check_launch("weighted attention")) return rc;
+    hipLaunchKernelGGL((weighted_join_kernel<T, D>), dim3((unsigned)(a.batch * a.kv_heads * (1 + blocks))), block, 0, s, a, blocks);
+    return check_launch("weighted join");
+}
+
+template <typename T>
+int launch_dim(const Args& a, int64_t head_dim, int blocks, hipStream_t s) {
+    switch (head_dim) {
+        case 16: return launch<T, 16>(a, blocks, s);
+        case 32: return launch<T, 32>(a, blocks, s);
+        case 64: return launch<T, 64>(a, blocks, s);
+        case 80: return launch<T, 80>(a, blocks, s);
+        case 96: return launch<T, 96>(a, blocks, s);
+        case 128: return launch<T, 128>(a, blocks, s);
+        case 192: return launch<T, 192>(a, blocks, s);
+        default: return launch<T, 256>(a, blocks, s);
+    }
+}
+
+}  // namespace
+}  // namespace lng
+}  // namespace mvme
+
+using namespace mvme;
+using namespace mvme::lng;
+
+extern "C" size_t mvme_paged_attention_weights_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                              int64_t head_dim, int64_t block_size, int64_t table_width) {
+    Args a{};
+    if (check_shape(a, batch, q_heads, kv_heads, head_dim, 1, block_size, table_width, MVME_FP16)) return 0;
+    return (size_t)sizes(batch, q_heads, kv_heads, head_dim, block_size, table_width).floats * sizeof(float);
+}
+
+extern "C" int mvme_paged_attention_weights(void* out, const void* query, const void* key_cache, const void* value_cache,
+                                            const int64_t* block_tables, const int64_t* context_lens, float* weights,
+                                            int64_t weight_row, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                            int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                                            int64_t table_width, int dtype, void* workspace, size_t workspace_bytes,
+                                            void* stream) {
+    Args a{};
+    if (int rc = check_shape(a, batch, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, dtype)) return rc;
+    if (weight_row < block_size * table_width) return fail(MVME_EINVAL, "weight rows must hold the tables' capacity");
+    if (!out || !query || !key_cache || !value_cache || !block_tables || !context_lens || !weights)
+        return fail(MVME_EINVAL, "weighted attention: null pointer");
+    if (!fp4::aligned(query, 16) || !fp4::aligned(key_cache, 16) || !fp4::aligned(value_cache, 16) || !fp4::aligned(out, 8) ||
+        !fp4::aligned(weights, 4))
+        return fail(MVME_EINVAL, "weighted attention: queries and caches must be 16-byte, the output 8-byte aligned");
+    const Sizes s = sizes(batch, q_heads, kv_heads, head_dim, block_size, table_width);
+    const int64_t blocks = (block_size * table_width - 1) / kAddKeys + 1;
+    if (batch * kv_heads > kMostThreads / kThreads / (1 + blocks)) return fail(MVME_EINVAL, "batch/head product too large");
+    if (!workspace || workspace_bytes < (size_t)s.floats * sizeof(float) || !fp4::aligned(workspace, 16))
+        return fail(MVME_EWORKSPACE, "weighted attention workspace too small: " + std::to_string(s.floats * 4) +
+                                         " bytes, 16-byte aligned, are needed");
+    a.out = out;
+    a.query = query;
+    a.key = static_cast<const uint8_t*>(key_cache);
+    a.value = static_cast<const uint8_t*>(value_cache);
+    a.tables = block_tables;
+    a.lens = context_lens;
+    a.shares = (int)s.shares;
+    a.narrow_slots = s.slots;
+    a.weights = weights;
+    a.weight_row = weight_row;
+    a.score_row = s.score_row;
+    a.scores = static_cast<float*>(workspace);
+    a.narrow = a.scores + batch * q_heads * s.score_row;
+    a.totals = a.narrow + s.slots * kColumns * (head_dim + 2);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return dtype == MVME_FP16 ? launch_dim<Half>(a, head_dim, (int)blocks, st) : launch_dim<BFloat16>(a, head_dim, (int)blocks, st);
+}

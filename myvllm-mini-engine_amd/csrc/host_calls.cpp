@@ -22,6 +22,7 @@
 #include <cstring>
 
 #include "mvme_fp4.h"
+#include "mvme_long.h"
 #include "mvme_paged.h"
 
 namespace {
@@ -49,6 +50,13 @@ struct Library {
     decltype(&mvme_fp4_paged_prefill_attention) fp4_prefill;
     decltype(&mvme_copy_pages) copy_pages;
     decltype(&mvme_compact_pages) compact_pages;
+    decltype(&mvme_paged_attention_shared_prefix_workspace_size) shared_workspace;
+    decltype(&mvme_paged_attention_shared_prefix) shared_prefix;
+    decltype(&mvme_paged_attention_weights_workspace_size) weights_workspace;
+    decltype(&mvme_paged_attention_weights) decode_weights;
+    decltype(&mvme_prefill_attention_weights_workspace_size) prefill_weights_workspace;
+    decltype(&mvme_prefill_attention_weights) prefill_weights;
+    decltype(&mvme_evict_kv_cache) evict;
 } lib;
 PyObject* current_raw_stream = nullptr;  // torch's getter: device index -> hipStream_t
 
@@ -658,6 +666,188 @@ PyObject* move_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// Operators for long contexts.
+// ---------------------------------------------------------------------------
+// Whether the memory of two contiguous tensors meets.
+bool meet(const at::Tensor& a, const at::Tensor& b) {
+    const auto begin = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+    const auto end = [&](const at::Tensor& t) { return begin(t) + t.numel() * t.element_size(); };
+    return a.numel() > 0 && b.numel() > 0 && begin(a) < end(b) && begin(b) < end(a);
+}
+
+// fp32 [lines..., at least `capacity`], beside a tensor.
+bool weight_rows(const at::Tensor& w, const at::Tensor& beside, int64_t capacity) {
+    return w.scalar_type() == at::kFloat && w.is_contiguous() && w.device() == beside.device() &&
+           w.size(w.dim() - 1) >= capacity;
+}
+
+// A decode call's plain arguments whose caches the operators of this part take.
+bool long_decode(const at::Tensor* const* t, int64_t block, DecodeShape& s) {
+    return eager() && on_current_device(*t[0]) && decode_shape(*t[0], *t[1], *t[2], *t[3], *t[4], block, s) &&
+           t[0]->is_contiguous() && aligned16(*t[0]) && aligned16(*t[1]) && aligned16(*t[2]);
+}
+
+// shared_prefix(query, key_cache, value_cache, block_tables, context_lens, block_size, group_offsets, prefix_lens)
+PyObject* shared_prefix(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0;
+    if (n != 8 || !as_int(args[5], block)) Py_RETURN_NONE;
+    const at::Tensor* t[8] = {};
+    for (int i = 0; i < 8; ++i)
+        if (i != 5 && !(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &q = *t[0], &offsets = *t[6], &prefixes = *t[7];
+    DecodeShape s;
+    if (!long_decode(t, block, s)) Py_RETURN_NONE;
+    if (offsets.dim() != 1 || prefixes.dim() != 1 || offsets.size(0) != prefixes.size(0) + 1 || prefixes.size(0) > s.batch ||
+        !index_list(offsets, q) || !index_list(prefixes, q))
+        Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(q, stream)) return nullptr;
+    at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+    const int64_t groups = prefixes.size(0);
+    const size_t need = lib.shared_workspace(s.batch, s.q_heads, s.kv_heads, s.head_dim, groups);
+    at::Tensor workspace = bytes_like(q, need);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.shared_prefix(out.data_ptr(), q.data_ptr(), t[1]->data_ptr(), t[2]->data_ptr(), indices(*t[3]),
+                               indices(*t[4]), indices(offsets), indices(prefixes), s.batch, groups, s.q_heads, s.kv_heads,
+                               s.head_dim, s.num_blocks, block, s.width, dtype_code(q), workspace.data_ptr(), need, stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_paged_attention_shared_prefix", status);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// decode_weights(query, key_cache, value_cache, block_tables, context_lens, block_size, weights)
+PyObject* decode_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0;
+    if (n != 7 || !as_int(args[5], block)) Py_RETURN_NONE;
+    const at::Tensor* t[7] = {};
+    for (int i = 0; i < 7; ++i)
+        if (i != 5 && !(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &q = *t[0], &w = *t[6];
+    DecodeShape s;
+    if (!long_decode(t, block, s)) Py_RETURN_NONE;
+    if (w.dim() != 3 || w.size(0) != s.batch || w.size(1) != s.kv_heads || !weight_rows(w, q, s.width * block)) Py_RETURN_NONE;
+    for (int i = 0; i < 5; ++i)
+        if (meet(w, *t[i])) Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(q, stream)) return nullptr;
+    at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+    const size_t need = lib.weights_workspace(s.batch, s.q_heads, s.kv_heads, s.head_dim, block, s.width);
+    at::Tensor workspace = bytes_like(q, need);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.decode_weights(out.data_ptr(), q.data_ptr(), t[1]->data_ptr(), t[2]->data_ptr(), indices(*t[3]),
+                                indices(*t[4]), static_cast<float*>(w.data_ptr()), w.size(2), s.batch, s.q_heads,
+                                s.kv_heads, s.head_dim, s.num_blocks, block, s.width, dtype_code(q), workspace.data_ptr(),
+                                need, stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_paged_attention_weights", status);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// prefill_weights(q, key_cache, cu_seqlens_q, query_starts, block_tables, context_lens, block_size, weights): True when
+// the weights were added.
+PyObject* prefill_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0;
+    if (n != 8 || !as_int(args[6], block)) Py_RETURN_NONE;
+    const at::Tensor* t[8] = {};
+    for (int i = 0; i < 8; ++i)
+        if (i != 6 && !(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    const at::Tensor &q = *t[0], &k = *t[1], &cu = *t[2], &starts = *t[3], &tables = *t[4], &lens = *t[5], &w = *t[7];
+    if (!eager() || !on_current_device(q) || q.dim() != 3 || !half_type(q) || !q.is_contiguous() || q.numel() <= 0 ||
+        !aligned16(q) || k.dim() != 4 || k.numel() <= 0 || k.device() != q.device() || k.scalar_type() != q.scalar_type() ||
+        !k.is_contiguous() || !aligned16(k) || block <= 0 || block > kMaxCapacity || k.size(1) != block)
+        Py_RETURN_NONE;
+    const int64_t tokens = q.size(0), q_heads = q.size(1), d = q.size(2), kv_heads = k.size(2);
+    if (k.size(3) != d || q_heads % kv_heads != 0) Py_RETURN_NONE;
+    switch (d) {
+        case 16: case 32: case 64: case 80: case 96: case 128: case 192: case 256: break;
+        default: Py_RETURN_NONE;
+    }
+    if (cu.dim() != 1 || starts.dim() != 1 || lens.dim() != 1 || tables.dim() != 2) Py_RETURN_NONE;
+    const int64_t seqs = starts.size(0), width = tables.size(1);
+    if (seqs <= 0 || tables.size(0) != seqs || lens.size(0) != seqs || cu.size(0) != seqs + 1 || width <= 0 ||
+        width > kMaxCapacity / block)
+        Py_RETURN_NONE;
+    for (int i = 2; i < 6; ++i)
+        if (!index_list(*t[i], q)) Py_RETURN_NONE;
+    if (w.dim() != 3 || w.size(0) != seqs || w.size(1) != kv_heads || !weight_rows(w, q, width * block)) Py_RETURN_NONE;
+    for (int i = 0; i < 6; ++i)
+        if (meet(w, *t[i])) Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(q, stream)) return nullptr;
+    const size_t need = lib.prefill_weights_workspace(seqs, tokens, q_heads, kv_heads, d, block, width);
+    at::Tensor workspace = bytes_like(q, need);
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.prefill_weights(q.data_ptr(), k.data_ptr(), indices(cu), indices(starts), indices(tables), indices(lens),
+                                 static_cast<float*>(w.data_ptr()), w.size(2), seqs, tokens, q_heads, kv_heads, d,
+                                 k.size(0), block, width, dtype_code(q), workspace.data_ptr(), need, stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_prefill_attention_weights", status);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// evict(key_cache, value_cache, weights, block_tables, context_lens, block_size, keep, first or None, recent): the three
+// new tensors.
+PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    int64_t block = 0, keep = 0, recent = 0;
+    if (n != 9 || !as_int(args[5], block) || !as_int(args[6], keep) || !as_int(args[8], recent)) Py_RETURN_NONE;
+    const at::Tensor* t[6] = {};
+    for (int i = 0; i < 5; ++i)
+        if (!(t[i] = plain(args[i]))) Py_RETURN_NONE;
+    if (args[7] != Py_None && !(t[5] = plain(args[7]))) Py_RETURN_NONE;
+    const at::Tensor &k = *t[0], &v = *t[1], &w = *t[2], &tables = *t[3], &lens = *t[4];
+    if (!eager() || !on_current_device(k) || (k.dim() != 4 && k.dim() != 5) || v.sizes() != k.sizes() || k.numel() <= 0 ||
+        !half_type(k) || v.scalar_type() != k.scalar_type() || v.device() != k.device() || !k.is_contiguous() ||
+        !v.is_contiguous() || !aligned16(k) || !aligned16(v))
+        Py_RETURN_NONE;
+    const int64_t lead = k.dim() - 4, layers = lead ? k.size(0) : 1;
+    const int64_t kv_heads = k.size(lead + 2), d = k.size(lead + 3);
+    if (block <= 0 || block > kMaxCapacity || k.size(lead + 1) != block || d % 8 != 0 || d > 1024 || keep <= 0 || recent < 0)
+        Py_RETURN_NONE;
+    if (tables.dim() != 2 || lens.dim() != 1 || tables.size(0) <= 0 || tables.size(1) <= 0 || lens.size(0) != tables.size(0) ||
+        tables.size(1) > kMaxCapacity / block || !index_list(tables, k) || !index_list(lens, k))
+        Py_RETURN_NONE;
+    const int64_t batch = tables.size(0), width = tables.size(1);
+    if (t[5] && (t[5]->dim() != 1 || t[5]->size(0) != batch || !index_list(*t[5], k))) Py_RETURN_NONE;
+    if (w.dim() != lead + 3 || (lead && w.size(0) != layers) || w.size(lead) != batch || w.size(lead + 1) != kv_heads ||
+        !weight_rows(w, k, width * block) || meet(k, v))
+        Py_RETURN_NONE;
+    for (int i = 2; i < 6; ++i)
+        if (t[i] && (meet(k, *t[i]) || meet(v, *t[i]))) Py_RETURN_NONE;
+    void* stream = nullptr;
+    if (!stream_of(k, stream)) return nullptr;
+    const int64_t row = w.size(lead + 2), columns = keep < row ? keep : row;
+    auto shape = w.sizes().vec();
+    shape.back() = columns;
+    at::Tensor kept = at::empty(shape, lens.options()), new_lens = at::empty(lens.sizes(), lens.options());
+    at::Tensor new_weights = at::empty(w.sizes(), w.options().requires_grad(false));
+    int status;
+    Py_BEGIN_ALLOW_THREADS
+    status = lib.evict(k.data_ptr(), v.data_ptr(), static_cast<const float*>(w.data_ptr()),
+                       static_cast<float*>(new_weights.data_ptr()), row, static_cast<int64_t*>(kept.data_ptr()),
+                       static_cast<int64_t*>(new_lens.data_ptr()), indices(tables), indices(lens),
+                       t[5] ? indices(*t[5]) : nullptr, layers, batch, kv_heads, d, k.size(lead), block, width, columns,
+                       recent, dtype_code(k), stream);
+    Py_END_ALLOW_THREADS
+    if (status != MVME_OK) return raise_status("mvme_evict_kv_cache", status);
+    PyObject* made[3] = {THPVariable_Wrap(std::move(kept)), THPVariable_Wrap(std::move(new_lens)),
+                         THPVariable_Wrap(std::move(new_weights))};
+    PyObject* all = made[0] && made[1] && made[2] ? PyTuple_Pack(3, made[0], made[1], made[2]) : nullptr;
+    for (PyObject* o : made) Py_XDECREF(o);
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(raw_stream_getter, (address, ...)): the library's entry points in the order of Library.
 PyObject* bind(PyObject*, PyObject* args) {
     PyObject *getter = nullptr, *addresses = nullptr;
@@ -698,6 +888,10 @@ PyMethodDef methods[] = {
     {"fp4_write_batch", reinterpret_cast<PyCFunction>(fp4_write_batch), METH_FASTCALL, nullptr},
     {"fp4_gather_slots", reinterpret_cast<PyCFunction>(fp4_gather_slots), METH_FASTCALL, nullptr},
     {"move_pages", reinterpret_cast<PyCFunction>(move_pages), METH_FASTCALL, nullptr},
+    {"shared_prefix", reinterpret_cast<PyCFunction>(shared_prefix), METH_FASTCALL, nullptr},
+    {"decode_weights", reinterpret_cast<PyCFunction>(decode_weights), METH_FASTCALL, nullptr},
+    {"prefill_weights", reinterpret_cast<PyCFunction>(prefill_weights), METH_FASTCALL, nullptr},
+    {"evict", reinterpret_cast<PyCFunction>(evict), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

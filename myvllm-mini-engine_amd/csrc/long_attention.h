@@ -1,0 +1,691 @@
+// Decode attention over 16-bit pages whose prefixes may be shared, and whose
+// weights may be kept: the walk that hands out the work, and the two kinds of
+// tiles.  Matrix tiles and the softmax's reference are those of
+// fp4_attention.h.
+//
+// A unit is what has the same keys: the rows of one group (its sequences'
+// query heads of one kv head) over the group's prefix, or one sequence's query
+// heads of one kv head over its own keys.  All units are laid end to end and
+// cut into equal shares (in rounds of 128 keys), one per work-group; a second
+// kernel joins the pieces.  Groups of more than kNarrowRows rows are taken 128
+// rows at a time (wide: a wave has 32 rows, tiles of keys and values in LDS
+// serve all four waves), everything else 16 rows at a time (narrow: the waves
+// take tiles of 32 keys in turn).
+#pragma once
+
+#include <algorithm>
+
+#include "fp4_attention.h"
+
+namespace mvme {
+namespace lng {
+
+using fp4::BlockDiv;
+using fp4::kRefBelow;
+using fp4::kRefNone;
+using fp4::kRefSlack;
+using fp4::kTileKeys;
+using fp4::TileAddress;
+using fp4::uniform_load;
+using fp4::value_operand;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kRound = 128;       // keys of a round: a narrow tile for every wave, or two wide tiles
+constexpr int kWideRows = 128;    // rows of a wide unit
+constexpr int kWideKeys = 64;     // keys of a wide tile
+constexpr int kNarrowRows = 32;   // a group with more rows is wide
+constexpr int kColumns = 16;      // rows of a narrow unit
+constexpr int64_t kMaxCapacity = fp4::kMaxCapacity;
+
+struct Args {
+    void* out;
+    const void* query;
+    const uint8_t* key;
+    const uint8_t* value;
+    const int64_t* tables;
+    const int64_t* lens;
+    const int64_t* offsets;   // [groups + 1]; rows of a group
+    const int64_t* prefixes;  // [groups]; tokens that they share
+    float* wide;              // [wide slots, 128, D] sums, then [wide slots, 128, 2] (reference, sum)
+    float* narrow;            // [narrow slots, 16, D], then [narrow slots, 16, 2]
+    float* totals;            // [batch, q_heads, 2]: (reference, sum) of units that one share holds (scores only)
+    float* scores;            // [batch, q_heads, capacity] dot products (scores only)
+    float* weights;           // [batch, kv_heads, weight_row]
+    int64_t weight_row, score_row;  // (score rows are a multiple of 32 long)
+    int64_t wide_slots, narrow_slots;
+    int64_t num_blocks;
+    uint64_t page_bytes;
+    uint32_t row_bytes;       // of a token: kv_heads * D * 2
+    int batch, groups, kv_heads, group, q_heads, width;
+    int head_tiles;           // ceil(group / 16)
+    int shares;               // work-groups of the walk
+    BlockDiv div, group_div;
+    float scale;              // log2(e) / sqrt(D)
+};
+
+template <int D>
+struct Shape {
+    static constexpr int kDim = (D + 31) / 32 * 32;      // padded with zeros
+    static constexpr int kChunks = kDim / 32;            // 16-byte pieces of a lane's part of a token
+    static constexpr int kDimTiles = kDim / 16;
+    static constexpr int kTileBytes = kTileKeys * 2 * kDim;  // a narrow tile's values; as large as its 16 rows of sums
+    static constexpr int kBlocks = kDim / 32;            // 32-dim blocks of a wide unit's sums
+    static constexpr int kSteps = kDim / 16;
+    static constexpr int kWidePlane = kWideKeys * 2 * kDim;
+};
+
+__device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// ---------------------------------------------------------------------------
+// The walk.  Every wave computes the same, lane-parallel over the groups or sequences.  Order: kv heads; of each the wide
+// units, the narrow units of groups, the sequences' units.
+// ---------------------------------------------------------------------------
+struct Group {
+    int first, rows;     // sequences
+    int prefix;          // tokens; 0: nothing is shared
+    bool wide;
+    int rounds, tiles;   // of a unit, and units
+};
+
+struct Walk {
+    bool grouped;                     // the offsets can be
+    int wide_units, narrow_units;     // of a kv head, of groups
+    int wide_rounds, narrow_rounds;   // the same in rounds
+    int total;                        // rounds of a kv head
+    int share;
+
+    __device__ static inline int64_t capacity(const Args& a) { return (int64_t)a.width * a.div.size; }
+
+    __device__ inline Group group(const Args& a, int g) const {
+        Group x{0, 0, 0, false, 0, 0};
+        if (!grouped || g >= a.groups) return x;
+        x.first = (int)a.offsets[g];
+        x.rows = (int)a.offsets[g + 1] - x.first;
+        const int64_t prefix = a.prefixes[g];
+        // (One row alone gains nothing, and needs no unit for it.)
+        x.prefix = x.rows >= 2 && prefix > 0 && prefix <= capacity(a) ? (int)prefix : 0;
+        const int64_t rows = (int64_t)x.rows * a.group;
+        x.wide = rows > kNarrowRows;
+        x.rounds = (x.prefix + kRound - 1) / kRound;
+        x.tiles = x.prefix ? (int)(x.wide ? (rows + kWideRows - 1) / kWideRows : (rows + kColumns - 1) / kColumns) : 0;
+        return x;
+    }
+    // Tokens of a sequence; 0 where the length cannot be.
+    __device__ static inline int length(const Args& a, int seq) {
+        const int64_t n = seq < a.batch ? a.lens[seq] : 0;
+        return n > 0 && n <= capacity(a) ? (int)n : 0;
+    }
+    // The group that a sequence is in, or -1.
+    __device__ inline int group_of(const Args& a, int seq) const {
+        if (!grouped) return -1;
+        int low = 0, high = a.groups;  // the last offset that is not above seq
+        while (high - low > 1) {
+            const int mid = (low + high) >> 1;
+            if (a.offsets[mid] <= seq) low = mid;
+            else high = mid;
+        }
+        return a.offsets[low] <= seq && seq < a.offsets[low + 1] ? low : -1;
+    }
+    // Where a sequence's own keys begin: behind its group's prefix, if it reaches to the end of that.
+    __device__ inline int start(const Args& a, int seq, int len, int* group_index = nullptr) const {
+        const int g = seq < a.batch ? group_of(a, seq) : -1;
+        if (group_index) *group_index = g;
+        if (g < 0) return 0;
+        const int prefix = group(a, g).prefix;
+        return prefix <= len ? prefix : 0;
+    }
+    __device__ inline int own_rounds(const Args& a, int seq) const {
+        const int n = length(a, seq);
+        return (n - start(a, seq, n) + kRound - 1) / kRound;
+    }
+
+    __device__ inline void count(const Args& a) {
+        const int lane = __lane_id();
+        wide_units = narrow_units = wide_rounds = narrow_rounds = total = 0;
+        grouped = a.groups > 0;
+        if (grouped) {
+            bool good = a.offsets[0] >= 0 && a.offsets[a.groups] <= a.batch;
+            for (int g0 = 0; g0 < a.groups; g0 += kWave)
+                if (g0 + lane < a.groups) good = good && a.offsets[g0 + lane] <= a.offsets[g0 + lane + 1];
+            grouped = __all(good);
+        }
+        if (grouped)
+            for (int g0 = 0; g0 < a.groups; g0 += kWave) {
+                const Group x = group(a, g0 + lane);
+                const int w = x.wide ? x.tiles : 0, n = x.wide ? 0 : x.tiles;
+                wide_units += lane_value(wave_incl_scan(w), kWave - 1);
+                narrow_units += lane_value(wave_incl_scan(n), kWave - 1);
+                wide_rounds += lane_value(wave_incl_scan(w * x.rounds), kWave - 1);
+                narrow_rounds += lane_value(wave_incl_scan(n * x.rounds), kWave - 1);
+            }
+        int own = 0;
+        for (int s0 = 0; s0 < a.batch; s0 += kWave) own += lane_value(wave_incl_scan(own_rounds(a, s0 + lane)), kWave - 1);
+        total = wide_rounds + narrow_rounds + own * a.head_tiles;
+        const int all = total * a.kv_heads;
+        // Two rounds at least, where that gives every CU one share: more pieces cost the join more than they save.
+        share = max(max((all + a.shares - 1) / a.shares, min((all + 255) / 256, 2)), 1);
+    }
+
+    // Unit `tile` of `group` begins at round `base` of its kv head and is number `unit` among its kind.
+    __device__ inline void place_of_group(const Args& a, int g, int& base, int& unit) const {
+        const int lane = __lane_id();
+        base = unit = 0;
+        const bool wide = group(a, g).wide;
+        for (int g0 = 0; g0 < g; g0 += kWave) {
+            const Group x = group(a, g0 + lane);
+            const bool counts = g0 + lane < g && x.wide == wide;
+            base += lane_value(wave_incl_scan(counts ? x.tiles * x.rounds : 0), kWave - 1);
+            unit += lane_value(wave_incl_scan(counts ? x.tiles : 0), kWave - 1);
+        }
+        if (!wide) base += wide_rounds;
+    }
+    // First round, in its kv head, of a sequence's own units.
+    __device__ inline int place_of_sequence(const Args& a, int seq) const {
+        const int lane = __lane_id();
+        int base = 0;
+        for (int s0 = 0; s0 < seq; s0 += kWave)
+            base += lane_value(wave_incl_scan(s0 + lane < seq ? own_rounds(a, s0 + lane) : 0), kWave - 1);
+        return wide_rounds + narrow_rounds + base * a.head_tiles;
+    }
+};
+
+// A run of rounds of one unit: what a work-group does at a time.  Wave-uniform.
+struct Segment {
+    int seq;              // whose pages
+    int kv_head, tile;
+    int first_row;        // of the group's sequences; -1: the sequence's own keys
+    int rows;             // live rows of the unit (wide, narrow)
+    uint32_t begin, end;  // keys
+    int slot;             // where its piece goes; -1: it is all that its rows have
+    int rounds;
+    bool wide;
+};
+
+__device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int stop) {
+    const int lane = __lane_id();
+    Segment s;
+    s.kv_head = at / w.total;
+    int q = at - s.kv_head * w.total;
+    const int wg = blockIdx.x;
+    int from, rounds, tokens, start = 0;
+    if (q < w.wide_rounds + w.narrow_rounds) {
+        s.wide = q < w.wide_rounds;
+        if (!s.wide) q -= w.wide_rounds;
+        int before = 0, units = 0, g = 0, base = 0, unit = 0;
+        for (int g0 = 0; g0 < a.groups; g0 += kWave) {
+            const Group x = w.group(a, g0 + lane);
+            const int tiles = x.wide == s.wide ? x.tiles : 0;
+            const int incl = before + wave_incl_scan(tiles * x.rounds), incl_units = units + wave_incl_scan(tiles);
+            const uint64_t hit = __ballot(incl > q);
+            if (hit) {
+                const int at_lane = __builtin_ctzll(hit);
+                g = g0 + at_lane;
+                base = lane_value(incl - tiles * x.rounds, at_lane);
+                unit = lane_value(incl_units - tiles, at_lane);
+                break;
+            }
+            before = lane_value(incl, kWave - 1);
+            units = lane_value(incl_units, kWave - 1);
+        }
+        const Group x = w.group(a, g);
+        rounds = max(x.rounds, 1);
+        s.tile = (q - base) / rounds;
+        from = q - base - s.tile * rounds;
+        tokens = x.prefix;
+        s.seq = x.first;
+        s.first_row = x.first;
+        s.rows = x.rows * a.group - s.tile * (s.wide ? kWideRows : kColumns);
+        unit += s.tile;
+        s.slot = (s.wide ? s.kv_head * w.wide_units + unit : s.kv_head * (w.narrow_units + a.batch * a.head_tiles) + unit) + wg;
+    } else {
+        q -= w.wide_rounds + w.narrow_rounds;
+        s.wide = false;
+        s.first_row = -1;
+        int before = 0, base = 0;
+        s.seq = 0;
+        for (int s0 = 0; s0 < a.batch; s0 += kWave) {
+            const int mine = w.own_rounds(a, s0 + lane) * a.head_tiles, incl = before + wave_incl_scan(mine);
+            const uint64_t hit = __ballot(incl > q);
+            if (hit) {
+                const int at_lane = __builtin_ctzll(hit);
+                s.seq = s0 + at_lane;
+                base = lane_value(incl - mine, at_lane);
+                break;
+            }
+            before = lane_value(incl, kWave - 1);
+        }
+        const int n = w.length(a, s.seq);
+        start = w.start(a, s.seq, n);
+        tokens = n - start;
+        rounds = max((tokens + kRound - 1) / kRound, 1);
+        s.tile = (q - base) / rounds;
+        from = q - base - s.tile * rounds;
+        s.rows = a.group - s.tile * kColumns;
+        s.slot = s.kv_head * (w.narrow_units + a.batch * a.head_tiles) + w.narrow_units + s.seq * a.head_tiles + s.tile + wg;
+    }
+    const int n = min(rounds - from, stop - at);
+    if (s.first_row < 0 && start == 0 && n == rounds) s.slot = -1;
+    s.begin = (uint32_t)(start + from * kRound);
+    s.end = (uint32_t)(start + min(tokens, (from + n) * kRound));
+    s.rounds = n;
+    // (Uniform all along, but only now provably so: what these address is loaded and computed once per wave.)
+    s.seq = uniform(s.seq);
+    s.kv_head = uniform(s.kv_head);
+    s.tile = uniform(s.tile);
+    s.first_row = uniform(s.first_row);
+    s.rows = uniform(s.rows);
+    s.begin = (uint32_t)uniform((int)s.begin);
+    s.end = (uint32_t)uniform((int)s.end);
+    s.slot = uniform(s.slot);
+    s.rounds = uniform(s.rounds);
+    s.wide = uniform(s.wide);
+    return s;
+}
+
+// Query head (of all) of a unit's row: rows of a group are its (sequence, head) pairs, sequence by sequence.
+__device__ inline int64_t head_of(const Args& a, const Segment& s, int row) {
+    if (s.first_row < 0) return (int64_t)s.seq * a.q_heads + s.kv_head * a.group + row;
+    const int seq = (int)a.group_div.page((uint32_t)row);
+    return (int64_t)(s.first_row + seq) * a.q_heads + s.kv_head * a.group + (row - seq * a.group);
+}
+
+// ---------------------------------------------------------------------------
+// Narrow tiles: 16 rows, 32 keys.  Lane (r, g) = (lane % 16, lane / 16) has token r of each half of the tile and the
+// dims of part g: keys are at once an operand of the score product, values go through LDS for the transposition.
+// ---------------------------------------------------------------------------
+// RUN tokens (block sizes that are multiples of it) lie in one page at consecutive places.
+struct Where {
+    int64_t at[2];     // byte offset of the half's first (RUN 1: the lane's) token in a plane; of one that exists
+    bool there[2];
+};
+
+template <int RUN>
+__device__ inline Where look_up(const Args& a, const int64_t* table, int64_t head_at, uint32_t first, uint32_t end, int r) {
+    Where w;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const uint32_t token = first + 16 * s + (RUN == 1 ? r : 0), block = a.div.page(token);
+        const int64_t* entry = table + min(block, (uint32_t)a.width - 1u);
+        int64_t page = RUN == 1 ? *entry : uniform_load(entry);
+        w.there[s] = token < end && (uint64_t)page < (uint64_t)a.num_blocks;
+        page = w.there[s] ? page : 0;
+        const uint32_t place = w.there[s] ? token - block * a.div.size : 0u;
+        w.at[s] = head_at + (int64_t)((uint64_t)(uint32_t)page * a.page_bytes) + (int64_t)((uint64_t)place * a.row_bytes);
+    }
+    return w;
+}
+
+// A lane's part of a token: pieces g * kChunks + c of 8 dims; zeros where the padded dims are.
+template <int D>
+__device__ inline void load_part(u32x4 (&x)[Shape<D>::kChunks], const uint8_t* at, int g) {
+#pragma unroll
+    for (int c = 0; c < Shape<D>::kChunks; ++c) {
+        if (D == Shape<D>::kDim || (g * Shape<D>::kChunks + c) * 8 < D) x[c] = *reinterpret_cast<const u32x4*>(at + 16 * c);
+        else x[c] = u32x4{0u, 0u, 0u, 0u};
+    }
+}
+
+// Two weights as sums of two numbers of the type each: the upper bits, and the rest rounded: at most 2^-15 (bf16) or 2^-21
+// (fp16) of the weight is lost.  The rest is positive, the type's smallest number at least (2^-32 of the largest weight),
+// so that an infinite value times a weight is infinite, as in the formula, and not NaN.
+template <typename T>
+__device__ inline u32x2 split_pair(float x, float y) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    constexpr uint16_t kLeast = T::kId == MVME_FP16 ? 0x0001 : 0x0080;
+    uint32_t high;
+    if constexpr (T::kId == MVME_FP16)
+        high = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+    else
+        high = __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+    const uint32_t rest = T::pack(x - T::lo(high), y - T::hi(high));
+    const u16x2 low = __builtin_elementwise_max(__builtin_bit_cast(u16x2, rest), u16x2{kLeast, kLeast});
+    return u32x2{high, __builtin_bit_cast(uint32_t, low)};
+}
+
+template <int D>
+struct NarrowLds {
+    uint8_t tiles[kWaves][Shape<D>::kTileBytes];
+    float stats[kWaves][2][kColumns];
+};
+
+// One segment of a narrow unit.  SCORES: its dot products are kept.
+template <typename T, int D, int RUN, bool SCORES>
+__device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowLds<D>& lds) {
+    using S = Shape<D>;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = uniform(threadIdx.x >> 6);
+    uint8_t* tile_lds = lds.tiles[wave];
+    TileAddress<S::kDim, 16> write_at(r, g * S::kChunks), read_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
+    uint32_t lane_at = (RUN == 1 ? 0u : (uint32_t)r * a.row_bytes) + (uint32_t)(g * S::kChunks * 16);
+    const int64_t* table = a.tables + (int64_t)seg.seq * a.width;
+    const int64_t head_at = (int64_t)seg.kv_head * (2 * D);
+    const int heads = min(kColumns, seg.rows);
+    const bool live = r < heads;
+    const int64_t head = head_of(a, seg, live ? seg.tile * kColumns + r : 0);
+
+    u32x4 q[S::kChunks], k[2][S::kChunks], v[2][S::kChunks];
+    f32x4 acc[S::kDimTiles];
+    float ref = kRefNone, sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < S::kDimTiles; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint32_t t0 = seg.begin + wave * kTileKeys;
+    Where now = look_up<RUN>(a, table, head_at, t0, seg.end, r);
+    if (t0 < seg.end) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) load_part<D>(k[s], a.key + now.at[s] + lane_at, g);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) load_part<D>(v[s], a.value + now.at[s] + lane_at, g);
+    }
+#pragma unroll
+    for (int c = 0; c < S::kChunks; ++c) q[c] = u32x4{0u, 0u, 0u, 0u};
+    if (live) load_part<D>(q, static_cast<const uint8_t*>(a.query) + head * (2 * D) + g * S::kChunks * 16, g);
+#pragma unroll 1
+    for (; t0 < seg.end; t0 += kRound) {
+        const bool more = t0 + kRound < seg.end;
+        write_at.forget();
+        read_at.forget();
+        asm volatile("" : "+v"(lane_at));
+        Where next = now;
+        if (more) next = look_up<RUN>(a, table, head_at, t0 + kRound, seg.end, r);
+        f32x4 x[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c) x[s] = T::mfma16x16x32(k[s][c], q[c], x[s]);
+        }
+        if (more)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) load_part<D>(k[s], a.key + next.at[s] + lane_at, g);
+        // Keys that are not there: no weight, and zeros as values (0 * NaN is NaN).
+        bool whole = t0 + kTileKeys <= seg.end && now.there[0] && now.there[1];
+        if constexpr (RUN == 1) whole = __all(whole);
+        if (!whole) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const bool mine = now.there[s] && t0 + 16 * s + r < seg.end;
+                const uint32_t present = (uint32_t)(__ballot(mine) & 0xffff) >> (4 * g);
+#pragma unroll
+                for (int c = 0; c < S::kChunks; ++c)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[s][c][j] = mine ? v[s][c][j] : 0u;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[s][j] = (present >> j) & 1 ? x[s][j] : kNegInf;
+            }
+        }
+        if constexpr (SCORES) {
+            // (Behind the context there is room up to the row's end: rows are a multiple of 32 long.)
+            if (live) {
+                float* to = a.scores + head * a.score_row + t0 + 4 * g;
+                *reinterpret_cast<f32x4*>(to) = x[0];
+                *reinterpret_cast<f32x4*>(to + 16) = x[1];
+            }
+        }
+        // Values to LDS, row-major.
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+                *reinterpret_cast<u32x4*>(tile_lds + write_at.chunk(c) + 16 * s * 2 * S::kDim) = v[s][c];
+        if (more)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) load_part<D>(v[s], a.value + next.at[s] + lane_at, g);
+        float top = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) top = fmaxf(top, fmaxf(x[0][j], x[1][j]));
+        top = row4_max(top) * a.scale;
+        if (__any(top > ref + kRefSlack)) {
+            const float moved = top > ref + kRefSlack ? top - kRefBelow : ref;
+            const float by = fast_exp2(ref - moved);
+            ref = moved;
+            sum *= by;
+#pragma unroll
+            for (int n = 0; n < S::kDimTiles; ++n) acc[n] *= by;
+        }
+        // A weight is the sum of two 16-bit numbers: the products are there anyhow, and the output's own rounding stays
+        // the only one that counts.
+        u32x4 high, low;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                const float p0 = fast_exp2(__builtin_fmaf(x[s][j], a.scale, -ref));
+                const float p1 = fast_exp2(__builtin_fmaf(x[s][j + 1], a.scale, -ref));
+                const u32x2 both = split_pair<T>(p0, p1);
+                high[2 * s + j / 2] = both[0];
+                low[2 * s + j / 2] = both[1];
+                sum += p0 + p1;
+            }
+        // A wave reads only what it wrote: the LDS queue is in order, no barrier.
+#pragma unroll
+        for (int n = 0; n < S::kDimTiles; ++n) {
+            const u32x4 vt = value_operand(tile_lds, read_at.chunk(2 * n), read_at.chunk(2 * n) + 16 * 2 * S::kDim);
+            acc[n] = T::mfma16x16x32(vt, high, acc[n]);
+            acc[n] = T::mfma16x16x32(vt, low, acc[n]);
+        }
+        now = next;
+    }
+    sum = row4_sum(sum);
+
+    // Join the waves: sums [16][D] in their tiles' LDS, each relative to its own reference.
+    float* mine = reinterpret_cast<float*>(tile_lds);
+    if (live) {
+#pragma unroll
+        for (int n = 0; n < S::kDimTiles; ++n) *reinterpret_cast<f32x4*>(mine + r * S::kDim + 16 * n + 4 * g) = acc[n];
+        if (g == 0) {
+            lds.stats[wave][0][r] = ref;
+            lds.stats[wave][1][r] = sum;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * D; i += kThreads) {
+        const int h = i / D, d = i - h * D;
+        float top = lds.stats[0][0][h];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) top = fmaxf(top, lds.stats[w][0][h]);
+        float total = 0.f, value = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float by = fast_exp2(lds.stats[w][0][h] - top);
+            total += by * lds.stats[w][1][h];
+            value += by * reinterpret_cast<const float*>(lds.tiles[w])[h * S::kDim + d];
+        }
+        if (seg.slot < 0) {
+            const int64_t to = head_of(a, seg, seg.tile * kColumns + h);
+            static_cast<uint16_t*>(a.out)[to * D + d] = T::from_float(total != 0.f ? value / total : 0.f);
+            if (SCORES && d == 0) {
+                a.totals[to * 2] = top;
+                a.totals[to * 2 + 1] = total;
+            }
+        } else if (seg.slot < a.narrow_slots) {
+            const int64_t slot = (int64_t)seg.slot * kColumns + h;
+            a.narrow[slot * D + d] = value;
+            if (d == 0) {
+                float* stats = a.narrow + a.narrow_slots * kColumns * D + slot * 2;
+                stats[0] = top;
+                stats[1] = total;
+            }
+        }
+    }
+    __syncthreads();  // the tiles are free again
+}
+
+// ---------------------------------------------------------------------------
+// The join: one work-group per sequence and kv head; four dims of a head per thread, the pieces dealt to what threads are
+// left.  A head's pieces are those of its row of the group's unit and those of the sequence's own unit.
+// ---------------------------------------------------------------------------
+struct Pieces {
+    int wide_slot, wide_count;      // of the unit's first piece: the others follow
+    int64_t wide_row;
+    int prefix_slot, prefix_count, prefix_row;  // a narrow unit of the group
+    int own_slot, own_count, own_row;
+    int count;
+    __device__ inline const float* at(const Args& a, int i, int D, const float*& stats) const {
+        if (i < wide_count) {
+            const int64_t row = (int64_t)(wide_slot + i) * kWideRows + wide_row;
+            stats = a.wide + a.wide_slots * kWideRows * D + row * 2;
+            return a.wide + row * D;
+        }
+        i -= wide_count;
+        int64_t row;
+        if (i < prefix_count) row = (int64_t)(prefix_slot + i) * kColumns + prefix_row;
+        else row = (int64_t)(own_slot + i - prefix_count) * kColumns + own_row;
+        stats = a.narrow + a.narrow_slots * kColumns * D + row * 2;
+        return a.narrow + row * D;
+    }
+};
+
+// What all heads of a sequence and kv head have in common.
+struct Join {
+    Walk w;
+    int kv_head, seq, len, start;
+    int group, group_base, group_unit;  // of the group's units, if start > 0
+    Group x;
+    int own_base;
+    __device__ inline void find(const Args& a, int s, int h) {
+        w.count(a);
+        seq = s;
+        kv_head = h;
+        len = w.length(a, seq);
+        start = w.start(a, seq, len, &group);
+        group_base = group_unit = 0;
+        x = Group{0, 0, 0, false, 0, 0};
+        if (start > 0) {
+            x = w.group(a, group);
+            w.place_of_group(a, group, group_base, group_unit);
+        }
+        own_base = w.place_of_sequence(a, seq);
+    }
+    // False: one share had the whole unit, and wrote the output.
+    __device__ inline bool pieces(const Args& a, int head, Pieces& p) const {
+        p = Pieces{0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        const int units = w.narrow_units + a.batch * a.head_tiles;
+        if (start > 0) {
+            const int64_t row = (int64_t)(seq - x.first) * a.group + head;
+            const int per = x.wide ? kWideRows : kColumns, tile = (int)(row / per);
+            const int at = kv_head * w.total + group_base + tile * x.rounds;
+            const int first = at / w.share, last = (at + x.rounds - 1) / w.share;
+            if (x.wide) {
+                p.wide_slot = kv_head * w.wide_units + group_unit + tile + first;
+                p.wide_count = last - first + 1;
+                p.wide_row = row - (int64_t)tile * per;
+            } else {
+                p.prefix_slot = kv_head * units + group_unit + tile + first;
+                p.prefix_count = last - first + 1;
+                p.prefix_row = (int)(row - (int64_t)tile * per);
+            }
+        }
+        const int rounds = (len - start + kRound - 1) / kRound;
+        if (rounds > 0) {
+            const int tile = head / kColumns;
+            const int at = kv_head * w.total + own_base + tile * rounds;
+            const int first = at / w.share, last = (at + rounds - 1) / w.share;
+            if (start == 0 && first == last) return false;
+            p.own_slot = kv_head * units + w.narrow_units + seq * a.head_tiles + tile + first;
+            p.own_count = last - first + 1;
+            p.own_row = head - tile * kColumns;
+        }
+        p.count = p.wide_count + p.prefix_count + p.own_count;
+        return true;
+    }
+};
+
+template <typename T, int D>
+__device__ inline void join_heads(const Args& a, int seq, int kv_head) {
+    constexpr int kLanes = D / 4, kGroups = kThreads / kLanes;
+    __shared__ __attribute__((aligned(16))) float sums[kGroups][D];
+    __shared__ float stats[kGroups][2];
+    Join j;
+    j.find(a, seq, kv_head);
+    const int heads = min(a.group, kGroups), parts = kGroups / heads;
+    const int group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    const int part = group / heads;
+    for (int h0 = 0; h0 < a.group; h0 += heads) {
+        const int head = h0 + group % heads;
+        const bool mine = group < kGroups && part < parts && head < a.group;
+        Pieces p;
+        const bool joins = mine && j.pieces(a, head, p);
+        f32x4 value = {0.f, 0.f, 0.f, 0.f};
+        float ref = kRefNone, sum = 0.f;
+        if (joins) {
+#pragma unroll 4
+            for (int i = part; i < p.count; i += parts) {
+                const float* s;
+                const f32x4 v = *reinterpret_cast<const f32x4*>(p.at(a, i, D, s) + 4 * lane);
+                const float top = fmaxf(ref, s[0]), keep = fast_exp2(ref - top), by = fast_exp2(s[0] - top);
+                value = value * keep + v * by;
+                sum = sum * keep + s[1] * by;
+                ref = top;
+            }
+        }
+        __syncthreads();  // (the pass before has read the sums)
+        if (group < kGroups) {
+            *reinterpret_cast<f32x4*>(&sums[group][4 * lane]) = value;
+            if (lane == 0) {
+                stats[group][0] = ref;
+                stats[group][1] = sum;
+            }
+        }
+        __syncthreads();
+        if (joins && part == 0) {
+            for (int i = 1; i < parts; ++i) {
+                const int other = group + i * heads;
+                const float top = fmaxf(ref, stats[other][0]);
+                const float keep = fast_exp2(ref - top), by = fast_exp2(stats[other][0] - top);
+                value = value * keep + *reinterpret_cast<const f32x4*>(&sums[other][4 * lane]) * by;
+                sum = sum * keep + stats[other][1] * by;
+                ref = top;
+            }
+            const float by = 1.f / sum;
+            const f32x4 v = sum != 0.f ? value * by : f32x4{0.f, 0.f, 0.f, 0.f};
+            const int64_t to = (int64_t)seq * a.q_heads + kv_head * a.group + head;
+            u32x2 out = {T::pack(v[0], v[1]), T::pack(v[2], v[3])};
+            *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to * D + 4 * lane) = out;
+        }
+    }
+}
+
+inline bool head_dim_built(int64_t d) {
+    return d == 16 || d == 32 || d == 64 || d == 80 || d == 96 || d == 128 || d == 192 || d == 256;
+}
+
+constexpr int64_t kMostBatchHeads = int64_t(1) << 24;
+
+// The checks that the decode entry points make of their shapes, and what follows from these.
+inline int check_shape(Args& a, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,
+                       int64_t block_size, int64_t table_width, int dtype) {
+    if (!valid_dtype(dtype)) return fail(MVME_EINVAL, "FP16/BF16 required");
+    if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || num_blocks <= 0) return fail(MVME_EINVAL, "empty batch/heads/cache");
+    if (q_heads % kv_heads != 0) return fail(MVME_EINVAL, "head dimension or GQA mismatch");
+    if (!head_dim_built(head_dim)) return fail(MVME_EINVAL, "supported head_dim: 16,32,64,80,96,128,192,256");
+    if (block_size <= 0 || table_width <= 0) return fail(MVME_EINVAL, "invalid block table");
+    if (block_size > kMaxCapacity || table_width > kMaxCapacity / block_size)
+        return fail(MVME_EINVAL, "maximum table capacity is 1M tokens");
+    if (q_heads > kMostBatchHeads || batch > kMostBatchHeads / q_heads) return fail(MVME_EINVAL, "batch/head product too large");
+    // Positions in the walk are 32-bit: a sequence's own units, and at most as many again of its group (narrow units of
+    // whose rows the last may be partial).
+    const int64_t group = q_heads / kv_heads, rounds = (block_size * table_width - 1) / kRound + 1;
+    if (batch * kv_heads * ((group - 1) / kColumns + 1) * 3 > (int64_t(1) << 30) / rounds)
+        return fail(MVME_EINVAL, "too many cached tokens for one call");
+    const int64_t row = kv_heads * head_dim * 2;
+    if (row > 65536 * 16 || num_blocks > 2147483647 || num_blocks > (int64_t(1) << 62) / row / block_size)
+        return fail(MVME_EINVAL, "KV cache too large");
+    a.num_blocks = num_blocks;
+    a.page_bytes = (uint64_t)(row * block_size);
+    a.row_bytes = (uint32_t)row;
+    a.batch = (int)batch;
+    a.kv_heads = (int)kv_heads;
+    a.q_heads = (int)q_heads;
+    a.group = (int)group;
+    a.width = (int)table_width;
+    a.head_tiles = (int)((group - 1) / kColumns + 1);
+    a.div = fp4::make_block_div(block_size);
+    a.group_div = fp4::make_block_div(group);
+    a.scale = kLog2e / __builtin_sqrtf((float)head_dim);
+    return MVME_OK;
+}
+
+}  // namespace lng
+}  // namespace mvme

@@ -88,7 +88,8 @@ def host_digest() -> str:
     import torch
 
     digest = hashlib.sha256()
-    for path in (SOURCE_DIR / "host_calls.cpp", INCLUDE_DIR / "mvme_paged.h", INCLUDE_DIR / "mvme_fp4.h"):
+    for path in (SOURCE_DIR / "host_calls.cpp", INCLUDE_DIR / "mvme_paged.h", INCLUDE_DIR / "mvme_fp4.h",
+                 INCLUDE_DIR / "mvme_long.h"):
         digest.update(path.read_bytes())
     for part in (torch.__version__, torch.version.git_version, torch._C._GLIBCXX_USE_CXX11_ABI,
                  sysconfig.get_config_var("EXT_SUFFIX")):

@@ -24,6 +24,7 @@ from dataclasses import dataclass
 import torch
 
 from ..kernels import data as _data
+from ..kernels import evict as _evict
 from ..kernels import fp4 as _fp4
 from ..kernels import hip_extension as ext
 from ..kernels import pages as _pages
@@ -150,6 +151,11 @@ class KVCachePool(_PageMoves):
                          s.num_kv_heads, s.head_dim, pages.ids.data_ptr(), pages.ids.numel(), token_count,
                          ext.dtype_code(self.dtype), ext.current_stream(self.device))
         return packed[0], packed[1]
+
+    def evict(self, weights, block_tables, context_lens, keep, *, first=None, recent=0, validate=True):
+        """``evict_kv_cache`` over every layer: weights [layers, sequences, kv_heads, capacity]."""
+        return _evict.evict_kv_cache(self.key, self.value, weights, block_tables, context_lens, self.shape.block_size,
+                                     keep, first=first, recent=recent, validate=validate)
 
 
 class KVCachePoolFP4(_PageMoves):

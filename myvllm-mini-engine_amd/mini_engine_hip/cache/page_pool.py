@@ -115,6 +115,19 @@ class PagePool:
         table += self._take(max(0, self.blocks_required(token_count) - len(table)))
         return list(table)
 
+    def truncate(self, request_id: str, token_count: int) -> list[int]:
+        """Give back the pages of a request behind its first ``token_count`` tokens (after an eviction).
+
+        Returns its table.
+        """
+        table = self._owned[request_id]
+        if not 0 <= token_count <= len(table) * self.block_size:
+            raise ValueError("truncation passes the request's pages")
+        for page in reversed(table[self.blocks_required(token_count):]):
+            self._release(page)
+        del table[self.blocks_required(token_count):]
+        return list(table)
+
     def make_writable(self, request_id: str, index: int):
         """Before writing into page ``index`` of a table: a page that others hold too is replaced by a copy.
 

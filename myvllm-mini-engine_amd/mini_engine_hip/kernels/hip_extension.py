@@ -73,6 +73,17 @@ PACKED_SIGNATURES = {
     "mvme_compact_pages": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp]),
 }
 
+# The operators for long contexts; mirrors include/mvme_long.h.
+LONG_SIGNATURES = {
+    "mvme_paged_attention_shared_prefix_workspace_size": (_size, [_i64] * 5),
+    "mvme_paged_attention_shared_prefix": (_int, [_vp] * 8 + [_i64] * 8 + [_int, _vp, _size, _vp]),
+    "mvme_paged_attention_weights_workspace_size": (_size, [_i64] * 6),
+    "mvme_paged_attention_weights": (_int, [_vp] * 7 + [_i64] * 8 + [_int, _vp, _size, _vp]),
+    "mvme_prefill_attention_weights_workspace_size": (_size, [_i64] * 7),
+    "mvme_prefill_attention_weights": (_int, [_vp] * 7 + [_i64] * 9 + [_int, _vp, _size, _vp]),
+    "mvme_evict_kv_cache": (_int, [_vp] * 4 + [_i64] + [_vp] * 5 + [_i64] * 9 + [_int, _vp]),
+}
+
 
 class HipLibrary:
     """Typed handle on the shared object; every call checks its status."""
@@ -80,7 +91,7 @@ class HipLibrary:
     def __init__(self, lib: ctypes.CDLL, path):
         self._lib = lib
         self.path = path
-        for name, (restype, argtypes) in (SIGNATURES | PACKED_SIGNATURES).items():
+        for name, (restype, argtypes) in (SIGNATURES | PACKED_SIGNATURES | LONG_SIGNATURES).items():
             fn = getattr(lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -112,6 +123,15 @@ class HipLibrary:
     def fp4_prefill_workspace_size(self, *args) -> int:
         return int(self._lib.mvme_fp4_paged_prefill_workspace_size(*args))
 
+    def shared_prefix_workspace_size(self, *args) -> int:
+        return int(self._lib.mvme_paged_attention_shared_prefix_workspace_size(*args))
+
+    def weights_workspace_size(self, *args) -> int:
+        return int(self._lib.mvme_paged_attention_weights_workspace_size(*args))
+
+    def prefill_weights_workspace_size(self, *args) -> int:
+        return int(self._lib.mvme_prefill_attention_weights_workspace_size(*args))
+
     def argmax_workspace_size(self, *args) -> int:
         return int(self._lib.mvme_greedy_argmax_workspace_size(*args))
 
@@ -140,6 +160,7 @@ class NoNativeCalls:
         return None
 
     decode = decode_write = prefill = dense = linear = rope_slots = write_slots = _decline
+    shared_prefix = decode_weights = prefill_weights = evict = _decline
     fp4_decode = fp4_prefill = fp4_write_slots = fp4_write_batch = fp4_gather_slots = move_pages = _decline
 
 
@@ -181,7 +202,11 @@ _HOST_ENTRY_POINTS = ("mvme_last_error", "mvme_paged_attention_workspace_size", 
                       "mvme_qk_norm_rope_write_kv", "mvme_fp4_record_bytes", "mvme_fp4_write_slots",
                       "mvme_fp4_write_batch", "mvme_fp4_gather_slots", "mvme_fp4_paged_attention_workspace_size",
                       "mvme_fp4_paged_attention", "mvme_fp4_paged_prefill_workspace_size",
-                      "mvme_fp4_paged_prefill_attention", "mvme_copy_pages", "mvme_compact_pages")
+                      "mvme_fp4_paged_prefill_attention", "mvme_copy_pages", "mvme_compact_pages",
+                      "mvme_paged_attention_shared_prefix_workspace_size", "mvme_paged_attention_shared_prefix",
+                      "mvme_paged_attention_weights_workspace_size", "mvme_paged_attention_weights",
+                      "mvme_prefill_attention_weights_workspace_size", "mvme_prefill_attention_weights",
+                      "mvme_evict_kv_cache")
 
 
 @functools.lru_cache(maxsize=1)
