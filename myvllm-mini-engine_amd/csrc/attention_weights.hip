@@ -25,9 +25,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weighted_decode_ke
 }
 
 constexpr int kAddKeys = 4 * kThreads;  // keys whose weights a work-group adds up
+constexpr int kHeads = 8;               // heads whose scores are in flight
 
 // Joins the pieces, and adds weights: work-groups 0 .. batch * kv_heads - 1 do the first, the others take kAddKeys keys of
-// one sequence and kv head each.
+// one sequence and kv head each, four in a row per thread.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void weighted_join_kernel(Args a, int blocks) {
     const int units = a.batch * a.kv_heads;
@@ -37,28 +38,42 @@ __global__ __launch_bounds__(kThreads) void weighted_join_kernel(Args a, int blo
     }
     const int item = blockIdx.x - units, block = item % blocks, unit = item / blocks;
     const int seq = unit / a.kv_heads, kv_head = unit % a.kv_heads;
-    const int len = Walk::length(a, seq);
+    const int len = Walk::length_from(a, a.lens[seq]);
     if (block * kAddKeys >= len) return;
-    __shared__ float stats[kThreads][2];  // (reference, 1 / sum) of the heads at hand
-    Join j;
-    j.find(a, seq, kv_head);
+    __shared__ float stats[kHeads][2];  // (reference, 1 / sum) of the heads at hand
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t head0 = (int64_t)seq * a.q_heads + kv_head * a.group;
-    float* out = a.weights + ((int64_t)seq * a.kv_heads + kv_head) * a.weight_row;
-    float add[4] = {0.f, 0.f, 0.f, 0.f};
-    const int key = block * kAddKeys + threadIdx.x;
-    for (int h0 = 0; h0 < a.group; h0 += kThreads) {
-        const int heads = min(a.group - h0, kThreads);
+    const int key = block * kAddKeys + 4 * threadIdx.x;
+    float* out = a.weights + ((int64_t)seq * a.kv_heads + kv_head) * a.weight_row + key;
+    // The scores do not wait for the divisors.  (Keys behind the context are read where there are some, and not used.)
+    const float* scores = a.scores + head0 * a.score_row + (key < len ? key : 0);
+    f32x4 s[kHeads];
+    const auto load = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i)
+            s[i] = *reinterpret_cast<const f32x4*>(scores + min(h0 + i, a.group - 1) * a.score_row);
+    };
+    load(0);
+    float before[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) before[i] = key + i < len ? out[i] : 0.f;
+    Join j;
+    j.find(a, seq, kv_head);
+    f32x4 add = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int h0 = 0; h0 < a.group; h0 += kHeads) {
+        if (h0) load(h0);
         __syncthreads();
-        for (int h = wave; h < heads; h += kWaves) {
-            Pieces p;
+        for (int h = wave; h < kHeads; h += kWaves) {
             float ref = kRefNone, sum = 0.f;
-            if (j.pieces(a, h0 + h, p)) {
+            Pieces p;
+            if (h0 + h >= a.group) {
+            } else if (j.pieces(a, h0 + h, p)) {
                 for (int i = lane; i < p.count; i += kWave) {
-                    const float* s;
-                    p.at(a, i, D, s);
-                    const float top = fmaxf(ref, s[0]);
-                    sum = sum * fast_exp2(ref - top) + s[1] * fast_exp2(s[0] - top);
+                    const float* of;
+                    p.at(a, i, D, of);
+                    const float top = fmaxf(ref, of[0]);
+                    sum = sum * fast_exp2(ref - top) + of[1] * fast_exp2(of[0] - top);
                     ref = top;
                 }
                 float top = ref;
@@ -76,18 +91,17 @@ __global__ __launch_bounds__(kThreads) void weighted_join_kernel(Args a, int blo
             }
         }
         __syncthreads();
-        for (int h = 0; h < heads; ++h) {
-            const float ref = stats[h][0], by = stats[h][1];
-            const float* s = a.scores + (head0 + h0 + h) * a.score_row;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (key + i * kThreads < len)
-                    add[i] += fast_exp2(__builtin_fmaf(s[key + i * kThreads], a.scale, -ref)) * by;
-        }
+        for (int h = 0; h < kHeads; ++h)
+            if (h0 + h < a.group) {
+                const float ref = stats[h][0], by = stats[h][1];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) add[i] += fast_exp2(__builtin_fmaf(s[h][i], a.scale, -ref)) * by;
+            }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (key + i * kThreads < len) out[key + i * kThreads] += add[i];
+        if (key + i < len) out[i] = before[i] + add[i];
 }
 
 int work_groups(int64_t head_dim) { return head_dim <= 128 ? 512 : 256; }

@@ -82,11 +82,18 @@ __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v);
 // The walk.  Every wave computes the same, lane-parallel over the groups or sequences.  Order: kv heads; of each the wide
 // units, the narrow units of groups, the sequences' units.
 // ---------------------------------------------------------------------------
+// What a lane holds of a group.
 struct Group {
     int first, rows;     // sequences
     int prefix;          // tokens; 0: nothing is shared
     bool wide;
     int rounds, tiles;   // of a unit, and units
+};
+// What a lane holds of a sequence.
+struct Own {
+    int len;             // 0 where the length cannot be
+    int start;           // where its own keys begin: behind its group's prefix, if it reaches to the end of that
+    __device__ inline int rounds() const { return (len - start + kRound - 1) / kRound; }
 };
 
 struct Walk {
@@ -95,15 +102,13 @@ struct Walk {
     int wide_rounds, narrow_rounds;   // the same in rounds
     int total;                        // rounds of a kv head
     int share;
+    Group group0;                     // of group `lane`
+    Own own0;                         // of sequence `lane`
 
     __device__ static inline int64_t capacity(const Args& a) { return (int64_t)a.width * a.div.size; }
 
-    __device__ inline Group group(const Args& a, int g) const {
-        Group x{0, 0, 0, false, 0, 0};
-        if (!grouped || g >= a.groups) return x;
-        x.first = (int)a.offsets[g];
-        x.rows = (int)a.offsets[g + 1] - x.first;
-        const int64_t prefix = a.prefixes[g];
+    __device__ static inline Group group_from(const Args& a, int64_t first, int64_t next, int64_t prefix) {
+        Group x{(int)first, (int)(next - first), 0, false, 0, 0};
         // (One row alone gains nothing, and needs no unit for it.)
         x.prefix = x.rows >= 2 && prefix > 0 && prefix <= capacity(a) ? (int)prefix : 0;
         const int64_t rows = (int64_t)x.rows * a.group;
@@ -112,69 +117,108 @@ struct Walk {
         x.tiles = x.prefix ? (int)(x.wide ? (rows + kWideRows - 1) / kWideRows : (rows + kColumns - 1) / kColumns) : 0;
         return x;
     }
-    // Tokens of a sequence; 0 where the length cannot be.
-    __device__ static inline int length(const Args& a, int seq) {
-        const int64_t n = seq < a.batch ? a.lens[seq] : 0;
-        return n > 0 && n <= capacity(a) ? (int)n : 0;
+    // Group g0 + lane.
+    __device__ inline Group group(const Args& a, int g0) const {
+        const int g = g0 + __lane_id();
+        if (g0 == 0) return group0;
+        if (!grouped || g >= a.groups) return Group{0, 0, 0, false, 0, 0};
+        return group_from(a, a.offsets[g], a.offsets[g + 1], a.prefixes[g]);
     }
-    // The group that a sequence is in, or -1.
-    __device__ inline int group_of(const Args& a, int seq) const {
-        if (!grouped) return -1;
+    // Group g, for every lane.
+    __device__ inline Group group_at(const Args& a, int g) const {
+        if (g >= kWave) return group_from(a, a.offsets[g], a.offsets[g + 1], a.prefixes[g]);
+        return Group{lane_value(group0.first, g), lane_value(group0.rows, g), lane_value(group0.prefix, g),
+                     (bool)lane_value((int)group0.wide, g), lane_value(group0.rounds, g), lane_value(group0.tiles, g)};
+    }
+    // The prefix of the group that a sequence is in, 0 without one, and that group (-1).
+    __device__ inline int prefix_of(const Args& a, int seq, int& g) const {
+        g = -1;
+        if (!grouped) return 0;
+        int prefix = 0;
+        if (a.groups <= kWave) {
+            for (int i = 0; i < a.groups; ++i) {
+                const int behind = seq - lane_value(group0.first, i);
+                if (behind >= 0 && behind < lane_value(group0.rows, i)) {
+                    prefix = lane_value(group0.prefix, i);
+                    g = i;
+                }
+            }
+            return prefix;
+        }
         int low = 0, high = a.groups;  // the last offset that is not above seq
         while (high - low > 1) {
             const int mid = (low + high) >> 1;
             if (a.offsets[mid] <= seq) low = mid;
             else high = mid;
         }
-        return a.offsets[low] <= seq && seq < a.offsets[low + 1] ? low : -1;
+        const int64_t first = a.offsets[low], next = a.offsets[low + 1];
+        if (first > seq || seq >= next) return 0;
+        g = low;
+        return group_from(a, first, next, a.prefixes[low]).prefix;
     }
-    // Where a sequence's own keys begin: behind its group's prefix, if it reaches to the end of that.
-    __device__ inline int start(const Args& a, int seq, int len, int* group_index = nullptr) const {
-        const int g = seq < a.batch ? group_of(a, seq) : -1;
-        if (group_index) *group_index = g;
-        if (g < 0) return 0;
-        const int prefix = group(a, g).prefix;
-        return prefix <= len ? prefix : 0;
+    __device__ static inline int length_from(const Args& a, int64_t n) { return n > 0 && n <= capacity(a) ? (int)n : 0; }
+    __device__ inline Own own_from(const Args& a, int seq, int64_t length) const {
+        Own x{length_from(a, length), 0};
+        int g;
+        const int prefix = prefix_of(a, seq, g);
+        x.start = prefix <= x.len ? prefix : 0;
+        return x;
     }
-    __device__ inline int own_rounds(const Args& a, int seq) const {
-        const int n = length(a, seq);
-        return (n - start(a, seq, n) + kRound - 1) / kRound;
+    __device__ static inline int64_t load_length(const Args& a, int seq) { return seq < a.batch ? a.lens[seq] : 0; }
+    // Sequence s0 + lane.
+    __device__ inline Own own(const Args& a, int s0) const {
+        return s0 == 0 ? own0 : own_from(a, s0 + __lane_id(), load_length(a, s0 + __lane_id()));
+    }
+    // Sequence s, for every lane.
+    __device__ inline Own own_at(const Args& a, int s) const {
+        if (s < kWave) return Own{lane_value(own0.len, s), lane_value(own0.start, s)};
+        return own_from(a, s, a.lens[s]);
     }
 
     __device__ inline void count(const Args& a) {
         const int lane = __lane_id();
         wide_units = narrow_units = wide_rounds = narrow_rounds = total = 0;
+        // All that is needed first, in one round trip.
+        const int64_t length0 = load_length(a, lane);
+        int64_t first = 0, next = 0, prefix = 0, end = 0;
+        if (lane < a.groups) {
+            first = a.offsets[lane];
+            next = a.offsets[lane + 1];
+            prefix = a.prefixes[lane];
+        }
+        if (a.groups > 0) end = a.offsets[a.groups];
         grouped = a.groups > 0;
         if (grouped) {
-            bool good = a.offsets[0] >= 0 && a.offsets[a.groups] <= a.batch;
-            for (int g0 = 0; g0 < a.groups; g0 += kWave)
-                if (g0 + lane < a.groups) good = good && a.offsets[g0 + lane] <= a.offsets[g0 + lane + 1];
+            bool good = lane >= a.groups || first <= next;
+            if (lane == 0) good = good && first >= 0 && end <= a.batch;
+            for (int g = kWave + lane; g < a.groups; g += kWave) good = good && a.offsets[g] <= a.offsets[g + 1];
             grouped = __all(good);
         }
+        group0 = grouped && lane < a.groups ? group_from(a, first, next, prefix) : Group{0, 0, 0, false, 0, 0};
         if (grouped)
             for (int g0 = 0; g0 < a.groups; g0 += kWave) {
-                const Group x = group(a, g0 + lane);
+                const Group x = group(a, g0);
                 const int w = x.wide ? x.tiles : 0, n = x.wide ? 0 : x.tiles;
                 wide_units += lane_value(wave_incl_scan(w), kWave - 1);
                 narrow_units += lane_value(wave_incl_scan(n), kWave - 1);
                 wide_rounds += lane_value(wave_incl_scan(w * x.rounds), kWave - 1);
                 narrow_rounds += lane_value(wave_incl_scan(n * x.rounds), kWave - 1);
             }
-        int own = 0;
-        for (int s0 = 0; s0 < a.batch; s0 += kWave) own += lane_value(wave_incl_scan(own_rounds(a, s0 + lane)), kWave - 1);
-        total = wide_rounds + narrow_rounds + own * a.head_tiles;
+        own0 = own_from(a, lane, length0);
+        int rounds = 0;
+        for (int s0 = 0; s0 < a.batch; s0 += kWave) rounds += lane_value(wave_incl_scan(own(a, s0).rounds()), kWave - 1);
+        total = wide_rounds + narrow_rounds + rounds * a.head_tiles;
         const int all = total * a.kv_heads;
         // Two rounds at least, where that gives every CU one share: more pieces cost the join more than they save.
         share = max(max((all + a.shares - 1) / a.shares, min((all + 255) / 256, 2)), 1);
     }
 
-    // Unit `tile` of `group` begins at round `base` of its kv head and is number `unit` among its kind.
-    __device__ inline void place_of_group(const Args& a, int g, int& base, int& unit) const {
+    // The units of `group` begin at round `base` of a kv head, and number `unit` among their kind.
+    __device__ inline void place_of_group(const Args& a, int g, bool wide, int& base, int& unit) const {
         const int lane = __lane_id();
         base = unit = 0;
-        const bool wide = group(a, g).wide;
         for (int g0 = 0; g0 < g; g0 += kWave) {
-            const Group x = group(a, g0 + lane);
+            const Group x = group(a, g0);
             const bool counts = g0 + lane < g && x.wide == wide;
             base += lane_value(wave_incl_scan(counts ? x.tiles * x.rounds : 0), kWave - 1);
             unit += lane_value(wave_incl_scan(counts ? x.tiles : 0), kWave - 1);
@@ -186,7 +230,7 @@ struct Walk {
         const int lane = __lane_id();
         int base = 0;
         for (int s0 = 0; s0 < seq; s0 += kWave)
-            base += lane_value(wave_incl_scan(s0 + lane < seq ? own_rounds(a, s0 + lane) : 0), kWave - 1);
+            base += lane_value(wave_incl_scan(s0 + lane < seq ? own(a, s0).rounds() : 0), kWave - 1);
         return wide_rounds + narrow_rounds + base * a.head_tiles;
     }
 };
@@ -196,7 +240,7 @@ struct Segment {
     int seq;              // whose pages
     int kv_head, tile;
     int first_row;        // of the group's sequences; -1: the sequence's own keys
-    int rows;             // live rows of the unit (wide, narrow)
+    int rows;             // rows of the unit from the tile's first on
     uint32_t begin, end;  // keys
     int slot;             // where its piece goes; -1: it is all that its rows have
     int rounds;
@@ -204,20 +248,19 @@ struct Segment {
 };
 
 __device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int stop) {
-    const int lane = __lane_id();
     Segment s;
     s.kv_head = at / w.total;
     int q = at - s.kv_head * w.total;
-    const int wg = blockIdx.x;
     int from, rounds, tokens, start = 0;
+    const int units = w.narrow_units + a.batch * a.head_tiles;
     if (q < w.wide_rounds + w.narrow_rounds) {
         s.wide = q < w.wide_rounds;
         if (!s.wide) q -= w.wide_rounds;
-        int before = 0, units = 0, g = 0, base = 0, unit = 0;
+        int before = 0, units_before = 0, g = 0, base = 0, unit = 0;
         for (int g0 = 0; g0 < a.groups; g0 += kWave) {
-            const Group x = w.group(a, g0 + lane);
+            const Group x = w.group(a, g0);
             const int tiles = x.wide == s.wide ? x.tiles : 0;
-            const int incl = before + wave_incl_scan(tiles * x.rounds), incl_units = units + wave_incl_scan(tiles);
+            const int incl = before + wave_incl_scan(tiles * x.rounds), incl_units = units_before + wave_incl_scan(tiles);
             const uint64_t hit = __ballot(incl > q);
             if (hit) {
                 const int at_lane = __builtin_ctzll(hit);
@@ -227,9 +270,9 @@ __device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int
                 break;
             }
             before = lane_value(incl, kWave - 1);
-            units = lane_value(incl_units, kWave - 1);
+            units_before = lane_value(incl_units, kWave - 1);
         }
-        const Group x = w.group(a, g);
+        const Group x = w.group_at(a, g);
         rounds = max(x.rounds, 1);
         s.tile = (q - base) / rounds;
         from = q - base - s.tile * rounds;
@@ -238,7 +281,7 @@ __device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int
         s.first_row = x.first;
         s.rows = x.rows * a.group - s.tile * (s.wide ? kWideRows : kColumns);
         unit += s.tile;
-        s.slot = (s.wide ? s.kv_head * w.wide_units + unit : s.kv_head * (w.narrow_units + a.batch * a.head_tiles) + unit) + wg;
+        s.slot = (s.wide ? s.kv_head * w.wide_units : s.kv_head * units) + unit + (int)blockIdx.x;
     } else {
         q -= w.wide_rounds + w.narrow_rounds;
         s.wide = false;
@@ -246,7 +289,7 @@ __device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int
         int before = 0, base = 0;
         s.seq = 0;
         for (int s0 = 0; s0 < a.batch; s0 += kWave) {
-            const int mine = w.own_rounds(a, s0 + lane) * a.head_tiles, incl = before + wave_incl_scan(mine);
+            const int mine = w.own(a, s0).rounds() * a.head_tiles, incl = before + wave_incl_scan(mine);
             const uint64_t hit = __ballot(incl > q);
             if (hit) {
                 const int at_lane = __builtin_ctzll(hit);
@@ -256,14 +299,14 @@ __device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int
             }
             before = lane_value(incl, kWave - 1);
         }
-        const int n = w.length(a, s.seq);
-        start = w.start(a, s.seq, n);
-        tokens = n - start;
-        rounds = max((tokens + kRound - 1) / kRound, 1);
+        const Own own = w.own_at(a, uniform(s.seq));
+        start = own.start;
+        tokens = own.len - start;
+        rounds = max(own.rounds(), 1);
         s.tile = (q - base) / rounds;
         from = q - base - s.tile * rounds;
         s.rows = a.group - s.tile * kColumns;
-        s.slot = s.kv_head * (w.narrow_units + a.batch * a.head_tiles) + w.narrow_units + s.seq * a.head_tiles + s.tile + wg;
+        s.slot = s.kv_head * units + w.narrow_units + s.seq * a.head_tiles + s.tile + (int)blockIdx.x;
     }
     const int n = min(rounds - from, stop - at);
     if (s.first_row < 0 && start == 0 && n == rounds) s.slot = -1;
@@ -292,39 +335,88 @@ __device__ inline int64_t head_of(const Args& a, const Segment& s, int row) {
 }
 
 // ---------------------------------------------------------------------------
-// Narrow tiles: 16 rows, 32 keys.  Lane (r, g) = (lane % 16, lane / 16) has token r of each half of the tile and the
-// dims of part g: keys are at once an operand of the score product, values go through LDS for the transposition.
+// Narrow tiles: 16 rows, 32 keys, of one wave alone.  Loads take whole rows of memory; both planes go through LDS, keys to
+// become operands of the score product, values for their transposition.
 // ---------------------------------------------------------------------------
-// RUN tokens (block sizes that are multiples of it) lie in one page at consecutive places.
-struct Where {
-    int64_t at[2];     // byte offset of the half's first (RUN 1: the lane's) token in a plane; of one that exists
-    bool there[2];
-};
-
+// RUN tokens (block sizes that are multiples of it) lie in one page at consecutive places.  RUN 16: a tile's halves are
+// looked up by the whole wave; RUN 1: lane i looks up token i of the tile.
 template <int RUN>
-__device__ inline Where look_up(const Args& a, const int64_t* table, int64_t head_at, uint32_t first, uint32_t end, int r) {
-    Where w;
+struct Where {
+    int64_t at[RUN == 16 ? 2 : 1];  // byte offset of the half's first (the lane's) token in a plane, or of one that exists
+    uint32_t present;               // the tile's tokens that are there
+};
+template <int RUN>
+struct Pages {
+    int64_t page[RUN == 16 ? 2 : 1];
+};
+template <int RUN>
+__device__ inline Pages<RUN> load_pages(const Args& a, const int64_t* table, uint32_t first) {
+    Pages<RUN> p;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const uint32_t token = first + 16 * s + (RUN == 1 ? r : 0), block = a.div.page(token);
-        const int64_t* entry = table + min(block, (uint32_t)a.width - 1u);
-        int64_t page = RUN == 1 ? *entry : uniform_load(entry);
-        w.there[s] = token < end && (uint64_t)page < (uint64_t)a.num_blocks;
-        page = w.there[s] ? page : 0;
-        const uint32_t place = w.there[s] ? token - block * a.div.size : 0u;
-        w.at[s] = head_at + (int64_t)((uint64_t)(uint32_t)page * a.page_bytes) + (int64_t)((uint64_t)place * a.row_bytes);
+    for (int s = 0; s < (RUN == 16 ? 2 : 1); ++s) {
+        const uint32_t token = first + (RUN == 16 ? 16 * s : (int)(threadIdx.x & 31));
+        const int64_t* entry = table + min(a.div.page(token), (uint32_t)a.width - 1u);
+        p.page[s] = RUN == 1 ? *entry : uniform_load(entry);
+    }
+    return p;
+}
+template <int RUN>
+__device__ inline Where<RUN> look_up(const Args& a, const Pages<RUN>& p, int64_t head_at, uint32_t first, uint32_t end) {
+    Where<RUN> w;
+    const uint32_t left = end > first ? end - first : 0u;
+    w.present = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+#pragma unroll
+    for (int s = 0; s < (RUN == 16 ? 2 : 1); ++s) {
+        const uint32_t token = first + (RUN == 16 ? 16 * s : (int)(threadIdx.x & 31)), block = a.div.page(token);
+        const bool there = token < end && (uint64_t)p.page[s] < (uint64_t)a.num_blocks;
+        const uint32_t page = there ? (uint32_t)p.page[s] : 0u, place = there ? token - block * a.div.size : 0u;
+        w.at[s] = head_at + (int64_t)((uint64_t)page * a.page_bytes) + (int64_t)((uint64_t)place * a.row_bytes);
+        if constexpr (RUN == 16) w.present &= there ? 0xffffffffu : s ? 0x0000ffffu : 0xffff0000u;
+        else w.present = (uint32_t)__ballot(there);
     }
     return w;
 }
 
-// A lane's part of a token: pieces g * kChunks + c of 8 dims; zeros where the padded dims are.
+// What a lane loads of a half tile (16 tokens): pieces of 16 bytes, the i-th being number lane + 64 i of the half's.
 template <int D>
-__device__ inline void load_part(u32x4 (&x)[Shape<D>::kChunks], const uint8_t* at, int g) {
+struct Lines {
+    using S = Shape<D>;
+    static constexpr int kRow = S::kDim / 8;  // pieces of a row
+    uint32_t from[S::kChunks];  // byte offset from the half's first token (RUN 1: in its row)
+    int to[S::kChunks];         // in a tile
+    int row[S::kChunks];
+    bool real[S::kChunks];      // not padding
+    __device__ inline Lines(uint32_t row_bytes) {
 #pragma unroll
-    for (int c = 0; c < Shape<D>::kChunks; ++c) {
-        if (D == Shape<D>::kDim || (g * Shape<D>::kChunks + c) * 8 < D) x[c] = *reinterpret_cast<const u32x4*>(at + 16 * c);
-        else x[c] = u32x4{0u, 0u, 0u, 0u};
+        for (int i = 0; i < S::kChunks; ++i) {
+            const int piece = (threadIdx.x & 63) + 64 * i, chunk = piece % kRow;
+            row[i] = piece / kRow;
+            from[i] = row[i] * row_bytes + chunk * 16;
+            to[i] = fp4::TileLayout<S::kDim, 16>::at(row[i], chunk);
+            real[i] = D == S::kDim || chunk * 8 < D;
+        }
     }
+};
+
+template <int D, int RUN>
+__device__ inline void load_tile(u32x4 (&x)[2][Shape<D>::kChunks], const uint8_t* plane, const Where<RUN>& w,
+                                 const Lines<D>& l, uint32_t row_bytes) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < Shape<D>::kChunks; ++i) {
+            const uint8_t* at;
+            if constexpr (RUN == 16) {
+                at = plane + w.at[s] + l.from[i];
+            } else {
+                const int from = (l.row[i] + 16 * s) << 2;
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)w.at[0]);
+                const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)(uint32_t)((uint64_t)w.at[0] >> 32));
+                at = plane + (int64_t)(((uint64_t)hi << 32) | lo) + (l.from[i] - l.row[i] * row_bytes);
+            }
+            if (D == Shape<D>::kDim || l.real[i]) x[s][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+            else x[s][i] = u32x4{0u, 0u, 0u, 0u};
+        }
 }
 
 // Two weights as sums of two numbers of the type each: the upper bits, and the rest rounded: at most 2^-15 (bf16) or 2^-21
@@ -346,7 +438,7 @@ __device__ inline u32x2 split_pair(float x, float y) {
 
 template <int D>
 struct NarrowLds {
-    uint8_t tiles[kWaves][Shape<D>::kTileBytes];
+    uint8_t tiles[kWaves][2][Shape<D>::kTileBytes];  // keys, values
     float stats[kWaves][2][kColumns];
 };
 
@@ -356,9 +448,10 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
     using S = Shape<D>;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = uniform(threadIdx.x >> 6);
-    uint8_t* tile_lds = lds.tiles[wave];
-    TileAddress<S::kDim, 16> write_at(r, g * S::kChunks), read_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
-    uint32_t lane_at = (RUN == 1 ? 0u : (uint32_t)r * a.row_bytes) + (uint32_t)(g * S::kChunks * 16);
+    uint8_t *keys_lds = lds.tiles[wave][0], *values_lds = lds.tiles[wave][1];
+    // An operand's lane (r, g) has key r of a half tile and pieces 4 c + g of 8 dims; the row's pieces likewise.
+    TileAddress<S::kDim, 16> key_at(r, g), value_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
+    Lines<D> lines(a.row_bytes);
     const int64_t* table = a.tables + (int64_t)seg.seq * a.width;
     const int64_t head_at = (int64_t)seg.kv_head * (2 * D);
     const int heads = min(kColumns, seg.rows);
@@ -371,49 +464,66 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
 #pragma unroll
     for (int n = 0; n < S::kDimTiles; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     uint32_t t0 = seg.begin + wave * kTileKeys;
-    Where now = look_up<RUN>(a, table, head_at, t0, seg.end, r);
+    Where<RUN> now;
+    Pages<RUN> pages;
     if (t0 < seg.end) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) load_part<D>(k[s], a.key + now.at[s] + lane_at, g);
-#pragma unroll
-        for (int s = 0; s < 2; ++s) load_part<D>(v[s], a.value + now.at[s] + lane_at, g);
+        now = look_up<RUN>(a, load_pages<RUN>(a, table, t0), head_at, t0, seg.end);
+        pages = load_pages<RUN>(a, table, t0 + kRound);  // of the next tile
+        load_tile<D, RUN>(k, a.key, now, lines, a.row_bytes);
+        load_tile<D, RUN>(v, a.value, now, lines, a.row_bytes);
     }
 #pragma unroll
-    for (int c = 0; c < S::kChunks; ++c) q[c] = u32x4{0u, 0u, 0u, 0u};
-    if (live) load_part<D>(q, static_cast<const uint8_t*>(a.query) + head * (2 * D) + g * S::kChunks * 16, g);
+    for (int c = 0; c < S::kChunks; ++c) {
+        q[c] = u32x4{0u, 0u, 0u, 0u};
+        if (live && (D == S::kDim || (4 * c + g) * 8 < D))
+            q[c] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.query) + head * D + (4 * c + g) * 8);
+    }
 #pragma unroll 1
     for (; t0 < seg.end; t0 += kRound) {
-        const bool more = t0 + kRound < seg.end;
-        write_at.forget();
-        read_at.forget();
-        asm volatile("" : "+v"(lane_at));
-        Where next = now;
-        if (more) next = look_up<RUN>(a, table, head_at, t0 + kRound, seg.end, r);
+        key_at.forget();
+        value_at.forget();
+        // (Behind the last tile the loads go on, from a page that exists: a branch around them would make every wait one
+        // for all of them.)
+        const Where<RUN> next = look_up<RUN>(a, pages, head_at, t0 + kRound, seg.end);
+        pages = load_pages<RUN>(a, table, t0 + 2 * kRound);
+        const uint32_t present = now.present;
+        // A wave reads only what it wrote: the LDS queue is in order, no barrier.  Registers are refilled as soon as they
+        // are in LDS.
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < S::kChunks; ++i)
+                *reinterpret_cast<u32x4*>(keys_lds + lines.to[i] + 16 * s * 2 * S::kDim) = k[s][i];
+        load_tile<D, RUN>(k, a.key, next, lines, a.row_bytes);
+        // Keys that are not there: no weight, and zeros as values (0 * NaN is NaN).
+        if (present != 0xffffffffu) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < S::kChunks; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[s][i][j] = (present >> (16 * s + lines.row[i])) & 1 ? v[s][i][j] : 0u;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < S::kChunks; ++i)
+                *reinterpret_cast<u32x4*>(values_lds + lines.to[i] + 16 * s * 2 * S::kDim) = v[s][i];
+        load_tile<D, RUN>(v, a.value, next, lines, a.row_bytes);
         f32x4 x[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < S::kChunks; ++c) x[s] = T::mfma16x16x32(k[s][c], q[c], x[s]);
+            for (int c = 0; c < S::kChunks; ++c)
+                x[s] = T::mfma16x16x32(*reinterpret_cast<const u32x4*>(keys_lds + key_at.chunk(4 * c) + 16 * s * 2 * S::kDim),
+                                       q[c], x[s]);
         }
-        if (more)
+        if (present != 0xffffffffu) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s) load_part<D>(k[s], a.key + next.at[s] + lane_at, g);
-        // Keys that are not there: no weight, and zeros as values (0 * NaN is NaN).
-        bool whole = t0 + kTileKeys <= seg.end && now.there[0] && now.there[1];
-        if constexpr (RUN == 1) whole = __all(whole);
-        if (!whole) {
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bool mine = now.there[s] && t0 + 16 * s + r < seg.end;
-                const uint32_t present = (uint32_t)(__ballot(mine) & 0xffff) >> (4 * g);
-#pragma unroll
-                for (int c = 0; c < S::kChunks; ++c)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[s][c][j] = mine ? v[s][c][j] : 0u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[s][j] = (present >> j) & 1 ? x[s][j] : kNegInf;
-            }
+                for (int j = 0; j < 4; ++j) x[s][j] = (present >> (16 * s + 4 * g + j)) & 1 ? x[s][j] : kNegInf;
         }
         if constexpr (SCORES) {
             // (Behind the context there is room up to the row's end: rows are a multiple of 32 long.)
@@ -423,15 +533,6 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
                 *reinterpret_cast<f32x4*>(to + 16) = x[1];
             }
         }
-        // Values to LDS, row-major.
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int c = 0; c < S::kChunks; ++c)
-                *reinterpret_cast<u32x4*>(tile_lds + write_at.chunk(c) + 16 * s * 2 * S::kDim) = v[s][c];
-        if (more)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) load_part<D>(v[s], a.value + next.at[s] + lane_at, g);
         float top = fmaxf(x[0][0], x[1][0]);
 #pragma unroll
         for (int j = 1; j < 4; ++j) top = fmaxf(top, fmaxf(x[0][j], x[1][j]));
@@ -458,10 +559,9 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
                 low[2 * s + j / 2] = both[1];
                 sum += p0 + p1;
             }
-        // A wave reads only what it wrote: the LDS queue is in order, no barrier.
 #pragma unroll
         for (int n = 0; n < S::kDimTiles; ++n) {
-            const u32x4 vt = value_operand(tile_lds, read_at.chunk(2 * n), read_at.chunk(2 * n) + 16 * 2 * S::kDim);
+            const u32x4 vt = value_operand(values_lds, value_at.chunk(2 * n), value_at.chunk(2 * n) + 16 * 2 * S::kDim);
             acc[n] = T::mfma16x16x32(vt, high, acc[n]);
             acc[n] = T::mfma16x16x32(vt, low, acc[n]);
         }
@@ -470,7 +570,7 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
     sum = row4_sum(sum);
 
     // Join the waves: sums [16][D] in their tiles' LDS, each relative to its own reference.
-    float* mine = reinterpret_cast<float*>(tile_lds);
+    float* mine = reinterpret_cast<float*>(keys_lds);
     if (live) {
 #pragma unroll
         for (int n = 0; n < S::kDimTiles; ++n) *reinterpret_cast<f32x4*>(mine + r * S::kDim + 16 * n + 4 * g) = acc[n];
@@ -490,7 +590,7 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
         for (int w = 0; w < kWaves; ++w) {
             const float by = fast_exp2(lds.stats[w][0][h] - top);
             total += by * lds.stats[w][1][h];
-            value += by * reinterpret_cast<const float*>(lds.tiles[w])[h * S::kDim + d];
+            value += by * reinterpret_cast<const float*>(lds.tiles[w][0])[h * S::kDim + d];
         }
         if (seg.slot < 0) {
             const int64_t to = head_of(a, seg, seg.tile * kColumns + h);
@@ -540,21 +640,23 @@ struct Pieces {
 // What all heads of a sequence and kv head have in common.
 struct Join {
     Walk w;
-    int kv_head, seq, len, start;
-    int group, group_base, group_unit;  // of the group's units, if start > 0
+    int kv_head, seq;
+    Own own;
+    int group_base, group_unit;  // of the group's units, if own.start > 0
     Group x;
     int own_base;
     __device__ inline void find(const Args& a, int s, int h) {
         w.count(a);
         seq = s;
         kv_head = h;
-        len = w.length(a, seq);
-        start = w.start(a, seq, len, &group);
+        own = w.own_at(a, seq);
         group_base = group_unit = 0;
         x = Group{0, 0, 0, false, 0, 0};
-        if (start > 0) {
-            x = w.group(a, group);
-            w.place_of_group(a, group, group_base, group_unit);
+        if (own.start > 0) {
+            int g;
+            w.prefix_of(a, seq, g);
+            x = w.group_at(a, uniform(g));
+            w.place_of_group(a, uniform(g), x.wide, group_base, group_unit);
         }
         own_base = w.place_of_sequence(a, seq);
     }
@@ -562,7 +664,7 @@ struct Join {
     __device__ inline bool pieces(const Args& a, int head, Pieces& p) const {
         p = Pieces{0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         const int units = w.narrow_units + a.batch * a.head_tiles;
-        if (start > 0) {
+        if (own.start > 0) {
             const int64_t row = (int64_t)(seq - x.first) * a.group + head;
             const int per = x.wide ? kWideRows : kColumns, tile = (int)(row / per);
             const int at = kv_head * w.total + group_base + tile * x.rounds;
@@ -577,12 +679,12 @@ struct Join {
                 p.prefix_row = (int)(row - (int64_t)tile * per);
             }
         }
-        const int rounds = (len - start + kRound - 1) / kRound;
+        const int rounds = own.rounds();
         if (rounds > 0) {
             const int tile = head / kColumns;
             const int at = kv_head * w.total + own_base + tile * rounds;
             const int first = at / w.share, last = (at + rounds - 1) / w.share;
-            if (start == 0 && first == last) return false;
+            if (own.start == 0 && first == last) return false;
             p.own_slot = kv_head * units + w.narrow_units + seq * a.head_tiles + tile + first;
             p.own_count = last - first + 1;
             p.own_row = head - tile * kColumns;

@@ -182,10 +182,8 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_rows_kernel(PromptArgs a) 
                 x[k] = mfma32<T>(*reinterpret_cast<const u32x4*>(keys + 32 * k * 2 * P + key_at.chunk(2 * i)), q[i], x[k]);
         }
         stage(staged, buffer ^ 1);
-        if (t0 + kTile < end) {
-            load(staged, t0 + 2 * kTile, page);
-            page = page_of(t0 + 3 * kTile);
-        }
+        load(staged, t0 + 2 * kTile, page);
+        page = page_of(t0 + 3 * kTile);
         const uint32_t odds = (uint32_t)uniform(*reinterpret_cast<const int*>(odd[buffer]));
         uint64_t mask = ~uint64_t(0);
         if (odds) mask = __ballot((odds >> (8 * (lane >> 4))) & 0xff ? present[buffer][lane] : true);
@@ -300,13 +298,12 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_keys_kernel(PromptArgs a) 
     };
     TileAddress<P, 32> stage_at(row, quarter), query_at(column, h);
     const auto load = [&](Piece<D>& x, uint32_t r0) {
-        const uint32_t r = r0 + row;
-        const bool live = r < rows;
-        const uint8_t* from = static_cast<const uint8_t*>(a.q) + head_of_row(live ? r : 0u) * (2 * D) + quarter * 16;
+        // (Behind the last row: the last row again, without a divisor.)
+        const uint8_t* from = static_cast<const uint8_t*>(a.q) + head_of_row(min(r0 + row, rows - 1)) * (2 * D) + quarter * 16;
 #pragma unroll
         for (int i = 0; i < S::kChunks; ++i) {
-            x.x[i] = u32x4{0u, 0u, 0u, 0u};
-            if (live && (D == P || (4 * i + quarter) * 8 < D)) x.x[i] = *reinterpret_cast<const u32x4*>(from + 64 * i);
+            if (D == P || (4 * i + quarter) * 8 < D) x.x[i] = *reinterpret_cast<const u32x4*>(from + 64 * i);
+            else x.x[i] = u32x4{0u, 0u, 0u, 0u};
         }
     };
     const auto stage = [&](Piece<D>& x, int buffer) {
@@ -318,7 +315,8 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_keys_kernel(PromptArgs a) 
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const uint32_t r = r0 + 32 * c + column;
-            x[c] = r < rows ? reinterpret_cast<const f32x2*>(a.rows)[head_of_row(r)] : f32x2{0.f, 0.f};
+            x[c] = reinterpret_cast<const f32x2*>(a.rows)[head_of_row(min(r, rows - 1))];
+            x[c][1] = r < rows ? x[c][1] : 0.f;
         }
     };
     Piece<D> staged;

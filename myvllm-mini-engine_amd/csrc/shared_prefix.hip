@@ -142,10 +142,8 @@ __device__ inline void wide_segment(const Args& a, const Segment& seg, WideLds<D
         }
         // The next tile (behind the last one: zeros) goes into the other buffer, and the one after it is loaded.
         stage(staged, buffer ^ 1);
-        if (t0 + kWideKeys < seg.end) {
-            load(staged, t0 + 2 * kWideKeys, page);
-            page = page_of(t0 + 3 * kWideKeys);
-        }
+        load(staged, t0 + 2 * kWideKeys, page);
+        page = page_of(t0 + 3 * kWideKeys);
         const uint32_t odds = (uint32_t)uniform(*reinterpret_cast<const int*>(lds.odd[buffer]));
         if (odds) {
             const bool there = (odds >> (8 * (lane >> 4))) & 0xff ? lds.present[buffer][lane] : true;
