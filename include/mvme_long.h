@@ -18,10 +18,11 @@ extern "C" {
 
 /*
  * Bytes of device workspace mvme_paged_attention_shared_prefix needs for these
- * shapes (0 for shapes that it refuses).  Pure host function.
+ * shapes (0: none, or shapes that it refuses).  Pure host function.
  */
 size_t mvme_paged_attention_shared_prefix_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
-                                                         int64_t head_dim, int64_t groups);
+                                                         int64_t head_dim, int64_t groups, int64_t block_size,
+                                                         int64_t table_width, int always);
 
 /*
  * mvme_paged_attention for a batch in which sequences share prefixes.  Group g
@@ -35,21 +36,26 @@ size_t mvme_paged_attention_shared_prefix_workspace_size(int64_t batch, int64_t 
  * all sequences ungrouped.  Every row's result is that of
  * mvme_paged_attention, to rounding: scale 1/sqrt(head_dim), zeros for lengths
  * <= 0 or beyond the table's capacity, pages out of range skipped.
- * Scores, softmax statistics and accumulators are fp32.  For the value product
- * the probabilities are rounded to the inputs' type where a prefix has more
- * than 32 query rows, and to the sum of two numbers of it elsewhere.
+ * Calls of few cached tokens (by the tables' capacity) are attended without
+ * regard to the groups, as is every call without groups: by
+ * mvme_paged_attention; always != 0 shares at any size.  Where prefixes are
+ * shared scores, softmax statistics and
+ * accumulators are fp32; for the value product the probabilities are rounded to
+ * the inputs' type where a prefix has more than 32 query rows, and to the sum
+ * of two numbers of it elsewhere.
  */
 int mvme_paged_attention_shared_prefix(void* out, const void* query, const void* key_cache, const void* value_cache,
                                        const int64_t* block_tables, const int64_t* context_lens,
                                        const int64_t* group_offsets, const int64_t* prefix_lens,
                                        int64_t batch, int64_t groups, int64_t q_heads, int64_t kv_heads,
                                        int64_t head_dim, int64_t num_blocks, int64_t block_size, int64_t table_width,
-                                       int dtype, void* workspace, size_t workspace_bytes, void* stream);
+                                       int always, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Bytes of device workspace mvme_paged_attention_weights needs for these
- * shapes (0 for shapes that it refuses): 4 per query head and token of the
- * tables' capacity, and the pieces of split sequences.  Pure host function.
+ * shapes: 4 per query head and token of the tables' capacity, and the pieces of
+ * split sequences; 0 where sequences are taken whole, or for shapes that it
+ * refuses.  Pure host function.
  */
 size_t mvme_paged_attention_weights_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                                    int64_t block_size, int64_t table_width);

@@ -10,18 +10,31 @@ namespace {
 
 template <typename T, int D, int RUN>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weighted_decode_kernel(Args a) {
-    __shared__ __attribute__((aligned(16))) NarrowLds<D> lds;
+    __shared__ __attribute__((aligned(16))) NarrowLds<D, kStoreScores> lds;
     Walk w;
     w.count(a);
-    const int all = w.total * a.kv_heads;
-    const int first = (int)min((int64_t)blockIdx.x * w.share, (int64_t)all);
-    const int stop = (int)min((int64_t)first + w.share, (int64_t)all);
+    if ((int)blockIdx.x >= w.total * a.kv_heads) return;
+    const int first = w.first_of(blockIdx.x), stop = w.first_of(blockIdx.x + 1);
 #pragma unroll 1
     for (int at = first; at < stop;) {
         const Segment s = find_segment(a, w, at, stop);
         at += s.rounds;
-        narrow_segment<T, D, RUN, true>(a, s, lds);
+        narrow_segment<T, D, RUN, kStoreScores>(a, s, lds);
     }
+}
+
+// A sequence's query heads of one kv head, whole: no walk, no workspace and no second kernel.
+template <typename T, int D, int RUN>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weighted_whole_kernel(Args a) {
+    __shared__ __attribute__((aligned(16))) NarrowLds<D, kAddWeights> lds;
+    Segment s{};
+    s.seq = blockIdx.x / a.kv_heads;
+    s.kv_head = blockIdx.x - s.seq * a.kv_heads;
+    s.first_row = -1;
+    s.rows = a.group;
+    s.end = (uint32_t)uniform(Walk::length_from(a, uniform_load(a.lens + s.seq)));
+    s.slot = -1;
+    narrow_segment<T, D, RUN, kAddWeights>(a, s, lds);
 }
 
 constexpr int kAddKeys = 4 * kThreads;  // keys whose weights a work-group adds up
@@ -46,12 +59,13 @@ __global__ __launch_bounds__(kThreads) void weighted_join_kernel(Args a, int blo
     const int key = block * kAddKeys + 4 * threadIdx.x;
     float* out = a.weights + ((int64_t)seq * a.kv_heads + kv_head) * a.weight_row + key;
     // The scores do not wait for the divisors.  (Keys behind the context are read where there are some, and not used.)
-    const float* scores = a.scores + head0 * a.score_row + (key < len ? key : 0);
+    const f32x4* scores = reinterpret_cast<const f32x4*>(a.scores) +
+                          ((int64_t)unit * (a.score_row / 4) + (key < len ? key / 4 : 0)) * a.group;
     f32x4 s[kHeads];
     const auto load = [&](int h0) {
 #pragma unroll
         for (int i = 0; i < kHeads; ++i)
-            s[i] = *reinterpret_cast<const f32x4*>(scores + min(h0 + i, a.group - 1) * a.score_row);
+            s[i] = scores[min(h0 + i, a.group - 1)];
     };
     load(0);
     float before[4];
@@ -106,12 +120,22 @@ __global__ __launch_bounds__(kThreads) void weighted_join_kernel(Args a, int blo
 
 int work_groups(int64_t head_dim) { return head_dim <= 128 ? 512 : 256; }
 
+// Whether sequences are taken whole: their scores fit the ring, and they are short or nearly fill the chip.  Whole against
+// split, us, 16 heads on 8: 1 x 512 tokens 9.2 and 11.0, 1 x 1024 14.4 and 11.9, 8 x 1024 16.3 and 15.7, 32 x 1024 25.0
+// and 32.6, 64 x 4096 177 and 199; 32 heads on 4: 1 x 1024 15.3 and 13.8, 16 x 1024 17.6 and 19.2.
+bool whole(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t capacity) {
+    const int64_t group = q_heads / kv_heads;
+    if (group > kColumns || capacity > kRound * (kRing / (8 * group))) return false;
+    return capacity <= 512 || batch * kv_heads >= 128;
+}
+
 struct Sizes {
     int64_t shares, slots, score_row;
-    int64_t floats;  // or -1: too many
+    int64_t floats;
 };
 Sizes sizes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t block_size, int64_t width) {
     Sizes s{};
+    if (whole(batch, q_heads, kv_heads, block_size * width)) return s;
     s.shares = work_groups(head_dim);
     s.slots = kv_heads * batch * ((q_heads / kv_heads - 1) / kColumns + 1) + s.shares;
     s.score_row = (block_size * width + 31) / 32 * 32;
@@ -121,7 +145,12 @@ Sizes sizes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, 
 
 template <typename T, int D>
 int launch(const Args& a, int blocks, hipStream_t s) {
-    const dim3 grid((unsigned)a.shares), block(kThreads);
+    const dim3 grid((unsigned)a.shares), block(kThreads), units((unsigned)(a.batch * a.kv_heads));
+    if (a.shares == 0) {
+        if (a.div.size % 16 == 0) hipLaunchKernelGGL((weighted_whole_kernel<T, D, 16>), units, block, 0, s, a);
+        else hipLaunchKernelGGL((weighted_whole_kernel<T, D, 1>), units, block, 0, s, a);
+        return check_launch("weighted attention");
+    }
     if (a.div.size % 16 == 0) hipLaunchKernelGGL((weighted_decode_kernel<T, D, 16>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((weighted_decode_kernel<T, D, 1>), grid, block, 0, s, a);
     if (int rc = check_launch("weighted attention")) return rc;
@@ -174,7 +203,7 @@ extern "C" int mvme_paged_attention_weights(void* out, const void* query, const 
     const Sizes s = sizes(batch, q_heads, kv_heads, head_dim, block_size, table_width);
     const int64_t blocks = (block_size * table_width - 1) / kAddKeys + 1;
     if (batch * kv_heads > kMostThreads / kThreads / (1 + blocks)) return fail(MVME_EINVAL, "batch/head product too large");
-    if (!workspace || workspace_bytes < (size_t)s.floats * sizeof(float) || !fp4::aligned(workspace, 16))
+    if (s.floats > 0 && (!workspace || workspace_bytes < (size_t)s.floats * sizeof(float) || !fp4::aligned(workspace, 16)))
         return fail(MVME_EWORKSPACE, "weighted attention workspace too small: " + std::to_string(s.floats * 4) +
                                          " bytes, 16-byte aligned, are needed");
     a.out = out;

@@ -706,13 +706,15 @@ PyObject* shared_prefix(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!stream_of(q, stream)) return nullptr;
     at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
     const int64_t groups = prefixes.size(0);
-    const size_t need = lib.shared_workspace(s.batch, s.q_heads, s.kv_heads, s.head_dim, groups);
-    at::Tensor workspace = bytes_like(q, need);
+    const size_t need = lib.shared_workspace(s.batch, s.q_heads, s.kv_heads, s.head_dim, groups, block, s.width, 0);
+    at::Tensor workspace;
+    if (need) workspace = bytes_like(q, need);
+    void* ws = need ? workspace.data_ptr() : nullptr;
     int status;
     Py_BEGIN_ALLOW_THREADS
     status = lib.shared_prefix(out.data_ptr(), q.data_ptr(), t[1]->data_ptr(), t[2]->data_ptr(), indices(*t[3]),
                                indices(*t[4]), indices(offsets), indices(prefixes), s.batch, groups, s.q_heads, s.kv_heads,
-                               s.head_dim, s.num_blocks, block, s.width, dtype_code(q), workspace.data_ptr(), need, stream);
+                               s.head_dim, s.num_blocks, block, s.width, 0, dtype_code(q), ws, need, stream);
     Py_END_ALLOW_THREADS
     if (status != MVME_OK) return raise_status("mvme_paged_attention_shared_prefix", status);
     return THPVariable_Wrap(std::move(out));
@@ -737,13 +739,14 @@ PyObject* decode_weights(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!stream_of(q, stream)) return nullptr;
     at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
     const size_t need = lib.weights_workspace(s.batch, s.q_heads, s.kv_heads, s.head_dim, block, s.width);
-    at::Tensor workspace = bytes_like(q, need);
+    at::Tensor workspace;
+    if (need) workspace = bytes_like(q, need);
+    void* ws = need ? workspace.data_ptr() : nullptr;
     int status;
     Py_BEGIN_ALLOW_THREADS
     status = lib.decode_weights(out.data_ptr(), q.data_ptr(), t[1]->data_ptr(), t[2]->data_ptr(), indices(*t[3]),
                                 indices(*t[4]), static_cast<float*>(w.data_ptr()), w.size(2), s.batch, s.q_heads,
-                                s.kv_heads, s.head_dim, s.num_blocks, block, s.width, dtype_code(q), workspace.data_ptr(),
-                                need, stream);
+                                s.kv_heads, s.head_dim, s.num_blocks, block, s.width, dtype_code(q), ws, need, stream);
     Py_END_ALLOW_THREADS
     if (status != MVME_OK) return raise_status("mvme_paged_attention_weights", status);
     return THPVariable_Wrap(std::move(out));

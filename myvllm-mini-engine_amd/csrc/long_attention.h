@@ -51,7 +51,7 @@ struct Args {
     float* wide;              // [wide slots, 128, D] sums, then [wide slots, 128, 2] (reference, sum)
     float* narrow;            // [narrow slots, 16, D], then [narrow slots, 16, 2]
     float* totals;            // [batch, q_heads, 2]: (reference, sum) of units that one share holds (scores only)
-    float* scores;            // [batch, q_heads, capacity] dot products (scores only)
+    float* scores;            // [batch, kv_heads, score_row / 4, group, 4] dot products (scores only)
     float* weights;           // [batch, kv_heads, weight_row]
     int64_t weight_row, score_row;  // (score rows are a multiple of 32 long)
     int64_t wide_slots, narrow_slots;
@@ -75,6 +75,13 @@ struct Shape {
     static constexpr int kSteps = kDim / 16;
     static constexpr int kWidePlane = kWideKeys * 2 * kDim;
 };
+
+// Barrier of the work-group for LDS alone: loads from memory stay in flight.
+__device__ inline void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
 __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -101,7 +108,7 @@ struct Walk {
     int wide_units, narrow_units;     // of a kv head, of groups
     int wide_rounds, narrow_rounds;   // the same in rounds
     int total;                        // rounds of a kv head
-    int share;
+    int share, longer;                // rounds of a share; the first `longer` shares have one more
     Group group0;                     // of group `lane`
     Own own0;                         // of sequence `lane`
 
@@ -208,9 +215,17 @@ struct Walk {
         int rounds = 0;
         for (int s0 = 0; s0 < a.batch; s0 += kWave) rounds += lane_value(wave_incl_scan(own(a, s0).rounds()), kWave - 1);
         total = wide_rounds + narrow_rounds + rounds * a.head_tiles;
-        const int all = total * a.kv_heads;
-        // Two rounds at least, where that gives every CU one share: more pieces cost the join more than they save.
-        share = max(max((all + a.shares - 1) / a.shares, min((all + 255) / 256, 2)), 1);
+        // Shares differ by a round at most, the first ones are longer.
+        const int all = total * a.kv_heads, shares = max(min(a.shares, all), 1);
+        share = all / shares;
+        longer = all - share * shares;
+    }
+    // First round of a work-group's share.
+    __device__ inline int first_of(int wg) const { return wg * share + min(wg, longer); }
+    // The work-group in whose share a round is.
+    __device__ inline int owner(int round) const {
+        const int until = longer * (share + 1);
+        return round < until ? round / (share + 1) : longer + (round - until) / max(share, 1);
     }
 
     // The units of `group` begin at round `base` of a kv head, and number `unit` among their kind.
@@ -436,19 +451,27 @@ __device__ inline u32x2 split_pair(float x, float y) {
     return u32x2{high, __builtin_bit_cast(uint32_t, low)};
 }
 
-template <int D>
+constexpr int kRing = 512;  // 16-byte pieces of scores that a wave gathers before it stores them
+
+// What becomes of a segment's dot products: nothing, they go to memory, or (the segment is a whole unit, and the ring holds
+// it) they become weights at its end.
+enum Scores { kNoScores, kStoreScores, kAddWeights };
+
+template <int D, Scores SCORES>
 struct NarrowLds {
-    uint8_t tiles[kWaves][2][Shape<D>::kTileBytes];  // keys, values
+    uint8_t tiles[kWaves][Shape<D>::kTileBytes];  // keys, then values
+    f32x4 ring[SCORES ? kWaves : 1][SCORES ? kRing : 1];
     float stats[kWaves][2][kColumns];
+    float divisors[2][kColumns];                  // (reference, 1 / sum)
 };
 
-// One segment of a narrow unit.  SCORES: its dot products are kept.
-template <typename T, int D, int RUN, bool SCORES>
-__device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowLds<D>& lds) {
+// One segment of a narrow unit.
+template <typename T, int D, int RUN, Scores SCORES>
+__device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowLds<D, SCORES>& lds) {
     using S = Shape<D>;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = uniform(threadIdx.x >> 6);
-    uint8_t *keys_lds = lds.tiles[wave][0], *values_lds = lds.tiles[wave][1];
+    uint8_t* tile_lds = lds.tiles[wave];
     // An operand's lane (r, g) has key r of a half tile and pieces 4 c + g of 8 dims; the row's pieces likewise.
     TileAddress<S::kDim, 16> key_at(r, g), value_at(4 * g + (r >> 2), (r & 3) >> 1, (r & 1) * 8);
     Lines<D> lines(a.row_bytes);
@@ -456,7 +479,23 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
     const int64_t head_at = (int64_t)seg.kv_head * (2 * D);
     const int heads = min(kColumns, seg.rows);
     const bool live = r < heads;
-    const int64_t head = head_of(a, seg, live ? seg.tile * kColumns + r : 0);
+    // (Columns without a row repeat the last row: what follows needs no branch for them.)
+    const int64_t head = head_of(a, seg, seg.tile * kColumns + min(r, heads - 1));
+
+    // Scores go to memory many tiles at a time: stores among the loads hold these up (a load is done only when the stores
+    // before it are).  4 x 65536 tokens, 8 heads per kv head: 119 us, 123 with a store per tile.
+    const int per_tile = 8 * heads, ring_tiles = kRing / per_tile;
+    int ring_used = 0;
+    uint32_t ring_first = 0;  // key of the first tile in the ring
+    const auto flush = [&]() {
+        f32x4* to = reinterpret_cast<f32x4*>(a.scores) +
+                    (int64_t)(seg.seq * a.kv_heads + seg.kv_head) * (a.score_row / 4) * a.group + seg.tile * kColumns;
+        for (int i = lane; i < ring_used * per_tile; i += kWave) {
+            const int four = i / heads, tile = four >> 3;  // four keys, of 8 in a tile
+            to[(int64_t)((ring_first + tile * kRound) / 4 + (four & 7)) * a.group + (i - four * heads)] = lds.ring[SCORES ? wave : 0][i];
+        }
+        ring_used = 0;
+    };
 
     u32x4 q[S::kChunks], k[2][S::kChunks], v[2][S::kChunks];
     f32x4 acc[S::kDimTiles];
@@ -475,7 +514,7 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
 #pragma unroll
     for (int c = 0; c < S::kChunks; ++c) {
         q[c] = u32x4{0u, 0u, 0u, 0u};
-        if (live && (D == S::kDim || (4 * c + g) * 8 < D))
+        if (D == S::kDim || (4 * c + g) * 8 < D)
             q[c] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.query) + head * D + (4 * c + g) * 8);
     }
 #pragma unroll 1
@@ -493,8 +532,17 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < S::kChunks; ++i)
-                *reinterpret_cast<u32x4*>(keys_lds + lines.to[i] + 16 * s * 2 * S::kDim) = k[s][i];
+                *reinterpret_cast<u32x4*>(tile_lds + lines.to[i] + 16 * s * 2 * S::kDim) = k[s][i];
         load_tile<D, RUN>(k, a.key, next, lines, a.row_bytes);
+        f32x4 x[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+                x[s] = T::mfma16x16x32(*reinterpret_cast<const u32x4*>(tile_lds + key_at.chunk(4 * c) + 16 * s * 2 * S::kDim),
+                                       q[c], x[s]);
+        }
         // Keys that are not there: no weight, and zeros as values (0 * NaN is NaN).
         if (present != 0xffffffffu) {
 #pragma unroll
@@ -508,17 +556,8 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
         for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < S::kChunks; ++i)
-                *reinterpret_cast<u32x4*>(values_lds + lines.to[i] + 16 * s * 2 * S::kDim) = v[s][i];
+                *reinterpret_cast<u32x4*>(tile_lds + lines.to[i] + 16 * s * 2 * S::kDim) = v[s][i];
         load_tile<D, RUN>(v, a.value, next, lines, a.row_bytes);
-        f32x4 x[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < S::kChunks; ++c)
-                x[s] = T::mfma16x16x32(*reinterpret_cast<const u32x4*>(keys_lds + key_at.chunk(4 * c) + 16 * s * 2 * S::kDim),
-                                       q[c], x[s]);
-        }
         if (present != 0xffffffffu) {
 #pragma unroll
             for (int s = 0; s < 2; ++s)
@@ -526,12 +565,15 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
                 for (int j = 0; j < 4; ++j) x[s][j] = (present >> (16 * s + 4 * g + j)) & 1 ? x[s][j] : kNegInf;
         }
         if constexpr (SCORES) {
-            // (Behind the context there is room up to the row's end: rows are a multiple of 32 long.)
+            // Four keys of every head side by side.  (Behind the context there is room: rows are a multiple of 32.)
+            if (ring_used == 0) ring_first = t0;
+            f32x4* to = lds.ring[wave] + ring_used * per_tile + g * heads + r;
             if (live) {
-                float* to = a.scores + head * a.score_row + t0 + 4 * g;
-                *reinterpret_cast<f32x4*>(to) = x[0];
-                *reinterpret_cast<f32x4*>(to + 16) = x[1];
+                to[0] = x[0];
+                to[4 * heads] = x[1];
             }
+            ++ring_used;
+            if (SCORES == kStoreScores && ring_used == ring_tiles) flush();
         }
         float top = fmaxf(x[0][0], x[1][0]);
 #pragma unroll
@@ -561,16 +603,17 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
             }
 #pragma unroll
         for (int n = 0; n < S::kDimTiles; ++n) {
-            const u32x4 vt = value_operand(values_lds, value_at.chunk(2 * n), value_at.chunk(2 * n) + 16 * 2 * S::kDim);
+            const u32x4 vt = value_operand(tile_lds, value_at.chunk(2 * n), value_at.chunk(2 * n) + 16 * 2 * S::kDim);
             acc[n] = T::mfma16x16x32(vt, high, acc[n]);
             acc[n] = T::mfma16x16x32(vt, low, acc[n]);
         }
         now = next;
     }
+    if constexpr (SCORES == kStoreScores) flush();
     sum = row4_sum(sum);
 
     // Join the waves: sums [16][D] in their tiles' LDS, each relative to its own reference.
-    float* mine = reinterpret_cast<float*>(keys_lds);
+    float* mine = reinterpret_cast<float*>(tile_lds);
     if (live) {
 #pragma unroll
         for (int n = 0; n < S::kDimTiles; ++n) *reinterpret_cast<f32x4*>(mine + r * S::kDim + 16 * n + 4 * g) = acc[n];
@@ -590,14 +633,18 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
         for (int w = 0; w < kWaves; ++w) {
             const float by = fast_exp2(lds.stats[w][0][h] - top);
             total += by * lds.stats[w][1][h];
-            value += by * reinterpret_cast<const float*>(lds.tiles[w][0])[h * S::kDim + d];
+            value += by * reinterpret_cast<const float*>(lds.tiles[w])[h * S::kDim + d];
         }
         if (seg.slot < 0) {
             const int64_t to = head_of(a, seg, seg.tile * kColumns + h);
             static_cast<uint16_t*>(a.out)[to * D + d] = T::from_float(total != 0.f ? value / total : 0.f);
-            if (SCORES && d == 0) {
+            if (SCORES == kStoreScores && d == 0) {
                 a.totals[to * 2] = top;
                 a.totals[to * 2 + 1] = total;
+            }
+            if (SCORES == kAddWeights && d == 0) {
+                lds.divisors[0][h] = top;
+                lds.divisors[1][h] = total != 0.f ? 1.f / total : 0.f;
             }
         } else if (seg.slot < a.narrow_slots) {
             const int64_t slot = (int64_t)seg.slot * kColumns + h;
@@ -610,6 +657,21 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
         }
     }
     __syncthreads();  // the tiles are free again
+    if constexpr (SCORES == kAddWeights) {
+        float* weights = a.weights + ((int64_t)seg.seq * a.kv_heads + seg.kv_head) * a.weight_row;
+        for (uint32_t key = 4 * threadIdx.x; key < seg.end; key += 4 * kThreads) {
+            const uint32_t tile = key / kTileKeys;
+            const f32x4* s = lds.ring[tile % kWaves] + (tile / kWaves * 8 + key / 4 % 8) * heads;
+            f32x4 add = {0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < heads; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    add[i] += fast_exp2(__builtin_fmaf(s[h][i], a.scale, -lds.divisors[0][h])) * lds.divisors[1][h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (key + i < seg.end) weights[key + i] += add[i];
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -668,7 +730,7 @@ struct Join {
             const int64_t row = (int64_t)(seq - x.first) * a.group + head;
             const int per = x.wide ? kWideRows : kColumns, tile = (int)(row / per);
             const int at = kv_head * w.total + group_base + tile * x.rounds;
-            const int first = at / w.share, last = (at + x.rounds - 1) / w.share;
+            const int first = w.owner(at), last = w.owner(at + x.rounds - 1);
             if (x.wide) {
                 p.wide_slot = kv_head * w.wide_units + group_unit + tile + first;
                 p.wide_count = last - first + 1;
@@ -683,7 +745,7 @@ struct Join {
         if (rounds > 0) {
             const int tile = head / kColumns;
             const int at = kv_head * w.total + own_base + tile * rounds;
-            const int first = at / w.share, last = (at + rounds - 1) / w.share;
+            const int first = w.owner(at), last = w.owner(at + rounds - 1);
             if (own.start == 0 && first == last) return false;
             p.own_slot = kv_head * units + w.narrow_units + seq * a.head_tiles + tile + first;
             p.own_count = last - first + 1;

@@ -15,13 +15,6 @@ __device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Barrier of the work-group for LDS alone: loads from memory stay in flight.
-__device__ inline void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 template <int D>
 struct WideLds {
     uint8_t tiles[2][2][Shape<D>::kWidePlane];  // [buffer][keys, values]
@@ -214,19 +207,18 @@ template <typename T, int D, int RUN>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void shared_prefix_kernel(Args a) {
     __shared__ __attribute__((aligned(16))) union Lds {
         WideLds<D> wide;
-        NarrowLds<D> narrow;
+        NarrowLds<D, kNoScores> narrow;
     } lds;
     Walk w;
     w.count(a);
-    const int all = w.total * a.kv_heads;
-    const int first = (int)min((int64_t)blockIdx.x * w.share, (int64_t)all);
-    const int stop = (int)min((int64_t)first + w.share, (int64_t)all);
+    if ((int)blockIdx.x >= w.total * a.kv_heads) return;
+    const int first = w.first_of(blockIdx.x), stop = w.first_of(blockIdx.x + 1);
 #pragma unroll 1
     for (int at = first; at < stop;) {
         const Segment s = find_segment(a, w, at, stop);
         at += s.rounds;
         if (s.wide) wide_segment<T, D, RUN>(a, s, lds.wide);
-        else narrow_segment<T, D, RUN, false>(a, s, lds.narrow);
+        else narrow_segment<T, D, RUN, kNoScores>(a, s, lds.narrow);
     }
 }
 
@@ -236,6 +228,16 @@ __global__ __launch_bounds__(kThreads) void shared_prefix_join_kernel(Args a) {
 }
 
 int work_groups(int64_t head_dim) { return head_dim <= 128 ? 512 : 256; }
+
+// Calls whose keys and values, each sequence's on its own, are this little are attended without regard to the groups: up
+// to there reading a prefix again costs less than the pieces and their join.  Sequences of a prefix and 100 tokens more, 16
+// heads on 8, alone and shared, us: 8 x 1024 9.7 and 14.3, 4 x 4096 (67 MB) 16.1 and 15.3, 16 x 1024 12.4 and 14.3, 32 x
+// 1024 (134 MB) 17.7 and 18.0, 16 x 2048 17.4 and 16.0, 64 x 1024 (268 MB) 25.6 and 20.7.
+constexpr int64_t kAloneBytes = 96 << 20;
+bool alone(int64_t batch, int64_t kv_heads, int64_t head_dim, int64_t groups, int64_t capacity, int always) {
+    if (always) return false;
+    return groups == 0 || batch * capacity <= kAloneBytes / (kv_heads * head_dim * 4);
+}
 
 struct Sizes {
     int64_t shares, wide_slots, narrow_slots;
@@ -287,10 +289,13 @@ using namespace mvme;
 using namespace mvme::lng;
 
 extern "C" size_t mvme_paged_attention_shared_prefix_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
-                                                                    int64_t head_dim, int64_t groups) {
-    if (batch <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || !head_dim_built(head_dim) || groups < 0 ||
-        groups > batch || batch > kMostBatchHeads / q_heads)
+                                                                    int64_t head_dim, int64_t groups, int64_t block_size,
+                                                                    int64_t table_width, int always) {
+    Args a{};
+    if (check_shape(a, batch, q_heads, kv_heads, head_dim, 1, block_size, table_width, MVME_FP16) || groups < 0 || groups > batch)
         return 0;
+    if (alone(batch, kv_heads, head_dim, groups, block_size * table_width, always))
+        return mvme_paged_attention_workspace_size(batch, q_heads, kv_heads, head_dim, block_size, table_width, 0);
     return sizes(batch, q_heads, kv_heads, head_dim, groups).bytes;
 }
 
@@ -299,8 +304,8 @@ extern "C" int mvme_paged_attention_shared_prefix(void* out, const void* query, 
                                                   const int64_t* context_lens, const int64_t* group_offsets,
                                                   const int64_t* prefix_lens, int64_t batch, int64_t groups,
                                                   int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                                                  int64_t num_blocks, int64_t block_size, int64_t table_width, int dtype,
-                                                  void* workspace, size_t workspace_bytes, void* stream) {
+                                                  int64_t num_blocks, int64_t block_size, int64_t table_width, int always,
+                                                  int dtype, void* workspace, size_t workspace_bytes, void* stream) {
     Args a{};
     if (int rc = check_shape(a, batch, q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, dtype)) return rc;
     if (groups < 0 || groups > batch) return fail(MVME_EINVAL, "groups must be between none and one per sequence");
@@ -308,6 +313,9 @@ extern "C" int mvme_paged_attention_shared_prefix(void* out, const void* query, 
         return fail(MVME_EINVAL, "shared-prefix attention: null pointer");
     if (!fp4::aligned(query, 16) || !fp4::aligned(key_cache, 16) || !fp4::aligned(value_cache, 16) || !fp4::aligned(out, 8))
         return fail(MVME_EINVAL, "shared-prefix attention: queries and caches must be 16-byte, the output 8-byte aligned");
+    if (alone(batch, kv_heads, head_dim, groups, block_size * table_width, always))
+        return mvme_paged_attention(out, query, key_cache, value_cache, block_tables, context_lens, batch, q_heads, kv_heads,
+                                    head_dim, num_blocks, block_size, table_width, 0, dtype, workspace, workspace_bytes, stream);
     const Sizes s = sizes(batch, q_heads, kv_heads, head_dim, groups);
     if (!workspace || workspace_bytes < s.bytes || !fp4::aligned(workspace, 16))
         return fail(MVME_EWORKSPACE, "shared-prefix workspace too small: " + std::to_string(s.bytes) +

@@ -75,8 +75,8 @@ PACKED_SIGNATURES = {
 
 # The operators for long contexts; mirrors include/mvme_long.h.
 LONG_SIGNATURES = {
-    "mvme_paged_attention_shared_prefix_workspace_size": (_size, [_i64] * 5),
-    "mvme_paged_attention_shared_prefix": (_int, [_vp] * 8 + [_i64] * 8 + [_int, _vp, _size, _vp]),
+    "mvme_paged_attention_shared_prefix_workspace_size": (_size, [_i64] * 7 + [_int]),
+    "mvme_paged_attention_shared_prefix": (_int, [_vp] * 8 + [_i64] * 8 + [_int, _int, _vp, _size, _vp]),
     "mvme_paged_attention_weights_workspace_size": (_size, [_i64] * 6),
     "mvme_paged_attention_weights": (_int, [_vp] * 7 + [_i64] * 8 + [_int, _vp, _size, _vp]),
     "mvme_prefill_attention_weights_workspace_size": (_size, [_i64] * 7),

@@ -25,6 +25,8 @@ def dense_rows(query):
 
 def take_workspace(workspace, need, device):
     """(address, bytes, owner) of the caller's workspace, or of a new one."""
+    if workspace is None and not need:
+        return None, 0, None
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     else:
@@ -41,9 +43,11 @@ def check_output(out, query, others):
     _check(out.data_ptr() % 8 == 0, "output buffer must be 8-byte aligned")
 
 
-def shared_prefix_workspace_bytes(batch, q_heads, kv_heads, head_dim, groups):
-    """Bytes of the workspace paged_attention_shared_prefix needs for these shapes."""
-    return ext.load_hip_extension().shared_prefix_workspace_size(batch, q_heads, kv_heads, head_dim, groups)
+def shared_prefix_workspace_bytes(batch, q_heads, kv_heads, head_dim, groups, block_size, table_width,
+                                  always_share=False):
+    """Bytes of the workspace paged_attention_shared_prefix needs for these shapes (0: none)."""
+    return ext.load_hip_extension().shared_prefix_workspace_size(batch, q_heads, kv_heads, head_dim, groups, block_size,
+                                                                 table_width, int(always_share))
 
 
 def _check_groups(tables, lengths, offsets, prefixes, block_size):
@@ -63,7 +67,8 @@ def _check_groups(tables, lengths, offsets, prefixes, block_size):
 
 
 def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, context_lens, block_size, group_offsets,
-                                  prefix_lens, *, backend="hip", validate=True, out=None, workspace=None):
+                                  prefix_lens, *, backend="hip", validate=True, always_share=False, out=None,
+                                  workspace=None):
     """``paged_attention`` for a batch in which sequences share prefixes.
 
     The first six arguments are those of ``paged_attention`` (full block tables
@@ -72,7 +77,8 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, c
     what is in no group shares nothing) hold their first ``prefix_lens[g]``
     tokens (int64 [groups]) in the same pages, which are read through the first
     one's table.  A sequence shorter than its group's prefix is attended on its
-    own.  ``validate=True`` reads the metadata on the host, and refuses groups
+    own.  Calls of few cached tokens run ``paged_attention``'s kernels, which
+    are ahead there, unless ``always_share``.  ``validate=True`` reads the metadata on the host, and refuses groups
     whose pages differ; with ``validate=False`` (graph capture) the caller
     answers for that, lengths and pages that cannot be are absent, and offsets
     that cannot be leave every sequence on its own.  ``out`` / ``workspace``
@@ -80,7 +86,7 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, c
     """
     if backend != "hip":
         raise ValueError("decode backend must be hip")
-    if not validate and out is None and workspace is None:
+    if not validate and not always_share and out is None and workspace is None:
         result = ext.native.shared_prefix(query, key_cache, value_cache, block_tables, context_lens, block_size,
                                           group_offsets, prefix_lens)
         if result is not None:
@@ -108,12 +114,13 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, c
                                   workspace))
     query = dense_rows(query)
     lib = ext.load_hip_extension()
-    need = lib.shared_prefix_workspace_size(batch, q_heads, kv_heads, head_dim, groups)
+    need = lib.shared_prefix_workspace_size(batch, q_heads, kv_heads, head_dim, groups, block_size,
+                                            block_tables.shape[1], int(bool(always_share)))
     with torch.cuda.device(query.device):
         ws_ptr, ws_bytes, workspace = take_workspace(workspace, need, query.device)
         lib.call("mvme_paged_attention_shared_prefix", out.data_ptr(), query.data_ptr(), key_cache.data_ptr(),
                  value_cache.data_ptr(), block_tables.data_ptr(), context_lens.data_ptr(), group_offsets.data_ptr(),
                  prefix_lens.data_ptr(), batch, groups, q_heads, kv_heads, head_dim, num_blocks, block_size,
-                 block_tables.shape[1], ext.dtype_code(query.dtype), ws_ptr, ws_bytes,
+                 block_tables.shape[1], int(bool(always_share)), ext.dtype_code(query.dtype), ws_ptr, ws_bytes,
                  ext.current_stream(query.device))
     return out

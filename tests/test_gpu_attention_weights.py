@@ -81,8 +81,8 @@ def test_step_probabilities_add_up_over_steps():
 
 
 def test_step_repeats_bit_for_bit_in_graphs_that_share_a_workspace():
-    a, b = step_case(4, [900, 30, 2500]), step_case(5, [64] * 40, heads=8, kv=8)
-    need = max(weights_workspace_bytes(3, 16, 8, 128, 16, a[3].shape[1]), weights_workspace_bytes(40, 8, 8, 128, 16, 4))
+    a, b = step_case(4, [900, 30, 2500]), step_case(5, [1000] * 9, heads=8, kv=8)
+    need = max(weights_workspace_bytes(3, 16, 8, 128, 16, a[3].shape[1]), weights_workspace_bytes(9, 8, 8, 128, 16, 63))
     ws = torch.empty(need, dtype=torch.uint8, device=DEV)
     start = [x[6].clone() for x in (a, b)]
     want = []
@@ -108,13 +108,13 @@ def test_step_repeats_bit_for_bit_in_graphs_that_share_a_workspace():
 
 
 def test_step_buffers_and_refusals():
-    args = step_case(7, [100, 200])
+    args = step_case(7, [100, 600])
     start = args[6].clone()
     want = paged_attention_weights(*args)
     after = args[6].clone()
     args[6].copy_(start)
     out = torch.empty_like(want)
-    ws = torch.full((weights_workspace_bytes(2, 16, 8, 128, 16, 13),), 255, dtype=torch.uint8, device=DEV)
+    ws = torch.full((weights_workspace_bytes(2, 16, 8, 128, 16, 38),), 255, dtype=torch.uint8, device=DEV)
     assert paged_attention_weights(*args, out=out, workspace=ws) is out
     assert torch.equal(out, want) and torch.equal(args[6], after)
     with pytest.raises(RuntimeError, match="workspace too small"):
@@ -122,7 +122,7 @@ def test_step_buffers_and_refusals():
     with pytest.raises(ValueError, match="FP32"):
         paged_attention_weights(*args[:6], args[6].half(), validate=False)
     with pytest.raises(ValueError, match="capacity"):
-        paged_attention_weights(*args[:6], args[6][..., :100].contiguous(), validate=False)
+        paged_attention_weights(*args[:6], args[6][..., :600].contiguous(), validate=False)
     with pytest.raises(RuntimeError, match="overlap"):
         paged_attention_weights(*args, out=args[0], validate=False)
     assert torch.equal(args[6], after)

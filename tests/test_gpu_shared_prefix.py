@@ -1,4 +1,10 @@
-"""Shared-prefix decode attention on the GPU against float64."""
+"""Shared-prefix decode attention on the GPU against float64.
+
+The calls are small, and so are made to share (``shared``); ``test_small_calls``
+has the form that leaves it to the library.
+"""
+
+import functools
 
 import pytest
 import torch
@@ -10,6 +16,7 @@ from mini_engine_hip.kernels.shared import paged_attention_shared_prefix, shared
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+shared = functools.partial(paged_attention_shared_prefix, always_share=True)
 
 
 def case(seed, lens, groups, *, heads=16, kv=8, dim=128, block=16, dtype=torch.bfloat16, pad=0, poison=True):
@@ -31,7 +38,7 @@ def case(seed, lens, groups, *, heads=16, kv=8, dim=128, block=16, dtype=torch.b
 
 
 def check(args, **kw):
-    out = paged_attention_shared_prefix(*args, **kw)
+    out = shared(*args, **kw)
     query, key, value, tables, lens, block = args[:6]
     # (Where a prefix has more than 32 rows its probabilities are rounded once to the type.)
     want, bound, _, _ = lc.decode(query, key, value, tables, lens.tolist(), block, lc.HALF_STEP[query.dtype])
@@ -102,7 +109,7 @@ def test_absent_pages_are_skipped():
     args[3] = tables
     check(args, validate=False)
     tables[:] = -1
-    assert not paged_attention_shared_prefix(*args, validate=False).any()
+    assert not shared(*args, validate=False).any()
 
 
 def test_offsets_that_cannot_be_leave_sequences_on_their_own():
@@ -129,14 +136,14 @@ def test_large_scores_and_infinite_values():
     # size differ by more than 104, where exp() of the difference is 0 in fp32, and 0 times infinity is NaN.)
     page = int(args[3][7, 16])
     args[2][page, 3, 0, 5] = float("inf")
-    out = paged_attention_shared_prefix(*args)
+    out = shared(*args)
     assert not torch.isfinite(out[7, :2, 5]).any() and torch.isfinite(out[:7]).all() and torch.isfinite(out[8:]).all()
 
 
 def test_nan_of_one_sequence_stays_there():
     args = list(case(10, [300] * 20 + [200] * 3, [(0, 20, 256)]))
     args[1][int(args[3][4, 16]), 2, 1] = float("nan")
-    out = paged_attention_shared_prefix(*args)
+    out = shared(*args)
     assert torch.isnan(out[4, 2:4]).all()
     out[4, 2:4] = 0
     assert torch.isfinite(out).all()
@@ -144,30 +151,30 @@ def test_nan_of_one_sequence_stays_there():
 
 def test_results_do_not_change_from_call_to_call():
     args = case(11, [700 + 13 * i for i in range(50)], [(0, 50, 640)])
-    first = paged_attention_shared_prefix(*args)
+    first = shared(*args)
     for _ in range(5):
-        assert torch.equal(paged_attention_shared_prefix(*args, validate=False), first)
+        assert torch.equal(shared(*args, validate=False), first)
 
 
 def test_buffers_and_strange_alignment():
     args = list(case(12, [300] * 5, [(0, 5, 256)]))
-    want = paged_attention_shared_prefix(*args)
-    need = shared_prefix_workspace_bytes(5, 16, 8, 128, 1)
+    want = shared(*args)
+    need = shared_prefix_workspace_bytes(5, 16, 8, 128, 1, 16, 19, True)
     ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
     out = torch.empty_like(want)
-    assert paged_attention_shared_prefix(*args, out=out, workspace=ws) is out and torch.equal(out, want)
+    assert shared(*args, out=out, workspace=ws) is out and torch.equal(out, want)
     flat = torch.empty(args[0].numel() + 1, dtype=args[0].dtype, device=DEV)
     flat[1:] = args[0].flatten()
     args[0] = flat[1:].view(args[0].shape)
-    assert torch.equal(paged_attention_shared_prefix(*args), want)
-    assert torch.equal(paged_attention_shared_prefix(*args, validate=False), want)
+    assert torch.equal(shared(*args), want)
+    assert torch.equal(shared(*args, validate=False), want)
     with pytest.raises(RuntimeError, match="workspace too small"):
-        paged_attention_shared_prefix(*args, workspace=ws[:need - 16])
+        shared(*args, workspace=ws[:need - 16])
     with pytest.raises(RuntimeError, match="overlap"):
-        paged_attention_shared_prefix(*args, out=args[0])
+        shared(*args, out=args[0])
     flat = torch.empty(args[1].numel() + 1, dtype=args[1].dtype, device=DEV)
     with pytest.raises(RuntimeError, match="aligned"):
-        paged_attention_shared_prefix(args[0], flat[1:].view(args[1].shape), *args[2:], validate=False)
+        shared(args[0], flat[1:].view(args[1].shape), *args[2:], validate=False)
 
 
 def test_pages_past_four_gigabytes():
@@ -190,11 +197,11 @@ def test_graph_follows_its_metadata():
     batch = 24
     args = list(case(14, [600] * batch, [(0, batch, 512)], pad=3, poison=False))
     tables, lens, offsets, prefixes = args[3], args[4], args[6], args[7]
-    paged_attention_shared_prefix(*args, validate=False)
+    shared(*args, validate=False)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        out = paged_attention_shared_prefix(*args, validate=False)
+        out = shared(*args, validate=False)
     original = tables.clone()
     for n, last, prefix in ((600, 24, 512), (520, 24, 512), (601, 9, 256), (513, 0, 0), (600, 24, 64)):
         lens.fill_(n)
@@ -206,23 +213,40 @@ def test_graph_follows_its_metadata():
         torch.cuda.synchronize()
         want, bound, _, _ = lc.decode(*args[:4], lens.tolist(), args[5], 2.0 ** -8)
         lc.assert_within(out, want, bound)
-        assert torch.equal(out, paged_attention_shared_prefix(*args, validate=False))
+        assert torch.equal(out, shared(*args, validate=False))
 
 
 def test_two_streams_at_once():
     args = case(15, [900 + i for i in range(40)], [(0, 40, 896)])
     other = case(16, [300 + i for i in range(10)], [(0, 10, 256)], heads=8, kv=8, dim=64)
-    want = [paged_attention_shared_prefix(*a) for a in (args, other)]
+    want = [shared(*a) for a in (args, other)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
     outs = []
     for _ in range(4):
         for a, stream in zip((args, other), streams):
             with torch.cuda.stream(stream):
-                outs.append(paged_attention_shared_prefix(*a, validate=False))
+                outs.append(shared(*a, validate=False))
     torch.cuda.synchronize()
     for i, out in enumerate(outs):
         assert torch.equal(out, want[i % 2])
+
+
+def test_small_calls():
+    args = list(case(18, [300, 0, 290, 17], [(0, 3, 256)]))
+    want, bound, _, _ = lc.decode(*args[:4], args[4].tolist(), 16, 2.0 ** -8)
+    out = paged_attention_shared_prefix(*args, validate=False)
+    lc.assert_within(out, want, bound)
+    assert torch.equal(out, paged_attention(*args[:6], validate=False))
+    assert torch.equal(out, paged_attention_shared_prefix(*args, validate=False, out=torch.empty_like(out)))
+
+
+def test_large_calls_share_by_themselves():
+    batch = 48
+    args = case(19, [4096 + 30 + b for b in range(batch)], [(0, batch, 4096)])
+    out = paged_attention_shared_prefix(*args, validate=False)
+    assert torch.equal(out, shared(*args))
+    check(args)
 
 
 def test_forked_requests():
