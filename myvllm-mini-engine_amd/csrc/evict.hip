@@ -38,7 +38,7 @@ __device__ inline int length(const Args& a, int seq) {
 // ---------------------------------------------------------------------------
 // The choice: one work-group per layer, sequence and kv head.
 // ---------------------------------------------------------------------------
-constexpr int kSelect = 1024, kSelectWaves = kSelect / kWave;
+constexpr int kCopies = 8;  // of the histogram: weights fall into few bins, and lanes that meet in one wait for each other
 
 // Weights in their order as unsigned numbers: NaN above all, -0 equal to +0.
 __device__ inline uint32_t rank_of(float x) {
@@ -48,7 +48,8 @@ __device__ inline uint32_t rank_of(float x) {
 }
 
 // Exclusive prefix over the work-group of two counts, and their totals.
-__device__ inline void scan_pair(int x, int y, int& before_x, int& before_y, int& all_x, int& all_y, int (*sums)[2]) {
+__device__ inline void scan_pair(int x, int y, int& before_x, int& before_y, int& all_x, int& all_y, int (*sums)[2],
+                                 int waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int ix = wave_incl_scan(x), iy = wave_incl_scan(y);
     if (lane == kWave - 1) {
@@ -59,7 +60,7 @@ __device__ inline void scan_pair(int x, int y, int& before_x, int& before_y, int
     before_x = ix - x;
     before_y = iy - y;
     all_x = all_y = 0;
-    for (int w = 0; w < kSelectWaves; ++w) {
+    for (int w = 0; w < waves; ++w) {
         if (w < wave) {
             before_x += sums[w][0];
             before_y += sums[w][1];
@@ -70,9 +71,11 @@ __device__ inline void scan_pair(int x, int y, int& before_x, int& before_y, int
     __syncthreads();
 }
 
+template <int kSelect>
 __global__ __launch_bounds__(kSelect) void choose_kernel(Args a) {
-    __shared__ int histogram[256];
-    __shared__ int sums[kSelectWaves][2];
+    constexpr int kWaves = kSelect / kWave;
+    __shared__ int histogram[256][kCopies];
+    __shared__ int sums[kWaves][2];
     __shared__ uint32_t chosen[2];
     const int64_t line = blockIdx.x;
     const int seq = (int)(line / a.kv_heads % a.batch);
@@ -101,17 +104,20 @@ __global__ __launch_bounds__(kSelect) void choose_kernel(Args a) {
     uint32_t prefix = 0, mask = 0;
     if (want > 0) {
         for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = threadIdx.x; i < 256; i += kSelect) histogram[i] = 0;
+            for (int i = threadIdx.x; i < 256 * kCopies; i += kSelect) histogram[i / kCopies][i % kCopies] = 0;
             __syncthreads();
             for (int i = first + threadIdx.x; i < stop; i += kSelect) {
                 const uint32_t rank = rank_of(w[i]);
-                if ((rank & mask) == prefix) atomicAdd(&histogram[(rank >> shift) & 255], 1);
+                if ((rank & mask) == prefix) atomicAdd(&histogram[(rank >> shift) & 255][threadIdx.x % kCopies], 1);
             }
             __syncthreads();
             // Bin 255 - t of thread t: the one in which the count from above reaches want.
-            const int mine = threadIdx.x < 256 ? histogram[255 - threadIdx.x] : 0;
+            int mine = 0;
+            if (threadIdx.x < 256)
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) mine += histogram[255 - threadIdx.x][i];
             int upto = wave_incl_scan(mine);
-            if ((threadIdx.x & 63) == 63) sums[threadIdx.x >> 6][0] = upto;
+            if ((threadIdx.x & 63) == 63 && threadIdx.x < 256) sums[threadIdx.x >> 6][0] = upto;
             __syncthreads();
             if (threadIdx.x < 256) {
                 for (int k = 0; k < (int)(threadIdx.x >> 6); ++k) upto += sums[k][0];
@@ -143,7 +149,7 @@ __global__ __launch_bounds__(kSelect) void choose_kernel(Args a) {
             }
         }
         int before_above, before_level, all_above, all_level;
-        scan_pair(is_above, is_level, before_above, before_level, all_above, all_level, sums);
+        scan_pair(is_above, is_level, before_above, before_level, all_above, all_level, sums, kWaves);
         const int levels = level + before_level;
         if (is_above || (is_level && levels < want)) {
             const int to = above + before_above + min(levels, want);
@@ -163,7 +169,7 @@ __global__ __launch_bounds__(kSelect) void choose_kernel(Args a) {
 constexpr int kMove = 256, kPasses = 8;
 
 __global__ __launch_bounds__(kMove) void move_kernel(Args a) {
-    __shared__ int64_t from[kMove], to[kMove];
+    __shared__ int64_t from[2][kMove], to[2][kMove];
     int64_t item = blockIdx.x;
     const int slice = (int)(item % a.slices);
     item /= a.slices;
@@ -186,35 +192,42 @@ __global__ __launch_bounds__(kMove) void move_kernel(Args a) {
                    ? (int64_t)((uint64_t)page * a.page_bytes + (uint64_t)(token - block * a.div.size) * a.row_bytes)
                    : (int64_t)-1;
     };
-    for (int i0 = 0; i0 < count; i0 += a.rows) {
-        if ((int)threadIdx.x < a.rows) {
-            const int i = i0 + threadIdx.x;
-            int64_t f = -1, t = -1;
-            if (i < count) {
-                const int64_t source = kept[i];
-                if (source != i) {
-                    f = place_of((uint32_t)source);
-                    t = place_of((uint32_t)i);
-                }
+    // This thread's row of a pass: where it comes from and goes to, -1 if it does not move.
+    int64_t f, t;
+    const auto look_up = [&](int i0) {
+        const int i = i0 + threadIdx.x;
+        f = t = -1;
+        if ((int)threadIdx.x < a.rows && i < count) {
+            const int64_t source = kept[i];
+            if (source != i) {
+                f = place_of((uint32_t)source);
+                t = f < 0 ? -1 : place_of((uint32_t)i);
             }
-            from[threadIdx.x] = f;
-            to[threadIdx.x] = f < 0 ? -1 : t;
+        }
+    };
+    look_up(0);
+    for (int i0 = 0, buffer = 0; i0 < count; i0 += a.rows, buffer ^= 1) {
+        if ((int)threadIdx.x < a.rows) {
+            from[buffer][threadIdx.x] = f;
+            to[buffer][threadIdx.x] = t;
         }
         __syncthreads();
         u32x4 x[kPasses];
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
             const int r = p * per + side;
-            if (side < per && r < a.rows && to[r] >= 0) x[p] = *reinterpret_cast<const u32x4*>(plane + from[r] + unit * 16);
+            if (side < per && r < a.rows && to[buffer][r] >= 0)
+                x[p] = *reinterpret_cast<const u32x4*>(plane + from[buffer][r] + unit * 16);
         }
+        look_up(i0 + a.rows);
         __builtin_amdgcn_s_waitcnt(0);  // every row of the pass is in registers
         __syncthreads();
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
             const int r = p * per + side;
-            if (side < per && r < a.rows && to[r] >= 0) *reinterpret_cast<u32x4*>(plane + to[r] + unit * 16) = x[p];
+            if (side < per && r < a.rows && to[buffer][r] >= 0)
+                *reinterpret_cast<u32x4*>(plane + to[buffer][r] + unit * 16) = x[p];
         }
-        __syncthreads();  // (the places are free again)
     }
 }
 
@@ -242,8 +255,8 @@ extern "C" int mvme_evict_kv_cache(void* key_cache, void* value_cache, const flo
     if (kv_heads > 65536 || num_blocks > 2147483647 || num_blocks > (int64_t(1) << 62) / row / block_size / layers)
         return fail(MVME_EINVAL, "KV cache too large");
     if (batch > 2147483647 || layers > 2147483647) return fail(MVME_EINVAL, "batch/head product too large");
-    const int64_t lines = layers * batch, most = kMostThreads / kSelect / 64;
-    if (lines > most / kv_heads) return fail(MVME_EINVAL, "batch/head product too large");
+    const int64_t lines = layers * batch, most = kMostThreads / 1024 / 64;
+    if (lines > most / kv_heads / 16) return fail(MVME_EINVAL, "batch/head product too large");
     if (!key_cache || !value_cache || !weights || !new_weights || !kept || !new_lens || !block_tables || !context_lens)
         return fail(MVME_EINVAL, "eviction: null pointer");
     if (!fp4::aligned(key_cache, 16) || !fp4::aligned(value_cache, 16)) return fail(MVME_EINVAL, "eviction: caches must be 16-byte aligned");
@@ -271,12 +284,20 @@ extern "C" int mvme_evict_kv_cache(void* key_cache, void* value_cache, const flo
     a.width = (int)table_width;
     a.div = fp4::make_block_div(block_size);
     a.slices = 1;
-    a.slice_bytes = (int)(head_dim * 2);
+    // Rows are cut where a work-group per row of a head leaves compute units without one; no further, since pieces of rows
+    // are slower to move (us: 16 sequences, one layer, 20.6 in halves and 25 whole; 28 layers of one sequence 235 whole, 288
+    // in halves).
+    while (lines * kv_heads * 2 * a.slices < 400 && head_dim * 2 / a.slices % 128 == 0) a.slices *= 2;
+    a.slice_bytes = (int)(head_dim * 2 / a.slices);
     a.units = a.slice_bytes / 16;
     const int per = kMove / a.units;
     a.rows = per * kPasses < kMove ? per * kPasses : kMove;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(choose_kernel, dim3((unsigned)(lines * kv_heads)), dim3(kSelect), 0, s, a);
+    // 512 threads choose sooner among few tokens, 1024 among many.
+    if (block_size * table_width <= 8192)
+        hipLaunchKernelGGL((choose_kernel<512>), dim3((unsigned)(lines * kv_heads)), dim3(512), 0, s, a);
+    else
+        hipLaunchKernelGGL((choose_kernel<1024>), dim3((unsigned)(lines * kv_heads)), dim3(1024), 0, s, a);
     if (int rc = check_launch("eviction choice")) return rc;
     hipLaunchKernelGGL(move_kernel, dim3((unsigned)(lines * kv_heads * 2 * a.slices)), dim3(kMove), 0, s, a);
     return check_launch("eviction moves");

@@ -14,6 +14,8 @@ namespace mvme {
 namespace lng {
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 constexpr int kRows = 128;     // query rows of a work-group of the first pass
 constexpr int kTile = 64;      // keys (first pass) or rows (second) of a tile in LDS
 constexpr int kKeys = 128;     // keys of a work-group of the second pass
@@ -26,15 +28,16 @@ struct PromptArgs {
     const int64_t* tables;
     const int64_t* lens;
     float* partial;   // [total_tokens, q_heads, chunks, 2]: (reference, sum) of a chunk's keys
-    float* rows;      // [total_tokens, q_heads, 2]: (reference, 1 / sum)
+    float* received;  // [parts, num_seqs, kv_heads, key_blocks, kKeys]: what the rows of a part give (several parts only)
     float* weights;   // [num_seqs, kv_heads, weight_row]
     int64_t weight_row;
     int64_t num_blocks, total_tokens;
     uint64_t page_bytes;
     uint32_t row_bytes;
     int num_seqs, kv_heads, q_heads, group, width;
-    int items, chunks, chunk_len, key_blocks;
-    BlockDiv div, group_div;
+    int items, chunks, chunk_len, key_blocks, parts;
+    uint32_t part_rows;  // rows of a work-group of the second pass
+    BlockDiv div, group_div, chunk_div;
     float scale;
 };
 
@@ -62,9 +65,29 @@ __device__ inline int row_blocks(const PromptArgs& a, int s) {
     const int64_t hi = min(max(a.cu[s + 1], lo), a.total_tokens);
     return (int)(((hi - lo) * a.group + kRows - 1) / kRows);
 }
-// The sequence and its row block (a sequence's last first: it sees most keys) that `item` is.  False behind all.
+// The sequence and its row block that `item` is: all sequences' last blocks, which see most keys, then those before them, and
+// so on (up to 64 sequences; more go one after the other).  False behind all.
 __device__ inline bool find_rows(const PromptArgs& a, int& item, int& s) {
     const int lane = __lane_id();
+    if (a.num_seqs <= kWave) {
+        const int blocks = lane < a.num_seqs ? row_blocks(a, lane) : 0;
+        const auto all = [&](int n) { return lane_value(wave_incl_scan(min(blocks, n)), kWave - 1); };
+        int top = blocks;
+#pragma unroll
+        for (int m = 1; m < kWave; m *= 2) top = max(top, __shfl_xor(top, m));
+        top = uniform(top);
+        if (item >= all(top)) return false;
+        int low = 0, high = top;  // the last number from the end with no more than `item` blocks behind it
+        while (high - low > 1) {
+            const int mid = (low + high) >> 1;
+            if (all(mid) <= item) low = mid;
+            else high = mid;
+        }
+        const int behind = item - all(low), scan = wave_incl_scan(blocks > low ? 1 : 0);
+        s = __builtin_ctzll(__ballot(scan > behind));
+        item = lane_value(blocks, s) - 1 - low;
+        return true;
+    }
     for (s = 0; s < a.num_seqs; s += kWave) {
         const int blocks = s + lane < a.num_seqs ? row_blocks(a, s + lane) : 0;
         const int scan = wave_incl_scan(blocks);
@@ -94,8 +117,8 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_rows_kernel(PromptArgs a) 
     __shared__ __attribute__((aligned(4))) uint8_t odd[2][4];
     const int lane = threadIdx.x & 63, column = lane & 31, h = lane >> 5;
     const int wave = uniform(threadIdx.x >> 6);
-    const int kv_head = blockIdx.x % a.kv_heads, chunk = blockIdx.x / a.kv_heads % a.chunks;
-    int item = blockIdx.x / a.kv_heads / a.chunks, s;
+    const int place = blockIdx.x, kv_head = place % a.kv_heads, chunk = place / a.kv_heads % a.chunks;
+    int item = place / a.kv_heads / a.chunks, s;
     if (!find_rows(a, item, s)) return;
     s = uniform(s);
     item = uniform(item);
@@ -142,7 +165,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_rows_kernel(PromptArgs a) 
     int64_t page = page_of(begin + kTile);
 
     const uint32_t qrow = row0 + wave * 32 + column;
-    const bool live = qrow < rows;
+    const bool live = qrow < rows, busy = row0 + wave * 32 < rows;
     const uint32_t token = live ? a.group_div.page(qrow) : 0u;
     const int32_t limit = live && seq.start + token < seq.usable ? (int32_t)(seq.start + token) : -1;  // last visible key
     const int64_t head = (seq.row0 + token) * a.q_heads + (int64_t)kv_head * a.group + (live ? qrow - token * a.group : 0u);
@@ -165,6 +188,13 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_rows_kernel(PromptArgs a) 
         stage_at.forget();
         asm volatile("" : "+v"(lane_at));
         const uint8_t* keys = tiles[buffer];
+        if (!busy) {  // no row: this wave only stages
+            stage(staged, buffer ^ 1);
+            load(staged, t0 + 2 * kTile, page);
+            page = page_of(t0 + 3 * kTile);
+            lds_barrier();
+            continue;
+        }
         f32x16 x[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -209,59 +239,29 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_rows_kernel(PromptArgs a) 
     }
     const float total = swap32_add(sum, sum);  // the other half of the keys is with the lane 32 away
     if (!live || h != 0) return;
-    if (a.chunks == 1) {
-        a.rows[head * 2] = ref;
-        a.rows[head * 2 + 1] = limit < 0 || total == 0.f ? 0.f : 1.f / total;
-    } else {
-        a.partial[(head * a.chunks + chunk) * 2] = ref;
-        a.partial[(head * a.chunks + chunk) * 2 + 1] = total;
-    }
-}
-
-// Joins the chunks of the packed rows; one row (of a query head) per thread.
-__global__ __launch_bounds__(kThreads) void prompt_join_kernel(PromptArgs a) {
-    const int64_t head = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (head >= a.total_tokens * a.q_heads) return;
-    const int64_t token = head / a.q_heads;
-    // The sequence of the token: the last that begins at or before it.
-    int low = 0, high = a.num_seqs;
-    while (high - low > 1) {
-        const int mid = (low + high) >> 1;
-        if (a.cu[mid] <= token) low = mid;
-        else high = mid;
-    }
-    const Seq seq = sequence(a, low);
-    float ref = kRefNone, sum = 0.f;
-    const int64_t pos = seq.start + (token - seq.row0);
-    if (token >= seq.row0 && token < seq.row0 + seq.rows && seq.usable > 0 && pos < seq.usable) {
-        const int chunks = min((int)(pos / a.chunk_len) + 1, a.chunks);
-        const float* s = a.partial + head * a.chunks * 2;
-        for (int c = 0; c < chunks; ++c) {
-            const float top = fmaxf(ref, s[2 * c]);
-            sum = sum * fast_exp2(ref - top) + s[2 * c + 1] * fast_exp2(s[2 * c] - top);
-            ref = top;
-        }
-    }
-    a.rows[head * 2] = ref;
-    a.rows[head * 2 + 1] = sum != 0.f ? 1.f / sum : 0.f;
+    a.partial[(head * a.chunks + chunk) * 2] = ref;
+    a.partial[(head * a.chunks + chunk) * 2 + 1] = total;
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void prompt_keys_kernel(PromptArgs a) {
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void prompt_keys_kernel(PromptArgs a) {
     using S = Shape<D>;
     constexpr int P = S::kDim;
     __shared__ __attribute__((aligned(16))) uint8_t tiles[2][kTile * 2 * P];
+    __shared__ f32x2 divisors[2][kTile];  // (reference, 1 / sum) of a tile's rows
     const int lane = threadIdx.x & 63, column = lane & 31, h = lane >> 5;
     const int wave = uniform(threadIdx.x >> 6);
-    const int kv_head = blockIdx.x % a.kv_heads, s = blockIdx.x / a.kv_heads % a.num_seqs;
-    const int block = blockIdx.x / a.kv_heads / a.num_seqs;
+    const int unit = blockIdx.x % (a.kv_heads * a.num_seqs * a.key_blocks), part = blockIdx.x / (a.kv_heads * a.num_seqs * a.key_blocks);
+    const int kv_head = unit % a.kv_heads, s = unit / a.kv_heads % a.num_seqs, block = unit / a.kv_heads / a.num_seqs;
     const Seq seq = sequence(a, s);
     const int key0 = block * kKeys;
     if (key0 >= seq.usable || seq.rows == 0) return;
     const int64_t past = (int64_t)key0 - seq.start;  // tokens before this one see none of these keys
-    const uint32_t rows = (uint32_t)seq.rows * a.group;
     if (past >= seq.rows) return;
-    const uint32_t first_row = past > 0 ? (uint32_t)past * a.group : 0u;
+    const uint32_t from_row = past > 0 ? (uint32_t)past * a.group : 0u;  // the first that sees any
+    const uint32_t first_row = max(from_row, (uint32_t)part * a.part_rows);
+    const uint32_t rows = (uint32_t)min(seq.rows * a.group, (int64_t)(part + 1) * a.part_rows);
+    if (first_row >= rows) return;
 
     // This lane's key: an operand of all its wave's products.
     const uint32_t key = (uint32_t)key0 + wave * 32 + column;
@@ -303,31 +303,63 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_keys_kernel(PromptArgs a) 
 #pragma unroll
         for (int i = 0; i < S::kChunks; ++i) *reinterpret_cast<u32x4*>(tiles[buffer] + stage_at.chunk(4 * i)) = x.x[i];
     };
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    const auto load_rows = [&](f32x2 (&x)[2], uint32_t r0) {
+    // A row's divisor: its chunks go round four lanes.  The first two of each are loaded ahead.
+    const uint32_t stat_row = threadIdx.x >> 2;
+    const f32x2* stats = reinterpret_cast<const f32x2*>(a.partial);
+    struct Chunks {
+        f32x2 x[2];
+    };
+    const auto first_chunks = [&](uint32_t r0) {
+        const f32x2* of_row = stats + head_of_row(min(r0 + stat_row, rows - 1)) * a.chunks;
+        return Chunks{of_row[min(quarter, a.chunks - 1)], of_row[min(quarter + 4, a.chunks - 1)]};
+    };
+    const auto divide = [&](uint32_t r0, const Chunks& ahead, f32x2* to) {
+        const uint32_t r = min(r0 + stat_row, rows - 1);
+        const int64_t pos = seq.start + a.group_div.page(r);
+        // (A row behind the last, or that sees no key, gets no divisor.)
+        const int count = r0 + stat_row < rows && pos < seq.usable ? (int)a.chunk_div.page((uint32_t)pos) + 1 : 0;
+        float ref = quarter < count ? ahead.x[0][0] : kRefNone, sum = quarter < count ? ahead.x[0][1] : 0.f;
+        const auto join = [&](f32x2 y) {
+            const float top = fmaxf(ref, y[0]);
+            sum = sum * fast_exp2(ref - top) + y[1] * fast_exp2(y[0] - top);
+            ref = top;
+        };
+        if (a.chunks > 1) {
+            if (quarter + 4 < count) join(ahead.x[1]);
+            if (a.chunks > 8) {
+                const f32x2* of_row = stats + head_of_row(r) * a.chunks;
+                for (int c0 = quarter + 8; c0 < a.chunks; c0 += 16) {
+                    f32x2 y[4];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const uint32_t r = r0 + 32 * c + column;
-            x[c] = reinterpret_cast<const f32x2*>(a.rows)[head_of_row(min(r, rows - 1))];
-            x[c][1] = r < rows ? x[c][1] : 0.f;
+                    for (int i = 0; i < 4; ++i) y[i] = of_row[min(c0 + 4 * i, a.chunks - 1)];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (c0 + 4 * i < count) join(y[i]);
+                }
+            }
+            float top = fmaxf(ref, dpp<kDppQuadSwap1>(ref));
+            top = fmaxf(top, dpp<kDppQuadSwap2>(top));
+            sum = group_sum<4>(sum * fast_exp2(ref - top));
+            ref = top;
         }
+        if (quarter == 0) to[stat_row] = f32x2{ref, sum != 0.f ? 1.f / sum : 0.f};
     };
     Piece<D> staged;
-    f32x2 of_row[2], next_row[2];
     load(staged, first_row);
-    load_rows(of_row, first_row);
+    Chunks ahead = first_chunks(first_row);
     float acc[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[i] = 0.f;
     stage(staged, 0);
     load(staged, first_row + kTile);
+    divide(first_row, ahead, divisors[0]);
+    ahead = first_chunks(first_row + kTile);
     lds_barrier();
     int buffer = 0;
 #pragma unroll 1
     for (uint32_t r0 = first_row; r0 < rows; r0 += kTile, buffer ^= 1) {
         query_at.forget();
         stage_at.forget();
-        load_rows(next_row, r0 + kTile);
         f32x16 x[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -339,13 +371,16 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_keys_kernel(PromptArgs a) 
         }
         stage(staged, buffer ^ 1);
         load(staged, r0 + 2 * kTile);
+        divide(r0 + kTile, ahead, divisors[buffer ^ 1]);
+        ahead = first_chunks(r0 + 2 * kTile);
         const int64_t first_pos = seq.start + a.group_div.page(r0);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const float ref = of_row[c][0], by = of_row[c][1];
+            const f32x2 of_row = divisors[buffer][32 * c + column];
+            const float ref = of_row[0], by = of_row[1];
             // (A row without a divisor sees nothing; its scores may be anything.)
             if (key0 + 32 * wave + 31 > first_pos || __any(by == 0.f)) {
-                const int64_t pos = seq.start + a.group_div.page(min(r0 + 32 * c + column, rows));
+                const int64_t pos = seq.start + a.group_div.page(min(r0 + 32 * c + column, rows - 1));
                 const int seen = by == 0.f ? -1 : (int)(pos - (key0 + 32 * wave + 4 * h));
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -357,7 +392,6 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_keys_kernel(PromptArgs a) 
                 for (int i = 0; i < 16; ++i)
                     acc[i] = __builtin_fmaf(fast_exp2(__builtin_fmaf(x[c][i], a.scale, -ref)), by, acc[i]);
             }
-            of_row[c] = next_row[c];
         }
         lds_barrier();
     }
@@ -370,22 +404,52 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_keys_kernel(PromptArgs a) 
     }
     const int at = 32 * wave + 8 * (column >> 2) + 4 * h + (column & 3);
     const uint64_t keys_there = __ballot(there);
-    if (column < 16 && ((keys_there >> (at & 31)) & 1))
+    if (column >= 16) return;
+    if (a.parts > 1)
+        a.received[((int64_t)part * (a.kv_heads * a.num_seqs * a.key_blocks) + unit) * kKeys + at] = mine;
+    else if ((keys_there >> (at & 31)) & 1)
         a.weights[((int64_t)s * a.kv_heads + kv_head) * a.weight_row + key0 + at] += mine;
 }
 
+// Adds up the parts, from the first that has rows which see the keys; one key per thread, in the order of the parts.
+__global__ __launch_bounds__(kKeys) void prompt_add_kernel(PromptArgs a) {
+    const int units = a.kv_heads * a.num_seqs * a.key_blocks, unit = blockIdx.x;
+    const int kv_head = unit % a.kv_heads, s = unit / a.kv_heads % a.num_seqs, block = unit / a.kv_heads / a.num_seqs;
+    const Seq seq = sequence(a, s);
+    const int key0 = block * kKeys, key = key0 + threadIdx.x;
+    const int64_t past = max((int64_t)key0 - seq.start, (int64_t)0);
+    if (key >= seq.usable || past >= seq.rows) return;
+    const int64_t page = a.tables[(int64_t)s * a.width + a.div.page((uint32_t)key)];
+    if ((uint64_t)page >= (uint64_t)a.num_blocks) return;
+    const int first = (int)((uint32_t)past * a.group / a.part_rows), last = (int)(((uint32_t)seq.rows * a.group - 1) / a.part_rows);
+    float sum = 0.f;
+    for (int p = first; p <= last; ++p) sum += a.received[((int64_t)p * units + unit) * kKeys + threadIdx.x];
+    a.weights[((int64_t)s * a.kv_heads + kv_head) * a.weight_row + key] += sum;
+}
+
 struct Plan {
-    int64_t items, chunks, chunk_len, key_blocks;
+    int64_t items, chunks, chunk_len, key_blocks, parts, part_rows;
+    size_t floats;
 };
 Plan plan(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_heads, int64_t block_size, int64_t width) {
     const int64_t capacity = block_size * width, group = q_heads / kv_heads;
-    const int64_t items = total * group / kRows + num_seqs;
+    Plan p{};
+    p.items = total * group / kRows + num_seqs;
     // Chunks of the keys, 256 at least, until there are about three work-groups per compute unit.
-    int64_t chunks = std::max<int64_t>(1, std::min((capacity + 255) / 256, 768 / (items * kv_heads)));
-    chunks = std::min<int64_t>(chunks, 64);
-    int64_t len = (capacity + chunks - 1) / chunks;
-    len = (len + kTile - 1) / kTile * kTile;
-    return {items, (capacity - 1) / len + 1, len, (capacity - 1) / kKeys + 1};
+    p.chunks = std::max<int64_t>(1, std::min((capacity + 255) / 256, 768 / (p.items * kv_heads)));
+    p.chunks = std::min<int64_t>(p.chunks, 64);
+    p.chunk_len = ((capacity + p.chunks - 1) / p.chunks + kTile - 1) / kTile * kTile;
+    p.chunks = (capacity - 1) / p.chunk_len + 1;
+    p.key_blocks = (capacity - 1) / kKeys + 1;
+    // Parts of the rows, if sequences are alike of 1024 to 2048 rows: the first keys are seen by all rows and the last by few,
+    // and the longest work-group is the last (2 x 4096 tokens, 16 heads on 8: 223 us, 257 in one part).  Where there are
+    // thousands of work-groups anyhow, they balance by themselves.
+    const int64_t all = total * group;
+    p.parts = std::max<int64_t>(1, std::min<int64_t>(all / num_seqs / 1024, 4096 / (num_seqs * kv_heads * p.key_blocks)));
+    p.part_rows = ((all - 1) / p.parts / kTile + 1) * kTile;
+    p.floats = (size_t)(total * q_heads * p.chunks * 2);
+    if (p.parts > 1) p.floats += (size_t)(p.parts * num_seqs * kv_heads * p.key_blocks) * kKeys;
+    return p;
 }
 
 template <typename T, int D>
@@ -394,12 +458,11 @@ int launch(const PromptArgs& a, hipStream_t s) {
     if (a.div.size % 16 == 0) hipLaunchKernelGGL((prompt_rows_kernel<T, D, 16>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((prompt_rows_kernel<T, D, 1>), grid, block, 0, s, a);
     if (int rc = check_launch("prompt weights, rows")) return rc;
-    if (a.chunks > 1) {
-        hipLaunchKernelGGL(prompt_join_kernel, dim3((unsigned)((a.total_tokens * a.q_heads - 1) / kThreads + 1)), block, 0, s, a);
-        if (int rc = check_launch("prompt weights, join")) return rc;
-    }
-    hipLaunchKernelGGL((prompt_keys_kernel<T, D>), dim3((unsigned)((int64_t)a.num_seqs * a.key_blocks * a.kv_heads)), block, 0, s, a);
-    return check_launch("prompt weights, keys");
+    hipLaunchKernelGGL((prompt_keys_kernel<T, D>), dim3((unsigned)((int64_t)a.num_seqs * a.key_blocks * a.kv_heads * a.parts)), block, 0, s, a);
+    if (int rc = check_launch("prompt weights, keys")) return rc;
+    if (a.parts == 1) return MVME_OK;
+    hipLaunchKernelGGL(prompt_add_kernel, dim3((unsigned)((int64_t)a.num_seqs * a.key_blocks * a.kv_heads)), dim3(kKeys), 0, s, a);
+    return check_launch("prompt weights, parts");
 }
 
 template <typename T>
@@ -435,7 +498,7 @@ extern "C" size_t mvme_prefill_attention_weights_workspace_size(int64_t num_seqs
                                                                 int64_t table_width) {
     if (!prompt_shape(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width)) return 0;
     const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, block_size, table_width);
-    return (size_t)(total_tokens * q_heads) * (size_t)(p.chunks == 1 ? 1 : 1 + p.chunks) * 2 * sizeof(float);
+    return p.floats * sizeof(float);
 }
 
 extern "C" int mvme_prefill_attention_weights(const void* q, const void* key_cache, const int64_t* cu_seqlens_q,
@@ -465,8 +528,7 @@ extern "C" int mvme_prefill_attention_weights(const void* q, const void* key_cac
     if (!fp4::aligned(q, 16) || !fp4::aligned(key_cache, 16) || !fp4::aligned(weights, 4))
         return fail(MVME_EINVAL, "prompt weights: queries and caches must be 16-byte aligned");
     const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, block_size, table_width);
-    if (p.items > kMostThreads / kThreads / kv_heads / p.chunks || num_seqs > kMostThreads / kThreads / kv_heads / p.key_blocks ||
-        total_tokens * q_heads / kThreads >= kMostThreads / kThreads)
+    if (p.items > kMostThreads / kThreads / kv_heads / p.chunks || num_seqs > kMostThreads / kThreads / kv_heads / p.key_blocks / p.parts)
         return fail(MVME_EINVAL, "too many packed query rows");
     const size_t need = mvme_prefill_attention_weights_workspace_size(num_seqs, total_tokens, q_heads, kv_heads, head_dim,
                                                                       block_size, table_width);
@@ -480,8 +542,8 @@ extern "C" int mvme_prefill_attention_weights(const void* q, const void* key_cac
     a.starts = query_starts;
     a.tables = block_tables;
     a.lens = context_lens;
-    a.rows = static_cast<float*>(workspace);
-    a.partial = a.rows + total_tokens * q_heads * 2;
+    a.partial = static_cast<float*>(workspace);
+    a.received = a.partial + total_tokens * q_heads * p.chunks * 2;
     a.weights = weights;
     a.weight_row = weight_row;
     a.num_blocks = num_blocks;
@@ -497,8 +559,11 @@ extern "C" int mvme_prefill_attention_weights(const void* q, const void* key_cac
     a.chunks = (int)p.chunks;
     a.chunk_len = (int)p.chunk_len;
     a.key_blocks = (int)p.key_blocks;
+    a.parts = (int)p.parts;
+    a.part_rows = (uint32_t)p.part_rows;
     a.div = fp4::make_block_div(block_size);
     a.group_div = fp4::make_block_div(a.group);
+    a.chunk_div = fp4::make_block_div(p.chunk_len);
     a.scale = kLog2e / __builtin_sqrtf((float)head_dim);
     hipStream_t st = static_cast<hipStream_t>(stream);
     return dtype == MVME_FP16 ? launch_dim<Half>(a, head_dim, st) : launch_dim<BFloat16>(a, head_dim, st);
