@@ -13,11 +13,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void weighted_decode_ke
     __shared__ __attribute__((aligned(16))) NarrowLds<D, kStoreScores> lds;
     Walk w;
     w.count(a);
-    if ((int)blockIdx.x >= w.total * a.kv_heads) return;
-    const int first = w.first_of(blockIdx.x), stop = w.first_of(blockIdx.x + 1);
+    const int wg = blockIdx.x;
+    if (wg >= w.shares) return;
+    const int first = w.first_of(wg), stop = w.first_of(wg + 1);
 #pragma unroll 1
     for (int at = first; at < stop;) {
-        const Segment s = find_segment(a, w, at, stop);
+        const Segment s = find_segment(a, w, wg, at, stop);
         at += s.rounds;
         narrow_segment<T, D, RUN, kStoreScores>(a, s, lds);
     }

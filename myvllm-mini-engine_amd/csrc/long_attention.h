@@ -108,6 +108,7 @@ struct Walk {
     int wide_units, narrow_units;     // of a kv head, of groups
     int wide_rounds, narrow_rounds;   // the same in rounds
     int total;                        // rounds of a kv head
+    int shares;                       // one per work-group, from the first on
     int share, longer;                // rounds of a share; the first `longer` shares have one more
     Group group0;                     // of group `lane`
     Own own0;                         // of sequence `lane`
@@ -215,10 +216,20 @@ struct Walk {
         int rounds = 0;
         for (int s0 = 0; s0 < a.batch; s0 += kWave) rounds += lane_value(wave_incl_scan(own(a, s0).rounds()), kWave - 1);
         total = wide_rounds + narrow_rounds + rounds * a.head_tiles;
-        // Shares differ by a round at most, the first ones are longer.
-        const int all = total * a.kv_heads, shares = max(min(a.shares, all), 1);
-        share = all / shares;
+        // Shares differ by a round at most, the first ones are longer.  They have two rounds at least where that leaves every
+        // compute unit one: more pieces cost the join more than they save.
+        const int all = total * a.kv_heads;
+        shares = max(min(a.shares, max(all / 2, min(all, 256))), 1);
+        shares = min(shares, all);  // (none where there are no rounds)
+        share = shares > 0 ? all / shares : 0;
         longer = all - share * shares;
+    }
+    // The share of this work-group, or -1: consecutive shares are on one XCD (work-groups are dealt to these in turn), whose L2
+    // then has keys that several row tiles of a group read at about the same time (128 sequences over 16384 tokens 82 us, 85
+    // with shares in the order of the work-groups; where nothing is read twice that order is ahead, by one in a hundred).
+    __device__ inline int mine() const {
+        const int per = (shares + 7) / 8, at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        return (int)(blockIdx.x >> 3) < per && at < shares ? at : -1;
     }
     // First round of a work-group's share.
     __device__ inline int first_of(int wg) const { return wg * share + min(wg, longer); }
@@ -262,7 +273,7 @@ struct Segment {
     bool wide;
 };
 
-__device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int stop) {
+__device__ inline Segment find_segment(const Args& a, const Walk& w, int wg, int at, int stop) {
     Segment s;
     s.kv_head = at / w.total;
     int q = at - s.kv_head * w.total;
@@ -296,7 +307,7 @@ __device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int
         s.first_row = x.first;
         s.rows = x.rows * a.group - s.tile * (s.wide ? kWideRows : kColumns);
         unit += s.tile;
-        s.slot = (s.wide ? s.kv_head * w.wide_units : s.kv_head * units) + unit + (int)blockIdx.x;
+        s.slot = (s.wide ? s.kv_head * w.wide_units : s.kv_head * units) + unit + wg;
     } else {
         q -= w.wide_rounds + w.narrow_rounds;
         s.wide = false;
@@ -321,7 +332,7 @@ __device__ inline Segment find_segment(const Args& a, const Walk& w, int at, int
         s.tile = (q - base) / rounds;
         from = q - base - s.tile * rounds;
         s.rows = a.group - s.tile * kColumns;
-        s.slot = s.kv_head * units + w.narrow_units + s.seq * a.head_tiles + s.tile + (int)blockIdx.x;
+        s.slot = s.kv_head * units + w.narrow_units + s.seq * a.head_tiles + s.tile + wg;
     }
     const int n = min(rounds - from, stop - at);
     if (s.first_row < 0 && start == 0 && n == rounds) s.slot = -1;

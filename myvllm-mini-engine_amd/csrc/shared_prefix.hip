@@ -211,11 +211,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void shared_prefix_kern
     } lds;
     Walk w;
     w.count(a);
-    if ((int)blockIdx.x >= w.total * a.kv_heads) return;
-    const int first = w.first_of(blockIdx.x), stop = w.first_of(blockIdx.x + 1);
+    const int wg = w.mine();
+    if (wg < 0) return;
+    const int first = w.first_of(wg), stop = w.first_of(wg + 1);
 #pragma unroll 1
     for (int at = first; at < stop;) {
-        const Segment s = find_segment(a, w, at, stop);
+        const Segment s = find_segment(a, w, wg, at, stop);
         at += s.rounds;
         if (s.wide) wide_segment<T, D, RUN>(a, s, lds.wide);
         else narrow_segment<T, D, RUN, kNoScores>(a, s, lds.narrow);
