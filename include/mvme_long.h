@@ -28,11 +28,11 @@ size_t mvme_paged_attention_shared_prefix_workspace_size(int64_t batch, int64_t 
  * mvme_paged_attention for a batch in which sequences share prefixes.  Group g
  * is the sequences group_offsets[g] .. group_offsets[g + 1] - 1 (offsets rise
  * from 0 or more to at most batch; sequences in no group share nothing); the
- * first prefix_lens[g] tokens of all of them are in the same pages, those of
- * the table of the group's first sequence, and are read once for all.
- * Sequences of a group that are shorter than its prefix are attended through
- * their own tables, as are groups of one and of a prefix that is not positive
- * or passes the tables' capacity.  Offsets that fall, or leave the batch, make
+ * first prefix_lens[g] tokens of all of them are in the same pages and are read
+ * once for all, through the table of the group's first sequence that has them
+ * all.  Sequences of a group that are shorter than its prefix (the empty ones of
+ * a padded batch) are attended through their own tables, as are groups of one
+ * and of a prefix that is not positive or passes the tables' capacity.  Offsets that fall, or leave the batch, make
  * all sequences ungrouped.  Every row's result is that of
  * mvme_paged_attention, to rounding: scale 1/sqrt(head_dim), zeros for lengths
  * <= 0 or beyond the table's capacity, pages out of range skipped.

@@ -239,6 +239,16 @@ struct Walk {
         return round < until ? round / (share + 1) : longer + (round - until) / max(share, 1);
     }
 
+    // The sequence whose table names a group's prefix: the first that reaches to its end.  (If none does, no row uses it.)
+    __device__ inline int reader_of(const Args& a, const Group& x) const {
+        const int lane = __lane_id();
+        for (int s0 = x.first & -kWave; s0 < x.first + x.rows; s0 += kWave) {
+            const int seq = s0 + lane, len = s0 == 0 ? own0.len : length_from(a, load_length(a, seq));
+            const uint64_t hit = __ballot(seq >= x.first && seq < x.first + x.rows && len >= x.prefix);
+            if (hit) return s0 + __builtin_ctzll(hit);
+        }
+        return x.first;
+    }
     // The units of `group` begin at round `base` of a kv head, and number `unit` among their kind.
     __device__ inline void place_of_group(const Args& a, int g, bool wide, int& base, int& unit) const {
         const int lane = __lane_id();
@@ -303,7 +313,7 @@ __device__ inline Segment find_segment(const Args& a, const Walk& w, int wg, int
         s.tile = (q - base) / rounds;
         from = q - base - s.tile * rounds;
         tokens = x.prefix;
-        s.seq = x.first;
+        s.seq = w.reader_of(a, x);
         s.first_row = x.first;
         s.rows = x.rows * a.group - s.tile * (s.wide ? kWideRows : kColumns);
         unit += s.tile;
@@ -826,7 +836,7 @@ inline bool head_dim_built(int64_t d) {
     return d == 16 || d == 32 || d == 64 || d == 80 || d == 96 || d == 128 || d == 192 || d == 256;
 }
 
-constexpr int64_t kMostBatchHeads = int64_t(1) << 24;
+constexpr int64_t kMostBatchHeads = kMostThreads / kThreads;
 
 // The checks that the decode entry points make of their shapes, and what follows from these.
 inline int check_shape(Args& a, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t num_blocks,

@@ -59,10 +59,9 @@ def _check_groups(tables, lengths, offsets, prefixes, block_size):
         _check(0 <= prefix <= tables.shape[1] * block_size, "prefix length exceeds block table capacity")
         if first == last or prefix == 0:
             continue
-        _check(lens[first] >= prefix, "the first sequence of a group must reach to the end of its prefix")
         pages = -(-prefix // block_size)
         whole = [b for b in range(first, last) if lens[b] >= prefix]
-        _check(bool((tables[whole, :pages] == tables[first, :pages]).all()),
+        _check(not whole or bool((tables[whole, :pages] == tables[whole[0], :pages]).all()),
                "sequences of a group must have the prefix in the same pages")
 
 
@@ -75,11 +74,11 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, c
     and lengths), and so are the results, to rounding.  Sequences
     ``group_offsets[g] .. group_offsets[g + 1] - 1`` (int64 [groups + 1], rising;
     what is in no group shares nothing) hold their first ``prefix_lens[g]``
-    tokens (int64 [groups]) in the same pages, which are read through the first
-    one's table.  A sequence shorter than its group's prefix is attended on its
-    own.  Calls of few cached tokens run ``paged_attention``'s kernels, which
-    are ahead there, unless ``always_share``.  ``validate=True`` reads the metadata on the host, and refuses groups
-    whose pages differ; with ``validate=False`` (graph capture) the caller
+    tokens (int64 [groups]) in the same pages.  A sequence shorter than its
+    group's prefix (an empty one of a padded batch) is attended on its own.
+    Calls of few cached tokens run ``paged_attention``'s kernels, which are
+    ahead there, unless ``always_share``.  ``validate=True`` reads the metadata
+    on the host, and refuses groups whose pages differ; with ``validate=False`` (graph capture) the caller
     answers for that, lengths and pages that cannot be are absent, and offsets
     that cannot be leave every sequence on its own.  ``out`` / ``workspace``
     may supply the buffers (``shared_prefix_workspace_bytes``).

@@ -101,6 +101,21 @@ def test_short_empty_and_single_members():
     assert not out[5].any() and not out[6].any()
 
 
+@pytest.mark.parametrize("batch", [6, 40, 100])
+def test_first_members_of_a_group_may_be_padding(batch):
+    # Empty rows with empty tables come first, and one too short.
+    for empty in (1, 2, 70):
+        if empty + 3 > batch:
+            continue
+        lens = [300 + i for i in range(batch)]
+        args = list(case(20 + batch, lens, [(0, batch, 256)], heads=8, kv=4, dim=64))
+        args[3], args[4] = args[3].clone(), args[4].clone()
+        args[3][:empty], args[4][:empty] = -1, 0
+        args[3][empty, 4:], args[4][empty] = -1, 60
+        out = check(args, validate=False)
+        assert not out[:empty].any() and out[empty:].any(-1).all()
+
+
 def test_absent_pages_are_skipped():
     args = list(case(6, [500, 400, 333, 480], [(0, 4, 320)]))
     tables = args[3].clone()
