@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kThreads) void weighted_join_kernel(Args a, int blo
             if (h0 + h < a.group) {
                 const float ref = stats[h][0], by = stats[h][1];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) add[i] += fast_exp2(__builtin_fmaf(s[h][i], a.scale, -ref)) * by;
+                for (int i = 0; i < 4; ++i) add[i] += probability(a, s[h][i], ref, by);
             }
     }
 #pragma unroll

@@ -256,7 +256,8 @@ extern "C" int mvme_evict_kv_cache(void* key_cache, void* value_cache, const flo
         return fail(MVME_EINVAL, "KV cache too large");
     if (batch > 2147483647 || layers > 2147483647) return fail(MVME_EINVAL, "batch/head product too large");
     const int64_t lines = layers * batch;  // (rows are cut, into more work-groups, only where there are few)
-    if (layers > kMostThreads / 1024 / batch || lines > kMostThreads / 1024 / kv_heads) return fail(MVME_EINVAL, "batch/head product too large");
+    if (layers > kMostThreads / 1024 / batch || lines > kMostThreads / 1024 / kv_heads)
+        return fail(MVME_EINVAL, "batch/head product too large");
     if (!key_cache || !value_cache || !weights || !new_weights || !kept || !new_lens || !block_tables || !context_lens)
         return fail(MVME_EINVAL, "eviction: null pointer");
     if (!fp4::aligned(key_cache, 16) || !fp4::aligned(value_cache, 16)) return fail(MVME_EINVAL, "eviction: caches must be 16-byte aligned");

@@ -474,6 +474,12 @@ __device__ inline u32x2 split_pair(float x, float y) {
 
 constexpr int kRing = 512;  // 16-byte pieces of scores that a wave gathers before it stores them
 
+// The probability that a dot product stands for.  (None where there is no token, whatever the divisor is: another key's NaN
+// makes that NaN.)
+__device__ inline float probability(const Args& a, float score, float ref, float by) {
+    return score == kNegInf ? 0.f : fast_exp2(__builtin_fmaf(score, a.scale, -ref)) * by;
+}
+
 // What becomes of a segment's dot products: nothing, they go to memory, or (the segment is a whole unit, and the ring holds
 // it) they become weights at its end.
 enum Scores { kNoScores, kStoreScores, kAddWeights };
@@ -687,7 +693,7 @@ __device__ inline void narrow_segment(const Args& a, const Segment& seg, NarrowL
             for (int h = 0; h < heads; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    add[i] += fast_exp2(__builtin_fmaf(s[h][i], a.scale, -lds.divisors[0][h])) * lds.divisors[1][h];
+                    add[i] += probability(a, s[h][i], lds.divisors[0][h], lds.divisors[1][h]);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (key + i < seg.end) weights[key + i] += add[i];

@@ -120,6 +120,6 @@ def evict_kv_cache(key_cache, value_cache, weights, block_tables, context_lens, 
         lib.call("mvme_evict_kv_cache", key_cache.data_ptr(), value_cache.data_ptr(), weights.data_ptr(),
                  new_weights.data_ptr(), row, kept.data_ptr(), lengths.data_ptr(), block_tables.data_ptr(),
                  context_lens.data_ptr(), first.data_ptr() if first is not None else None, layers, batch, kv_heads,
-                 head_dim, num_blocks, block_size, width, min(keep, row), recent, ext.dtype_code(key_cache.dtype),
+                 head_dim, num_blocks, block_size, width, min(keep, row), min(recent, row), ext.dtype_code(key_cache.dtype),
                  ext.current_stream(key_cache.device))
     return kept, lengths, new_weights

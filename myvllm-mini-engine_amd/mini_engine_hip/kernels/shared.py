@@ -78,10 +78,11 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, c
     group's prefix (an empty one of a padded batch) is attended on its own.
     Calls of few cached tokens run ``paged_attention``'s kernels, which are
     ahead there, unless ``always_share``.  ``validate=True`` reads the metadata
-    on the host, and refuses groups whose pages differ; with ``validate=False`` (graph capture) the caller
-    answers for that, lengths and pages that cannot be are absent, and offsets
-    that cannot be leave every sequence on its own.  ``out`` / ``workspace``
-    may supply the buffers (``shared_prefix_workspace_bytes``).
+    on the host, and refuses groups whose pages differ; with ``validate=False``
+    (graph capture) the caller answers for that, lengths and pages that cannot
+    be are absent, and offsets that cannot be leave every sequence on its own.
+    ``out`` / ``workspace`` may supply the buffers
+    (``shared_prefix_workspace_bytes``).
     """
     if backend != "hip":
         raise ValueError("decode backend must be hip")

@@ -70,6 +70,19 @@ def test_step_empty_sequences_and_absent_pages():
     assert not paged_attention_weights(*args, validate=False).any() and torch.equal(args[6], before)
 
 
+@pytest.mark.parametrize("n", [200, 3000])
+def test_step_nan_does_not_reach_absent_tokens(n):
+    args = list(step_case(9, [n, 40]))
+    args[0][0, 3] = float("nan")  # a head of kv head 1
+    args[3][0, 5] = -1
+    before = args[6].clone()
+    paged_attention_weights(*args, validate=False)
+    w, there = args[6][0, 1], torch.arange(args[6].shape[2], device=DEV)
+    there = (there < n) & (there // 16 != 5)
+    assert torch.isnan(w[there]).all() and torch.equal(w[~there], before[0, 1][~there])
+    assert torch.isfinite(args[6][0, 0]).all() and torch.isfinite(args[6][1]).all()
+
+
 def test_step_probabilities_add_up_over_steps():
     args = step_case(3, [257, 1000], heads=8, kv=2, dim=64)
     before = args[6].clone()
@@ -195,6 +208,12 @@ def test_prompt_nan_reaches_what_its_row_sees():
     prefill_attention_weights(*args)
     w = args[7][0]
     assert torch.isfinite(w[0]).all() and torch.isnan(w[1, :41]).all() and torch.isfinite(w[1, 41:]).all()
+    args = list(prompt_case(3, [100], [0], heads=2, kv=2, dim=64))
+    args[0][40, 1] = float("nan")
+    args[4][0, 1] = -1
+    prefill_attention_weights(*args, validate=False)
+    w = args[7][0, 1]
+    assert torch.isnan(w[:16]).all() and torch.isfinite(w[16:32]).all() and torch.isnan(w[32:41]).all()
 
 
 def test_prompt_large_scores():

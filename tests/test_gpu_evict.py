@@ -101,6 +101,9 @@ def test_strange_weights():
 def test_nothing_to_evict_and_lengths_that_cannot_be():
     args = list(case(2, [50, 60, 70, 80], pad=1))
     check(args, 100)
+    check(args, 2 ** 70, recent=2 ** 70)
+    check(args, 40, recent=2 ** 64 + 3)
+    args = list(case(2, [50, 60, 70, 80], pad=1))
     args[4] = torch.tensor([0, -7, 10 ** 8, 80], device=DEV)
     check(args, 40, validate=False)
 
