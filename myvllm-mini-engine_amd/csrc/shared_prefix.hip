@@ -1,5 +1,22 @@
 // Decode attention for batches whose sequences share prefixes: each prefix is
 // read once for all query heads of its group, and every row's own keys once.
+//
+// Softmax sums over disjoint sets of keys join: with references m_i, sums s_i
+// and outputs o_i = sum_j 2^(x_j - m_i) v_j, out = sum_i 2^(m_i - m) o_i /
+// sum_i 2^(m_i - m) s_i.  So a group's prefix is attended by all its rows at
+// once, each row's own keys by its heads alone, and both are cut where the
+// shares end.
+//
+// Bounds: with few rows per key the reads (16 sequences over 1024 shared
+// tokens and 64 in all, 401 MB: 77 us, of which the join is 5; 5.5 TB/s in
+// the walk), with many the matrix and vector units in turn (128 sequences, 32
+// heads on 8, over 16384 tokens: 82 us, 30 of them matrix products at the
+// card's rate).  There a wave's tile of 32 rows and 64 keys of 128 dims is, by
+// count, 1024 cycles of matrix products and about 900 of vector work, half of
+// that exponentials; two waves a SIMD overlap them in part.  128 rows a
+// work-group are what two work-groups' registers and LDS allow; three per
+// compute unit, or the next tile's scores beside this one's softmax, spill or
+// were slower (88 against 85).
 #include "../../include/mvme_long.h"
 #include "long_attention.h"
 
