@@ -1,11 +1,12 @@
 // Eviction from a paged cache: of every layer, sequence and kv head the tokens
 // that are kept are chosen and their rows moved to the front, in order.
 //
-// The choice is a radix select: four passes over a row of weights, the later ones
-// from L2, then one that ranks by prefix sums.  The moves are bound by HBM, reads
-// and writes alike.  28 layers of 8 sequences of 2048 tokens, half kept, 8 heads of
-// 128: 34 us to choose and 392 to move 0.94 GB (4.8 TB/s, what a large copy
-// reaches); one layer of 16 ragged sequences 10 and 11.
+// The choice is a radix select, four passes over a row of weights in registers,
+// then a prefix sum that ranks what is kept (read again by every pass, with a prefix
+// sum per 512 tokens, one layer of 16 ragged sequences took 21.0 us, and 18.8 so).
+// The moves are bound by HBM, reads and writes alike.  28 layers of 8 sequences of
+// 2048 tokens, half kept, 8 heads of 128: 417 us for 0.94 GB moved, 4.5 TB/s with
+// the choice, about the rate of a large copy without.
 #include "../../include/mvme_long.h"
 #include "fp4_cache.h"
 
@@ -77,7 +78,9 @@ __device__ inline void scan_pair(int x, int y, int& before_x, int& before_y, int
     __syncthreads();
 }
 
-template <int kSelect>
+// kHeld > 0: weights are read once, kHeld at most per thread, and a thread's are neighbours, so that one scan ranks all.
+// kHeld 0: rows of any length, read again by every pass.
+template <int kSelect, int kHeld>
 __global__ __launch_bounds__(kSelect) void choose_kernel(Args a) {
     constexpr int kWaves = kSelect / kWave;
     __shared__ int histogram[256][kCopies];
@@ -106,15 +109,28 @@ __global__ __launch_bounds__(kSelect) void choose_kernel(Args a) {
     const int recent = (int)min(a.recent, (int64_t)(keep - first));
     const int stop = n - recent;  // the weights decide about first .. stop - 1
     int want = keep - first - recent;
+    const bool choose = want > 0;
+    const int each = kHeld ? (n + kSelect - 1) / kSelect : 0, mine0 = each * (int)threadIdx.x;
+    float held[kHeld ? kHeld : 1];
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+        if (k < each) held[k] = w[min(mine0 + k, n - 1)];
     // The want-th largest rank, a byte at a time from the highest: `prefix` is what its upper bytes are.
     uint32_t prefix = 0, mask = 0;
     if (want > 0) {
         for (int shift = 24; shift >= 0; shift -= 8) {
             for (int i = threadIdx.x; i < 256 * kCopies; i += kSelect) histogram[i / kCopies][i % kCopies] = 0;
             __syncthreads();
-            for (int i = first + threadIdx.x; i < stop; i += kSelect) {
-                const uint32_t rank = rank_of(w[i]);
+            const auto count = [&](float x) {
+                const uint32_t rank = rank_of(x);
                 if ((rank & mask) == prefix) atomicAdd(&histogram[(rank >> shift) & 255][threadIdx.x % kCopies], 1);
+            };
+            if constexpr (kHeld) {
+#pragma unroll
+                for (int k = 0; k < kHeld; ++k)
+                    if (k < each && mine0 + k >= first && mine0 + k < stop) count(held[k]);
+            } else {
+                for (int i = first + threadIdx.x; i < stop; i += kSelect) count(w[i]);
             }
             __syncthreads();
             // Bin 255 - t of thread t: the one in which the count from above reaches want.
@@ -140,20 +156,44 @@ __global__ __launch_bounds__(kSelect) void choose_kernel(Args a) {
         }
     }
     // Kept: what is protected or above that rank, and the first `want` that equal it.
+    const auto sort_out = [&](int i, float x, int& is_above, int& is_level) {
+        const bool decided = i < first || i >= stop;
+        const uint32_t rank = rank_of(x);
+        is_above = i < n && (decided || (choose && rank > prefix));
+        is_level = i < n && !decided && choose && rank == prefix;
+    };
     int above = 0, level = 0;
+    if constexpr (kHeld) {
+        int aboves = 0, levels = 0, all_above, all_level;
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+            if (k < each) {
+                int is_above, is_level;
+                sort_out(mine0 + k, held[k], is_above, is_level);
+                aboves += is_above;
+                levels += is_level;
+            }
+        scan_pair(aboves, levels, above, level, all_above, all_level, sums, kWaves);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k)
+            if (k < each) {
+                int is_above, is_level;
+                sort_out(mine0 + k, held[k], is_above, is_level);
+                if (is_above || (is_level && level < want)) {
+                    const int to = above + min(level, want);
+                    kept[to] = mine0 + k;
+                    out[to] = held[k];
+                }
+                above += is_above;
+                level += is_level;
+            }
+        return;
+    }
     for (int i0 = 0; i0 < n; i0 += kSelect) {
         const int i = i0 + threadIdx.x;
-        int is_above = 0, is_level = 0;
-        float x = 0.f;
-        if (i < n) {
-            x = w[i];
-            if (i < first || i >= stop) is_above = 1;
-            else if (keep - first - recent > 0) {
-                const uint32_t rank = rank_of(x);
-                is_above = rank > prefix;
-                is_level = rank == prefix;
-            }
-        }
+        const float x = w[min(i, n - 1)];
+        int is_above, is_level;
+        sort_out(i, x, is_above, is_level);
         int before_above, before_level, all_above, all_level;
         scan_pair(is_above, is_level, before_above, before_level, all_above, all_level, sums, kWaves);
         const int levels = level + before_level;
@@ -301,10 +341,12 @@ extern "C" int mvme_evict_kv_cache(void* key_cache, void* value_cache, const flo
     a.rows = per * kPasses < kMove ? per * kPasses : kMove;
     hipStream_t s = static_cast<hipStream_t>(stream);
     // 512 threads choose sooner among few tokens, 1024 among many.
-    if (block_size * table_width <= 8192)
-        hipLaunchKernelGGL((choose_kernel<512>), dim3((unsigned)(lines * kv_heads)), dim3(512), 0, s, a);
-    else
-        hipLaunchKernelGGL((choose_kernel<1024>), dim3((unsigned)(lines * kv_heads)), dim3(1024), 0, s, a);
+    const int64_t capacity = block_size * table_width;
+    const dim3 grid((unsigned)(lines * kv_heads));
+    if (capacity <= 512 * 4) hipLaunchKernelGGL((choose_kernel<512, 4>), grid, dim3(512), 0, s, a);
+    else if (capacity <= 512 * 16) hipLaunchKernelGGL((choose_kernel<512, 16>), grid, dim3(512), 0, s, a);
+    else if (capacity <= 1024 * 16) hipLaunchKernelGGL((choose_kernel<1024, 16>), grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((choose_kernel<1024, 0>), grid, dim3(1024), 0, s, a);
     if (int rc = check_launch("eviction choice")) return rc;
     hipLaunchKernelGGL(move_kernel, dim3((unsigned)(lines * kv_heads * 2 * a.slices)), dim3(kMove), 0, s, a);
     return check_launch("eviction moves");

@@ -85,6 +85,12 @@ def test_long_sequences(n):
     check(case(n, [n], layers=1, kv=2, dim=32, block=32), n // 2 + 1, first=[3], recent=33)
 
 
+@pytest.mark.parametrize("n", [513, 2048, 2049, 8192, 8193, 12000, 20000])
+def test_long_rows_of_few_levels(n):
+    check(case(n, [n, n - 1, n // 3], layers=1, kv=1, dim=8, block=1, levels=3), n // 2, first=[3, 0, 1], recent=7)
+    check(case(n, [n, n - 1, n // 3], layers=1, kv=1, dim=8, block=1, levels=3), 10, first=[3, 10, 1], recent=9)
+
+
 def test_strange_weights():
     args = case(1, [300, 300, 300, 300], layers=1, kv=1, dim=8)
     w = args[2]
