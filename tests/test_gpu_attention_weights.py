@@ -52,6 +52,11 @@ def test_step_long(lens, block):
     check_step(step_case(len(lens), lens, block=block))
 
 
+@pytest.mark.parametrize("lens,pad", [([40, 3000], 4000), ([1, 17], 65530), ([700] * 20, 300)])
+def test_step_wide_tables(lens, pad):
+    check_step(step_case(len(lens), lens, heads=8, kv=4, dim=64, pad=pad), validate=False)
+
+
 def test_step_is_paged_attention():
     args = step_case(1, [500, 64, 1])
     out = check_step(args)
@@ -181,6 +186,36 @@ def test_prompt_shapes(heads, kv, new, prior):
                                              ([1], [30000], 256), ([20] * 70, [30 * i for i in range(70)], 16)])
 def test_prompt_long(new, prior, block):
     check_prompt(prompt_case(len(new), new, prior, block=block))
+
+
+@pytest.mark.parametrize("new,prior,pad", [([32], [500], 4000), ([3, 1000], [7, 0], 4000), ([1, 5], [0, 60], 65530),
+                                           ([128] * 9, [50] * 9, 300)])
+def test_prompt_wide_tables(new, prior, pad):
+    check_prompt(prompt_case(len(new), new, prior, heads=8, kv=4, dim=64, pad=pad), validate=False)
+
+
+def test_prompts_in_graphs_that_share_a_workspace():
+    cases = [prompt_case(11, [100, 17], [400, 0]), prompt_case(12, [1500], [0], heads=8, kv=8)]
+    need = [prefill_weights_workspace_bytes(x[3].numel(), x[0].shape[0], x[0].shape[1], x[1].shape[2], 128, 16, x[4].shape[1])
+            for x in cases]
+    ws = torch.empty(max(need), dtype=torch.uint8, device=DEV)
+    start, want, graphs = [x[7].clone() for x in cases], [], []
+    for x in cases:
+        prefill_attention_weights(*x, validate=False)
+        want.append(x[7].clone())
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            prefill_attention_weights(*x, validate=False, workspace=ws)
+        graphs.append(graph)
+    for _ in range(3):
+        for x, w in zip(cases, start):
+            x[7].copy_(w)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x[7], w) for x, w in zip(cases, want))
+        ws.fill_(255)
 
 
 def test_prompt_rows_that_no_sequence_owns_and_sequences_that_cannot_be():

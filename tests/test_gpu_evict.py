@@ -91,6 +91,11 @@ def test_long_rows_of_few_levels(n):
     check(case(n, [n, n - 1, n // 3], layers=1, kv=1, dim=8, block=1, levels=3), 10, first=[3, 10, 1], recent=9)
 
 
+@pytest.mark.parametrize("pad", [200, 2000, 65000])
+def test_wide_tables(pad):
+    check(case(pad, [300, 50, 120], layers=1, kv=2, dim=16, pad=pad), 100, first=[0, 7, 30], recent=20)
+
+
 def test_strange_weights():
     args = case(1, [300, 300, 300, 300], layers=1, kv=1, dim=8)
     w = args[2]

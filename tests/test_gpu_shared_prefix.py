@@ -136,6 +136,31 @@ def test_offsets_that_cannot_be_leave_sequences_on_their_own():
         check(args, validate=False)
 
 
+@pytest.mark.parametrize("pad", [300, 4000, 65000])
+def test_wide_tables(pad):
+    check(case(30, [400, 333, 320, 500, 41], [(0, 4, 320)], heads=8, kv=4, dim=64, pad=pad))
+
+
+def test_graphs_that_share_a_workspace():
+    cases = [case(31, [900, 850, 1000], [(0, 3, 800)]), case(32, [300 + i for i in range(40)], [(0, 20, 256), (20, 40, 288)])]
+    need = [shared_prefix_workspace_bytes(x[0].shape[0], 16, 8, 128, x[7].numel(), 16, x[3].shape[1], True) for x in cases]
+    ws = torch.empty(max(need), dtype=torch.uint8, device=DEV)
+    want, outs, graphs = [shared(*x) for x in cases], [], []
+    for x in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(shared(*x, validate=False, workspace=ws))
+        graphs.append(graph)
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        for out in outs:
+            out.zero_()
+        ws.fill_(255)
+
+
 def test_no_groups_is_paged_attention():
     args = list(case(8, [1, 128, 129, 4000, 77], []))
     out = check(args)
