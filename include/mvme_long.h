@@ -30,10 +30,12 @@ size_t mvme_paged_attention_shared_prefix_workspace_size(int64_t batch, int64_t 
  * from 0 or more to at most batch; sequences in no group share nothing); the
  * first prefix_lens[g] tokens of all of them are in the same pages and are read
  * once for all, through the table of the group's first sequence that has them
- * all.  Sequences of a group that are shorter than its prefix (the empty ones of
- * a padded batch) are attended through their own tables, as are groups of one
- * and of a prefix that is not positive or passes the tables' capacity.  Offsets that fall, or leave the batch, make
- * all sequences ungrouped.  Every row's result is that of
+ * all (on pages of a multiple of 16 tokens, whole runs of 16 of them: the rest
+ * is read with each sequence's own tokens).  Sequences of a group that are
+ * shorter than its prefix (the empty ones of a padded batch) are attended
+ * through their own tables, as are groups of one and of a prefix that is not
+ * positive or passes the tables' capacity.  Offsets that fall, or leave the
+ * batch, make all sequences ungrouped.  Every row's result is that of
  * mvme_paged_attention, to rounding: scale 1/sqrt(head_dim), zeros for lengths
  * <= 0 or beyond the table's capacity, pages out of range skipped.
  * Calls of few cached tokens (by the tables' capacity) are attended without

@@ -93,13 +93,13 @@ __device__ inline int uniform(int v) { return __builtin_amdgcn_readfirstlane(v);
 struct Group {
     int first, rows;     // sequences
     int prefix;          // tokens; 0: nothing is shared
-    bool wide;
+    bool wide;           // (units take prefix_taken() of them)
     int rounds, tiles;   // of a unit, and units
 };
 // What a lane holds of a sequence.
 struct Own {
     int len;             // 0 where the length cannot be
-    int start;           // where its own keys begin: behind its group's prefix, if it reaches to the end of that
+    int start;           // where its own keys begin: behind what its group's units take, if it has the whole prefix
     __device__ inline int rounds() const { return (len - start + kRound - 1) / kRound; }
 };
 
@@ -115,13 +115,19 @@ struct Walk {
 
     __device__ static inline int64_t capacity(const Args& a) { return (int64_t)a.width * a.div.size; }
 
+    // How much of a prefix a group's units take.  Where pages are looked up once for 16 tokens (RUN 16) these have to lie in
+    // one page, so that every segment, a sequence's own too, has to begin at a multiple of 16: the rest of the prefix is
+    // among each sequence's own keys.
+    __device__ static inline int prefix_taken(const Args& a, int prefix) { return a.div.size % 16 == 0 ? prefix & ~15 : prefix; }
+
     __device__ static inline Group group_from(const Args& a, int64_t first, int64_t next, int64_t prefix) {
         Group x{(int)first, (int)(next - first), 0, false, 0, 0};
         // (One row alone gains nothing, and needs no unit for it.)
-        x.prefix = x.rows >= 2 && prefix > 0 && prefix <= capacity(a) ? (int)prefix : 0;
+        const int taken = x.rows >= 2 && prefix > 0 && prefix <= capacity(a) ? prefix_taken(a, (int)prefix) : 0;
+        x.prefix = taken ? (int)prefix : 0;
         const int64_t rows = (int64_t)x.rows * a.group;
         x.wide = rows > kNarrowRows;
-        x.rounds = (x.prefix + kRound - 1) / kRound;
+        x.rounds = (taken + kRound - 1) / kRound;
         x.tiles = x.prefix ? (int)(x.wide ? (rows + kWideRows - 1) / kWideRows : (rows + kColumns - 1) / kColumns) : 0;
         return x;
     }
@@ -169,7 +175,8 @@ struct Walk {
         Own x{length_from(a, length), 0};
         int g;
         const int prefix = prefix_of(a, seq, g);
-        x.start = prefix <= x.len ? prefix : 0;
+        // (By the whole prefix: who has less of it need not have even the beginning in the same pages.)
+        x.start = prefix <= x.len ? prefix_taken(a, prefix) : 0;
         return x;
     }
     __device__ static inline int64_t load_length(const Args& a, int seq) { return seq < a.batch ? a.lens[seq] : 0; }
@@ -312,7 +319,7 @@ __device__ inline Segment find_segment(const Args& a, const Walk& w, int wg, int
         rounds = max(x.rounds, 1);
         s.tile = (q - base) / rounds;
         from = q - base - s.tile * rounds;
-        tokens = x.prefix;
+        tokens = Walk::prefix_taken(a, x.prefix);
         s.seq = w.reader_of(a, x);
         s.first_row = x.first;
         s.rows = x.rows * a.group - s.tile * (s.wide ? kWideRows : kColumns);

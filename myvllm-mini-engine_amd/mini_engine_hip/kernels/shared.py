@@ -74,8 +74,9 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, c
     and lengths), and so are the results, to rounding.  Sequences
     ``group_offsets[g] .. group_offsets[g + 1] - 1`` (int64 [groups + 1], rising;
     what is in no group shares nothing) hold their first ``prefix_lens[g]``
-    tokens (int64 [groups]) in the same pages.  A sequence shorter than its
-    group's prefix (an empty one of a padded batch) is attended on its own.
+    tokens (int64 [groups]; any number, whether or not a page ends there) in the
+    same pages.  A sequence shorter than its group's prefix (an empty one of a
+    padded batch) is attended on its own.
     Calls of few cached tokens run ``paged_attention``'s kernels, which are
     ahead there, unless ``always_share``.  ``validate=True`` reads the metadata
     on the host, and refuses groups whose pages differ; with ``validate=False``
