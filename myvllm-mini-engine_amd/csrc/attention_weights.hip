@@ -139,6 +139,12 @@ bool whole(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t capacity) {
     return capacity <= 512 || batch * kv_heads >= 128;
 }
 
+// Whether one launch holds the join's work-groups: one per sequence and kv head, and one for each kAddKeys keys of theirs.
+int64_t add_blocks(int64_t block_size, int64_t width) { return (block_size * width - 1) / kAddKeys + 1; }
+bool fits_launch(int64_t batch, int64_t kv_heads, int64_t block_size, int64_t width) {
+    return batch * kv_heads <= kMostThreads / kThreads / (1 + add_blocks(block_size, width));
+}
+
 struct Sizes {
     int64_t shares, slots, score_row;
     int64_t floats;
@@ -192,7 +198,9 @@ using namespace mvme::lng;
 extern "C" size_t mvme_paged_attention_weights_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                               int64_t head_dim, int64_t block_size, int64_t table_width) {
     Args a{};
-    if (check_shape(a, batch, q_heads, kv_heads, head_dim, 1, block_size, table_width, MVME_FP16)) return 0;
+    if (check_shape(a, batch, q_heads, kv_heads, head_dim, 1, block_size, table_width, MVME_FP16) ||
+        !fits_launch(batch, kv_heads, block_size, table_width))
+        return 0;
     return (size_t)sizes(batch, q_heads, kv_heads, head_dim, block_size, table_width).floats * sizeof(float);
 }
 
@@ -211,8 +219,8 @@ extern "C" int mvme_paged_attention_weights(void* out, const void* query, const 
         !fp4::aligned(weights, 4))
         return fail(MVME_EINVAL, "weighted attention: queries and caches must be 16-byte, the output 8-byte aligned");
     const Sizes s = sizes(batch, q_heads, kv_heads, head_dim, block_size, table_width);
-    const int64_t blocks = (block_size * table_width - 1) / kAddKeys + 1;
-    if (batch * kv_heads > kMostThreads / kThreads / (1 + blocks)) return fail(MVME_EINVAL, "batch/head product too large");
+    const int64_t blocks = add_blocks(block_size, table_width);
+    if (!fits_launch(batch, kv_heads, block_size, table_width)) return fail(MVME_EINVAL, "batch/head product too large");
     if (s.floats > 0 && (!workspace || workspace_bytes < (size_t)s.floats * sizeof(float) || !fp4::aligned(workspace, 16)))
         return fail(MVME_EWORKSPACE, "weighted attention workspace too small: " + std::to_string(s.floats * 4) +
                                          " bytes, 16-byte aligned, are needed");

@@ -493,6 +493,11 @@ bool prompt_shape(int64_t num_seqs, int64_t total, int64_t q_heads, int64_t kv_h
            head_dim_built(head_dim) && block_size > 0 && block_size <= kMaxCapacity && width > 0 &&
            width <= kMaxCapacity / block_size && q_heads <= 2147483647 / head_dim && total <= 2147483647 / q_heads;
 }
+bool row_fits(int64_t kv_heads, int64_t head_dim) { return kv_heads * head_dim * 2 <= 65536 * 16; }
+bool fits_launch(const Plan& p, int64_t num_seqs, int64_t kv_heads) {
+    return p.items <= kMostThreads / kThreads / kv_heads / p.chunks &&
+           num_seqs <= kMostThreads / kThreads / kv_heads / p.key_blocks / p.parts;
+}
 
 }  // namespace
 }  // namespace lng
@@ -504,9 +509,11 @@ using namespace mvme::lng;
 extern "C" size_t mvme_prefill_attention_weights_workspace_size(int64_t num_seqs, int64_t total_tokens, int64_t q_heads,
                                                                 int64_t kv_heads, int64_t head_dim, int64_t block_size,
                                                                 int64_t table_width) {
-    if (!prompt_shape(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width)) return 0;
+    if (!prompt_shape(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width) ||
+        !row_fits(kv_heads, head_dim) || total_tokens == 0)
+        return 0;
     const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, block_size, table_width);
-    return p.floats * sizeof(float);
+    return fits_launch(p, num_seqs, kv_heads) ? p.floats * sizeof(float) : 0;
 }
 
 extern "C" int mvme_prefill_attention_weights(const void* q, const void* key_cache, const int64_t* cu_seqlens_q,
@@ -527,7 +534,7 @@ extern "C" int mvme_prefill_attention_weights(const void* q, const void* key_cac
     if (!prompt_shape(num_seqs, total_tokens, q_heads, kv_heads, head_dim, block_size, table_width))
         return fail(MVME_EINVAL, "too many packed query rows");
     const int64_t row = kv_heads * head_dim * 2;
-    if (row > 65536 * 16 || num_blocks > 2147483647 || num_blocks > (int64_t(1) << 62) / row / block_size)
+    if (!row_fits(kv_heads, head_dim) || num_blocks > 2147483647 || num_blocks > (int64_t(1) << 62) / row / block_size)
         return fail(MVME_EINVAL, "KV cache too large");
     if (weight_row < block_size * table_width) return fail(MVME_EINVAL, "weight rows must hold the tables' capacity");
     if (total_tokens == 0) return MVME_OK;
@@ -536,10 +543,8 @@ extern "C" int mvme_prefill_attention_weights(const void* q, const void* key_cac
     if (!fp4::aligned(q, 16) || !fp4::aligned(key_cache, 16) || !fp4::aligned(weights, 4))
         return fail(MVME_EINVAL, "prompt weights: queries and caches must be 16-byte aligned");
     const Plan p = plan(num_seqs, total_tokens, q_heads, kv_heads, block_size, table_width);
-    if (p.items > kMostThreads / kThreads / kv_heads / p.chunks || num_seqs > kMostThreads / kThreads / kv_heads / p.key_blocks / p.parts)
-        return fail(MVME_EINVAL, "too many packed query rows");
-    const size_t need = mvme_prefill_attention_weights_workspace_size(num_seqs, total_tokens, q_heads, kv_heads, head_dim,
-                                                                      block_size, table_width);
+    if (!fits_launch(p, num_seqs, kv_heads)) return fail(MVME_EINVAL, "too many packed query rows");
+    const size_t need = p.floats * sizeof(float);
     if (!workspace || workspace_bytes < need || !fp4::aligned(workspace, 16))
         return fail(MVME_EWORKSPACE, "prompt weights workspace too small: " + std::to_string(need) +
                                          " bytes, 16-byte aligned, are needed");
