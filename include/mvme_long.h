@@ -114,9 +114,11 @@ int mvme_prefill_attention_weights(const void* q, const void* key_cache, const i
  * positions 0 .. keep - 1 of the sequence's pages, in place; rows behind these
  * keep what they held.  kept[l, b, hk, i] is the position that row i came
  * from, -1 behind the last; new_weights its weight, 0 behind the last;
- * new_lens[b] = min(n, keep).  A sequence whose length is not positive or
- * passes the tables' capacity keeps its length and nothing of it moves.  Rows
- * from or to a page out of range are not moved.
+ * new_lens[b] = min(n, keep).  A sequence whose length is not positive (an
+ * empty one of a padded batch) or passes the tables' capacity keeps its length
+ * and nothing of it moves; nothing of it is kept, so that its new_weights are 0
+ * and its kept -1: whoever needs its weights again has them in `weights`, which
+ * stay as they were.  Rows from or to a page out of range are not moved.
  *   key_cache, value_cache  [layers, num_blocks, block_size, kv_heads, head_dim],
  *                           head_dim a multiple of 8 up to 1024
  *   weights, new_weights    fp32 [layers, batch, kv_heads, weight_row], not

@@ -62,7 +62,9 @@ def evict_kv_cache(key_cache, value_cache, weights, block_tables, context_lens, 
     pages that cannot be, and rows that would move into a page that another
     sequence of the batch holds too (protect shared prefixes with ``first``, or
     ``PagePool.make_writable`` them).  With ``validate=False`` (graph capture)
-    the caller answers for that; lengths that cannot be are left alone.
+    the caller answers for that; a sequence whose length cannot be (0: an empty
+    row of a padded batch) keeps its length and its rows, and its line of the new
+    weights is zero (``weights`` itself never changes).
     """
     if backend != "hip":
         raise ValueError("eviction backend must be hip")
