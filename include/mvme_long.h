@@ -44,7 +44,10 @@ size_t mvme_paged_attention_shared_prefix_workspace_size(int64_t batch, int64_t 
  * shared scores, softmax statistics and
  * accumulators are fp32; for the value product the probabilities are rounded to
  * the inputs' type where a prefix has more than 32 query rows, and to the sum
- * of two numbers of it elsewhere.
+ * of two numbers of it elsewhere.  In fp16 they are finite while scores (times
+ * log2 e) are below 2^24 in magnitude, and in prefixes of more than 32 rows
+ * those below 2^-33 of the largest may be zero, which makes an infinite value
+ * NaN there.
  */
 int mvme_paged_attention_shared_prefix(void* out, const void* query, const void* key_cache, const void* value_cache,
                                        const int64_t* block_tables, const int64_t* context_lens,

@@ -9,7 +9,9 @@
 // 4 of 128: 537 MB of caches and 34 MB of scores each way in 119 us (104 in
 // the walk, 5.1 TB/s, and 16 in the join); the stores of scores are 17 to 22 of
 // the walk's.  Sequences whose scores fit a work-group's LDS are taken whole, with
-// no second kernel: 32 ragged ones of up to 4096 tokens 65 us, 5.0 TB/s.
+// no second kernel, and the longest one's work-group ends last: 32 ragged ones of
+// up to 4096 tokens take 64 us, the same tokens in 32 of one length 48.5 (5.6
+// TB/s), 4096 in each 90 (6.0 TB/s), and one of 4096 among 31 of 64 alone 48.7.
 #include "../../include/mvme_long.h"
 #include "long_attention.h"
 

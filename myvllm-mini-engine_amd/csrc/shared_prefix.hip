@@ -9,11 +9,16 @@
 //
 // Bounds: with few rows per key the reads (16 sequences over 1024 shared
 // tokens and 64 in all, 401 MB: 77 us, of which the join is 5; 5.5 TB/s in
-// the walk), with many the matrix and vector units in turn (128 sequences, 32
-// heads on 8, over 16384 tokens: 82 us, 30 of them matrix products at the
-// card's rate).  There a wave's tile of 32 rows and 64 keys of 128 dims is, by
-// count, 1024 cycles of matrix products and about 900 of vector work, half of
-// that exponentials; two waves a SIMD overlap them in part.  128 rows a
+// the walk), with many the wide loop.  128 sequences, 32 heads on 8, over 16384
+// tokens and up to 400 of their own take 82 us, and 72 with one token of their
+// own.  Of these the prefix's keys are 45 (what 32768 more of them add, halved;
+// 764 TFLOP/s, and 30 us at the rate of a large matrix product); the other 27
+// do not grow with them: the join (10), two launches, what begins and ends a
+// segment, and those last tokens.  In the loop a wave's tile of 32 rows and 64
+// keys of 128 dims takes a SIMD about 3400 cycles (at 2.4 GHz).  By count 1024
+// are matrix products and about 900 vector work, half of that exponentials, and
+// the work-group's four tiles keep the LDS busy for 1250: all three in turn
+// rather than at once, though two waves a SIMD could overlap them.  128 rows a
 // work-group are what two work-groups' registers and LDS allow; three per
 // compute unit, or the next tile's scores beside this one's softmax, spill or
 // were slower (88 against 85).
@@ -178,8 +183,11 @@ __device__ inline void wide_segment(const Args& a, const Segment& seg, WideLds<D
 #pragma unroll
             for (int n = 0; n < S::kBlocks; ++n) acc[n] *= by;
         }
-        // Weights are rounded to the inputs' type for the value product; the sum that divides is of the rounded ones, so
-        // that what a rounding adds it adds to both.
+        // Weights are rounded to the inputs' type for the value product, which is half of the matrix products here; the sum
+        // that divides is of the rounded ones, so that what a rounding adds it adds to both.  As sums of two numbers, as
+        // narrow units have them, 128 sequences over 16384 tokens take 98 us instead of 82, 20 over 4096 (16 heads) 24.8
+        // instead of 22.0.  Errors against 64 bits then equal those of fp32 weights, 0.00166 (bf16, the output's rounding)
+        // and 0.000207 (fp16); so they are 0.0023 and 0.00029.
         constexpr uint32_t kOnes = T::kId == MVME_FP16 ? 0x3c003c00u : 0x3f803f80u;
         u32x4 weights[4];
 #pragma unroll

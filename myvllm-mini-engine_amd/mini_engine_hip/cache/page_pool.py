@@ -118,7 +118,8 @@ class PagePool:
     def truncate(self, request_id: str, token_count: int) -> list[int]:
         """Give back the pages of a request behind its first ``token_count`` tokens (after an eviction).
 
-        Returns its table.
+        Returns its table.  Where that now ends inside a page that others hold
+        too, ``make_writable`` comes before the next token's write.
         """
         table = self._owned[request_id]
         if not 0 <= token_count <= len(table) * self.block_size:

@@ -78,7 +78,10 @@ def paged_attention_shared_prefix(query, key_cache, value_cache, block_tables, c
     same pages.  A sequence shorter than its group's prefix (an empty one of a
     padded batch) is attended on its own.
     Calls of few cached tokens run ``paged_attention``'s kernels, which are
-    ahead there, unless ``always_share``.  ``validate=True`` reads the metadata
+    ahead there, unless ``always_share``; a large batch most of which shares
+    nothing is about as fast with ``paged_attention`` itself.  Groups of more
+    than 32 query rows per kv head round the probabilities to the inputs' type
+    before they meet the values.  ``validate=True`` reads the metadata
     on the host, and refuses groups whose pages differ; with ``validate=False``
     (graph capture) the caller answers for that, lengths and pages that cannot
     be are absent, and offsets that cannot be leave every sequence on its own.
