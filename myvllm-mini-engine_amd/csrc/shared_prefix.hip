@@ -10,15 +10,15 @@
 // Bounds: with few rows per key the reads (16 sequences over 1024 shared
 // tokens and 64 in all, 401 MB: 77 us, of which the join is 5; 5.5 TB/s in
 // the walk), with many the wide loop.  128 sequences, 32 heads on 8, over 16384
-// tokens and up to 400 of their own take 82 us, and 72 with one token of their
+// tokens and up to 400 of their own take 82.6 us, and 72 with one token of their
 // own.  Of these the prefix's keys are 45 (what 32768 more of them add, halved;
 // 764 TFLOP/s, and 30 us at the rate of a large matrix product); the other 27
 // do not grow with them: the join (10), two launches, what begins and ends a
 // segment, and those last tokens.  In the loop a wave's tile of 32 rows and 64
 // keys of 128 dims takes a SIMD about 3400 cycles (at 2.4 GHz).  By count 1024
 // are matrix products and about 900 vector work, half of that exponentials, and
-// the work-group's four tiles keep the LDS busy for 1250: all three in turn
-// rather than at once, though two waves a SIMD could overlap them.  128 rows a
+// the work-group's four tiles keep the LDS busy for 1250: together about what a
+// tile takes, so little of it overlaps between the two waves of a SIMD.  128 rows a
 // work-group are what two work-groups' registers and LDS allow; three per
 // compute unit, or the next tile's scores beside this one's softmax, spill or
 // were slower (88 against 85).
